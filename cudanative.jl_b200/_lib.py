@@ -17,6 +17,7 @@ F16, F32, BF16 = 0, 1, 2
 MATRIX_A, MATRIX_B, ACCUMULATOR = 0, 1, 2
 LOWER_WARP, LOWER_TCGEN05 = 0, 1
 KERNEL_AUTO, KERNEL_TCGEN05, KERNEL_SIMPLE = 0, 1, 2
+STATUS_BAD_OFFSETS = 110  # device status word: a grouped product's offsets decrease or leave the matrix
 (OPT_FORCE_KERNEL, OPT_MAX_CTAS, OPT_WAIT_BUDGET_NS, OPT_TILE_N, OPT_SPLIT_K, OPT_CTA_PAIR,
  OPT_RASTER_GROUP, OPT_CHECK_ON_CALL, OPT_PDL, OPT_F16_ACCUMULATE) = range(10)
 SHARDED_GATED, SHARDED_NO_TRANSFER, SHARDED_NO_COMPUTE = 1, 2, 4
@@ -45,6 +46,9 @@ SIGNATURES = {
     "b200_gemm_ex": (_i, [_p, _p, _i, _i, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i, _f, _p, _i64, _i, _p, _i64, _i]),
     "b200_gemm_strided_batched": (_i, [_p, _p, _i, _i, _i64, _i64, _i64, _f, _p, _i64, _i64, _p, _i64, _i64, _i, _f, _p, _i64,
                                        _i64, _i, _p, _i64, _i64, _i, _i64]),
+    "b200_gemm_grouped": (_i, [_p, _p, _i, _i64, _i64, _i64, _f, _p, _i64, _i64, _p, _i64, _i, _f, _p, _i64, _i, _p, _i64, _i, _p, _i64]),
+    "b200_gemm_grouped_k": (_i, [_p, _p, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i, _f, _p, _i64, _i64, _i, _p, _i64, _i64, _i, _p,
+                                 _i64]),
     "b200_gemm_f16f32_gated": (_i, [_p, _p, _i, _i, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _f, _p, _i64, _p, _i64, _p, _i64]),
     "b200_stream_write_u32": (_i, [_p, _p, C.c_uint32]),
     "b200_stream_wait_u32": (_i, [_p, _p, C.c_uint32]),

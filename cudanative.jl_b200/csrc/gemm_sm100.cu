@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "tensor_map.h"
 
 namespace b200 {
 namespace {
@@ -28,14 +29,6 @@ EncodeFn get_encode_fn() {
     return fn;
 }
 
-// Matrices of one launch: how many and how far apart (elements); count == 0 asks for a 2-D map.
-struct BatchDim {
-    int64_t count = 0;
-    int64_t stride = 0;
-};
-
-// Tensor map over a column-major matrix: dim0 (contiguous) has `inner` elements, dim1 has `outer`
-// elements `ld` elements apart; batched problems add dim2 = matrix of the batch (box extent 1).
 // A tensor map is a pure function of the arguments below (it describes addresses and shapes, not
 // contents), so repeated launches on the same buffers reuse it: a small per-thread cache, most
 // recently used first.  Matters for launch-bound sizes only.
@@ -83,9 +76,11 @@ struct MapCache {
 };
 thread_local MapCache g_map_cache;
 
+}  // namespace
+
 int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
                 int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
-                const char* what, BatchDim batch = BatchDim()) {
+                const char* what, BatchDim batch) {
     const MapKey mk{base, inner, outer, ld, batch.count, batch.stride, box_inner, box_outer, static_cast<int>(dt), static_cast<int>(sw)};
     if (const CUtensorMap* hit = g_map_cache.find(mk)) {
         *tm = *hit;
@@ -107,6 +102,8 @@ int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const v
     g_map_cache.insert(mk, *tm);
     return B200_OK;
 }
+
+namespace {
 
 // The opt-in to more than 48 KiB of dynamic shared memory is per device and per kernel: made once
 // (this also makes the driver load the kernel, which a caller may want to have happen at start-up).
@@ -272,10 +269,6 @@ int gemm_tcgen05_launch(const GemmProblem& g, const GemmPlan& plan, float* scrat
             b.stride = stride;
         }
         return b;
-    };
-    auto map_type = [](int type) {
-        return type == B200_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                : (type == B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
     };
     const CUtensorMapDataType ab_dt = map_type(g.ab_type);
 

@@ -111,6 +111,9 @@ namespace b200 {
 // Validate, pick a kernel and enqueue one GEMM on `stream` (the body of every GEMM entry point).
 int gemm_dispatch(b200_handle* h, cudaStream_t stream, const GemmProblem& g);
 int check_current_device(const b200_handle* h);
+// B200_OPT_CHECK_ON_CALL around a launch: look at the failure word of the previous one, note this one.
+int poll_previous_launch(b200_handle* h);
+int note_launch(b200_handle* h, cudaStream_t stream);
 // Copies the handle's 4-int device status word to `word` (synchronous) and clears it when non-zero.
 int read_status(b200_handle* h, int* word);
 

@@ -107,7 +107,9 @@ enum : int {
     kWaitCTile = 105,        // epilogue waiting for its C chunk
     kWaitUnit = 106,         // 16x16x16 unit waiting for its MMA
     kWaitSelftest = 107,     // the bounded-wait self test (nothing ever arrives)
-    kWaitPanel = 108         // producer waiting for a panel of A to arrive in this GPU's memory
+    kWaitPanel = 108,        // producer waiting for a panel of A to arrive in this GPU's memory
+    kWaitTail = 109,         // grouped product: the last k-block of a group, zeros behind its end
+    kBadOffsets = 110        // not a wait: a group's offsets decrease or leave the matrix
 };
 
 // What a kernel needs to give up on a wait cleanly.

@@ -118,6 +118,27 @@ class Handle:
             stride_b, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type), d, ldd, stride_d,
             _type_code(d_type), batch), "gemm_strided_batched")
 
+    def gemm_grouped(self, transA: bool, M: int, N: int, K: int, alpha: float, A, lda: int, stride_a: int, B, ldb: int, ab_type,
+                     beta: float, Cm, ldc: int, c_type, D, ldd: int, d_type, offsets, groups: int, stream=None) -> None:
+        """``D[:, s_e] = alpha*op(A_e)*B[:, s_e] + beta*C[:, s_e]`` for the columns ``s_e`` of every group, whose
+        borders are ``groups + 1`` int32 on the device (b200_gemm_grouped): a layer with one weight matrix per
+        group (transA) or the gradient of its input."""
+        a, b, d = _addr(A), _addr(B), _addr(D)
+        c = _addr(Cm) if Cm is not None else None
+        _lib.check(_lib.lib().b200_gemm_grouped(
+            self._h, stream, int(bool(transA)), M, N, K, float(alpha), a, lda, stride_a, b, ldb, _type_code(ab_type), float(beta), c,
+            ldc, _type_code(c_type), d, ldd, _type_code(d_type), _addr(offsets), groups), "gemm_grouped")
+
+    def gemm_grouped_k(self, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int, ab_type, beta: float, Cm, ldc: int,
+                       stride_c: int, c_type, D, ldd: int, stride_d: int, d_type, offsets, groups: int, stream=None) -> None:
+        """``D_e = alpha*A[:, s_e]*B[:, s_e]^T + beta*C_e`` (b200_gemm_grouped_k): the gradient of the groups'
+        matrices; an empty group gives ``beta*C_e``."""
+        a, b, d = _addr(A), _addr(B), _addr(D)
+        c = _addr(Cm) if Cm is not None else None
+        _lib.check(_lib.lib().b200_gemm_grouped_k(
+            self._h, stream, M, N, K, float(alpha), a, lda, b, ldb, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type),
+            d, ldd, stride_d, _type_code(d_type), _addr(offsets), groups), "gemm_grouped_k")
+
     def gemm_gated(self, transA: bool, transB: bool, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int,
                    beta: float, Cm, ldc: int, D, ldd: int, panel_flags, panel_k: int, stream=None) -> None:
         """``gemm`` whose main loop reads columns [j*panel_k, (j+1)*panel_k) of op(A) only once the

@@ -193,6 +193,37 @@ int b200_gemm_strided_batched(b200_handle* h, b200_stream stream, int transA, in
                               int64_t ldc, int64_t stride_c, int c_type, void* D, int64_t ldd,
                               int64_t stride_d, int d_type, int64_t batch);
 
+/* Products of one operand with the matrices of several groups, where every group owns a run of
+ * columns whose length is known on the device only (the tokens of an expert after routing):
+ *     D[:, s_e] = alpha * op(A_e) * B[:, s_e] + beta * C[:, s_e],  s_e = [offsets[e], offsets[e + 1])
+ * for e < groups.  op(A_e) is M x K, A_e = A + e * stride_a elements (stride_a = 0: one matrix for all
+ * groups); B is K x N, C and D are M x N, column-major.  Stored row by row, as [tokens, features] and
+ * one [out, in] weight per group, transA = 1 is the forward product and transA = 0 (with M and K
+ * exchanged) the gradient of its input.
+ *   offsets: groups + 1 ascending 32-bit integers in DEVICE memory with 0 <= offsets[0] and
+ *   offsets[groups] <= N; equal neighbours are an empty group.  Read by the kernel, never by the host.
+ *   Columns that belong to no group are not written.  Offsets that decrease or leave [0, N] write
+ *   nothing and put id 110 into the device status word (b200_device_status).
+ *   groups <= 1024.  Types as in b200_gemm_ex; a column's result does not depend on its neighbours'
+ *   values.  D may alias C exactly (same pointer, ld and type).
+ * The tcgen05 kernel needs 16-byte aligned A and B, lda, ldb and stride_a multiples of 8 elements and
+ * stride_a at least one matrix (or 0); anything else runs on the simple kernel.  C and D may have any
+ * alignment.  The split-K option is ignored. */
+int b200_gemm_grouped(b200_handle* h, b200_stream stream, int transA, int64_t M, int64_t N, int64_t K,
+                      float alpha, const void* A, int64_t lda, int64_t stride_a, const void* B,
+                      int64_t ldb, int ab_type, float beta, const void* C, int64_t ldc, int c_type,
+                      void* D, int64_t ldd, int d_type, const int32_t* offsets, int64_t groups);
+
+/* The other ragged dimension, the gradient of the groups' matrices:
+ *     D_e = alpha * A[:, s_e] * B[:, s_e]^T + beta * C_e,   D_e = D + e * stride_d,  e < groups
+ * A is M x K, B is N x K (both column-major, one column per token), C_e and D_e are M x N.  An empty
+ * group gives D_e = beta * C_e (zeros for beta = 0).  Offsets, groups, types and alignment as above, K
+ * in the place of N; columns of A and B outside s_e, NaN and infinities among them, do not reach D_e. */
+int b200_gemm_grouped_k(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha,
+                        const void* A, int64_t lda, const void* B, int64_t ldb, int ab_type, float beta,
+                        const void* C, int64_t ldc, int64_t stride_c, int c_type, void* D, int64_t ldd,
+                        int64_t stride_d, int d_type, const int32_t* offsets, int64_t groups);
+
 /* b200_gemm_f16f32 whose main loop may start before all of A is in this GPU's memory: columns
  * [j*panel_k, (j+1)*panel_k) of op(A) are read only once the 32-bit word panel_flags[j] (device
  * memory) is non-zero.  panel_k is a multiple of 64; at most 32 panels.  The words are meant to

@@ -1,0 +1,300 @@
+"""Grouped products through the C ABI (b200_gemm_grouped, b200_gemm_grouped_k) against float64."""
+import numpy as np
+import pytest
+
+from cudanative_jl_b200 import _lib
+from cudanative_jl_b200.array import Array, CuArray, pointer
+from cudanative_jl_b200.bfloat16 import BFloat16
+from grouped_cases import close, grouped_k_ref, grouped_ref, memory_type, offsets_of, store, value
+
+pytestmark = pytest.mark.gpu
+
+F16, F32 = np.float16, np.float32
+
+
+def sync(handle, expect=0):
+    _lib.check(_lib.lib().b200_stream_sync(None), "sync")
+    code, block, detail = handle.device_status()
+    assert code == expect, f"device status {code} (block {block}, detail {detail})"
+
+
+def normal(r, shape, scale=1.0):
+    return r.standard_normal(shape).astype(np.float32) * np.float32(scale)
+
+
+def taller(x, ld, fill):
+    """Column-major x with leading dimension ld; what is between its columns holds `fill`."""
+    out = np.full((ld, x.shape[1]), fill, dtype=x.dtype, order="F")
+    out[: x.shape[0]] = x
+    return out
+
+
+def fill_of(elem, v):
+    return store(np.array([[v]]), elem)[0, 0]
+
+
+def run_grouped(handle, sizes, M, K, *, transA=True, ab=BFloat16, d_type=None, c_type=F32, alpha=1.0, beta=0.0, start=0, tail=0, pad=0, one_a=False,
+                alias=False, expect=None, seed=0, poison=True, shift=0, **options):
+    """One call against the statement; what lies outside a group's columns of B is NaN and of D a sentinel."""
+    d_type = ab if d_type is None else d_type
+    r = np.random.default_rng(seed)
+    off = offsets_of(sizes, start)
+    N = int(off[-1]) + tail
+    E = len(sizes)
+    shape = (K, M) if transA else (M, K)
+    A = [store(normal(r, shape, K ** -0.5 if K else 1.0), ab) for _ in range(1 if one_a else E)]
+    B = store(normal(r, (K, N)), ab)
+    if poison:
+        B[:, :start] = fill_of(ab, np.nan)
+        B[:, int(off[-1]):] = fill_of(ab, np.inf)
+    Cm = store(normal(r, (M, N)), c_type) if beta else None
+    sentinel = np.float32(-7.25)
+    D0 = Cm.copy(order="F") if alias else store(np.full((M, N), sentinel), d_type)
+    lda, ldb, ldd = max(shape[0] + pad, 1), K + pad, M + pad
+    nan = fill_of(ab, np.nan)
+    a_host = np.concatenate([taller(a, lda, nan).ravel("F") for a in A if a.size]) if K else np.zeros(8, memory_type(ab))
+    a_dev = CuArray(np.concatenate([np.full(shift, nan, memory_type(ab)), a_host]))
+    b_dev = CuArray(taller(B, max(ldb, 1), nan))
+    d_dev = CuArray(taller(D0, ldd, fill_of(d_type, sentinel)))
+    c_dev = d_dev if alias else CuArray(taller(Cm, ldd, fill_of(c_type, np.nan))) if beta else None
+    for k in ("FORCE_KERNEL", "TILE_N", "CTA_PAIR"):
+        handle.set_option(getattr(_lib, "OPT_" + k), options.get(k.lower(), 0))
+    handle.gemm_grouped(transA, M, N, K, alpha, pointer(a_dev) + shift, lda, 0 if one_a else lda * shape[1], b_dev, max(ldb, 1), ab, beta, c_dev,
+                        ldd, c_type, d_dev, ldd, d_type, CuArray(off), E)
+    sync(handle)
+    if expect is not None:
+        assert handle.last_launch()["kernel"] == expect
+    got = Array(d_dev)
+    assert np.all(value(got[M:], d_type) == sentinel), "rows between the columns of D were written"
+    a64 = [value(a, ab) for a in (A * E if one_a else A)]
+    exact, S = grouped_ref(a64, value(B, ab), value(Cm, c_type) if beta else None, off, alpha, beta, transA, value(D0, d_type))
+    got = value(got[:M], d_type)
+    outside = np.ones(N, bool)
+    outside[int(off[0]):int(off[-1])] = False
+    assert np.array_equal(got[:, outside], value(D0, d_type)[:, outside]), "columns of no group were written"
+    close(got, exact, S, K, d_type, f"sizes {sizes} M {M} K {K}")
+
+
+SIZES = [[1], [0, 1, 0], [5, 0, 17, 33, 0], [31, 32, 33, 1], [64, 65, 127, 3], [128, 129, 200], [256, 300, 1, 255], [0, 0], [700]]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=str)
+@pytest.mark.parametrize("transA", [True, False])
+def test_sizes(handle, sizes, transA):
+    run_grouped(handle, sizes, 264, 200, transA=transA, expect=_lib.KERNEL_TCGEN05, start=3, tail=5)
+
+
+@pytest.mark.parametrize("tile_n,cta_pair", [(64, 1), (128, 1), (128, 2), (256, 2)])
+@pytest.mark.parametrize("transA", [True, False])
+def test_every_tile_shape(handle, tile_n, cta_pair, transA):
+    run_grouped(handle, [3, 0, 70, 300, 257, 31], 392, 136, transA=transA, tile_n=tile_n, cta_pair=cta_pair, force_kernel=_lib.KERNEL_TCGEN05, tail=9)
+
+
+@pytest.mark.parametrize("ab", [F16, BFloat16])
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+@pytest.mark.parametrize("c_type", [None, F16, BFloat16, F32])
+def test_types(handle, ab, d_type, c_type):
+    for sizes in ([40, 3, 90], [260, 0, 41]):
+        run_grouped(handle, sizes, 136, 72, ab=ab, d_type=d_type, c_type=c_type or F32, beta=0.5 if c_type else 0.0, alpha=-1.5, tail=2)
+
+
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 63, 127, 129, 255, 257, 260])
+@pytest.mark.parametrize("d_type", [BFloat16, F32])
+def test_any_number_of_rows(handle, M, d_type):
+    """A stored row by row: M has no alignment rule at all; bulk stores need whole 16-byte chunks, other rows
+    are stored one by one."""
+    run_grouped(handle, [50, 140, 0, 9], M, 64, d_type=d_type, expect=_lib.KERNEL_TCGEN05)
+
+
+@pytest.mark.parametrize("K", [0, 1, 8, 15, 16, 24, 63, 64, 65, 128, 513])
+@pytest.mark.parametrize("transA", [True, False])
+def test_any_k(handle, K, transA):
+    run_grouped(handle, [20, 130], 72, K, transA=transA, beta=1.0, c_type=F32)
+
+
+@pytest.mark.parametrize("transA", [True, False])
+def test_unaligned_runs_on_the_simple_kernel(handle, transA):
+    run_grouped(handle, [9, 0, 70, 1], 70, 33, transA=transA, pad=1, expect=_lib.KERNEL_SIMPLE, beta=0.25, tail=3, start=2)
+    run_grouped(handle, [9, 0, 70, 1], 72, 40, transA=transA, shift=1, expect=_lib.KERNEL_SIMPLE, tail=3, start=2)
+    run_grouped(handle, [9, 0, 70, 1], 72, 40, transA=transA, force_kernel=_lib.KERNEL_SIMPLE, expect=_lib.KERNEL_SIMPLE)
+
+
+def test_one_matrix_for_all_groups_and_in_place(handle):
+    run_grouped(handle, [9, 0, 70, 140], 264, 136, one_a=True)
+    run_grouped(handle, [9, 0, 70, 140], 264, 136, beta=1.0, c_type=F32, d_type=F32, alias=True, tail=4)
+    run_grouped(handle, [9, 0, 70, 140], 264, 136, beta=1.0, c_type=BFloat16, d_type=BFloat16, alias=True, pad=8)
+
+
+@pytest.mark.parametrize("groups", [255, 256, 257, 1000, 1024])
+def test_many_groups(handle, groups):
+    r = np.random.default_rng(groups)
+    sizes = r.integers(0, 4, groups).tolist()
+    run_grouped(handle, sizes, 72, 64, start=1, tail=1)
+    run_grouped(handle, [0] * (groups - 1) + [2], 72, 64)
+    run_grouped(handle, [2] + [0] * (groups - 1), 72, 64)
+    run_grouped(handle, sizes, 70, 33, force_kernel=_lib.KERNEL_SIMPLE)
+
+
+def test_a_neighbours_nan_stays_its_own(handle):
+    """The tile of one group reads columns of the next one: what they hold changes nothing."""
+    r = np.random.default_rng(5)
+    sizes, M, K = [5, 40, 3], 136, 72
+    off = offsets_of(sizes)
+    A, X = CuArray(store(normal(r, (K, 3 * M)), F16)), normal(r, (K, 48))
+    out = []
+    for bad in (None, np.nan, np.inf):
+        Y = X.copy()
+        if bad is not None:
+            Y[:, 5:45] = bad
+        d = CuArray(np.zeros((M, 48), np.float32, order="F"))
+        handle.gemm_grouped(True, M, 48, K, 1.0, A, K, K * M, CuArray(store(Y, F16)), K, F16, 0.0, None, M, F32, d, M, F32, CuArray(off), 3)
+        sync(handle)
+        out.append(Array(d))
+    for o in out[1:]:
+        assert np.array_equal(o[:, :5], out[0][:, :5]) and np.array_equal(o[:, 45:], out[0][:, 45:])
+        assert not np.any(np.isfinite(o[:, 5:45]))
+
+
+BAD = [[0, 5, 3, 9], [-1, 2, 3, 9], [0, 2, 3, 10], [0, 100, 3, 9], [5, 5, 5, 4], [0, 0, -2147483648, 9], [0, 2147483647, 3, 9]]
+
+
+@pytest.mark.parametrize("off", BAD, ids=str)
+@pytest.mark.parametrize("kernel", [_lib.KERNEL_TCGEN05, _lib.KERNEL_SIMPLE])
+def test_bad_offsets_write_nothing_and_are_reported(handle, off, kernel):
+    """The kernel checks the offsets before it forms an address with one."""
+    handle.set_option(_lib.OPT_FORCE_KERNEL, kernel)
+    a, b, o = CuArray(np.ones((64, 192), F16, order="F")), CuArray(np.ones((64, 9), F16, order="F")), CuArray(np.array(off, np.int32))
+    d = CuArray(np.full((64, 9), 3.5, F32, order="F"))
+    handle.gemm_grouped(True, 64, 9, 64, 1.0, a, 64, 4096, b, 64, F16, 0.0, None, 64, F32, d, 64, F32, o, 3)
+    sync(handle, _lib.STATUS_BAD_OFFSETS)
+    assert np.all(Array(d) == 3.5)
+    d = CuArray(np.full((64, 192), 3.5, F32, order="F"))
+    handle.gemm_grouped_k(64, 64, 9, 1.0, b, 64, b, 64, F16, 0.0, None, 64, 4096, F32, d, 64, 4096, F32, o, 3)
+    sync(handle, _lib.STATUS_BAD_OFFSETS)
+    assert np.all(Array(d) == 3.5)
+
+
+def run_grouped_k(handle, sizes, M, N, *, ab=BFloat16, d_type=F32, c_type=F32, alpha=1.0, beta=0.0, start=0, tail=0, pad=0, gap=0, alias=False,
+                  expect=None, seed=0, **options):
+    r = np.random.default_rng(seed)
+    off = offsets_of(sizes, start)
+    K, E = int(off[-1]) + tail, len(sizes)
+    A, B = store(normal(r, (M, K)), ab), store(normal(r, (N, K)), ab)
+    for x in (A, B):  # infinities times zeros would show as NaN
+        x[:, :start] = fill_of(ab, np.nan)
+        x[:, int(off[-1]):] = fill_of(ab, np.inf)
+    C = [store(normal(r, (M, N)), c_type) for _ in range(E)]
+    ldab, ldd = pad, M + pad
+    nan, sentinel = fill_of(ab, np.nan), np.float32(-7.25)
+    stride = ldd * N + gap
+
+    def pack(mats, elem, fill):
+        out = np.full(stride * len(mats), fill_of(elem, fill), memory_type(elem))
+        for e, m in enumerate(mats):
+            out[e * stride: e * stride + ldd * N].reshape(ldd, N, order="F")[:M] = m
+        return out
+
+    d_host = pack(C, c_type, sentinel) if alias else pack([store(np.full((M, N), sentinel), d_type)] * E, d_type, sentinel)
+    d_dev = CuArray(d_host)
+    c_dev = d_dev if alias else CuArray(pack(C, c_type, np.nan)) if beta else None
+    for k in ("FORCE_KERNEL", "TILE_N", "CTA_PAIR"):
+        handle.set_option(getattr(_lib, "OPT_" + k), options.get(k.lower(), 0))
+    a_dev, b_dev = CuArray(taller(A, M + ldab, nan)), CuArray(taller(B, N + ldab, nan))
+    handle.gemm_grouped_k(M, N, K, alpha, a_dev, M + ldab, b_dev, N + ldab, ab, beta, c_dev, ldd, stride, c_type, d_dev, ldd, stride, d_type,
+                          CuArray(off), E)
+    sync(handle)
+    if expect is not None:
+        assert handle.last_launch()["kernel"] == expect
+    got = Array(d_dev)
+    exact, S = grouped_k_ref(value(A, ab), value(B, ab), [value(c, c_type) for c in C], off, alpha, beta)
+    for e in range(E):
+        mat = got[e * stride: e * stride + ldd * N].reshape(ldd, N, order="F")
+        close(value(mat[:M], d_type), exact[e], S[e], sizes[e], d_type, f"group {e} of {sizes}")
+        assert np.all(value(mat[M:], d_type) == sentinel), "rows between the columns were written"
+        assert np.all(value(got[e * stride + ldd * N:(e + 1) * stride], d_type) == sentinel), "gap between the matrices was written"
+
+
+SIZES_K = [[1], [0, 1, 0], [15, 16, 17, 0, 31], [63, 64, 65], [48, 80, 112, 128], [1, 2, 3, 4, 5, 6, 7, 8, 9], [200, 0, 333], [0, 0, 0], [1000]]
+
+
+@pytest.mark.parametrize("sizes", SIZES_K, ids=str)
+@pytest.mark.parametrize("beta", [0.0, 1.0])
+def test_k_sizes(handle, sizes, beta):
+    run_grouped_k(handle, sizes, 264, 200, beta=beta, start=3, tail=5, expect=_lib.KERNEL_TCGEN05)
+
+
+@pytest.mark.parametrize("tile_n,cta_pair", [(64, 1), (128, 1), (128, 2), (256, 2)])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_k_every_tile_shape(handle, tile_n, cta_pair, beta):
+    run_grouped_k(handle, [3, 0, 70, 300, 257, 31, 16], 392, 320, tile_n=tile_n, cta_pair=cta_pair, beta=beta, alpha=2.0,
+                  force_kernel=_lib.KERNEL_TCGEN05, tail=9)
+
+
+@pytest.mark.parametrize("ab", [F16, BFloat16])
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+@pytest.mark.parametrize("c_type", [None, F16, BFloat16, F32])
+def test_k_types(handle, ab, d_type, c_type):
+    run_grouped_k(handle, [40, 0, 93], 136, 264, ab=ab, d_type=d_type, c_type=c_type or F32, beta=0.5 if c_type else 0.0, alpha=-1.5)
+
+
+@pytest.mark.parametrize("M,N", [(1, 1), (7, 9), (8, 264), (250, 40), (136, 1), (257, 300), (128, 96)])
+@pytest.mark.parametrize("beta", [0.0, 1.0])
+def test_k_any_shape(handle, M, N, beta):
+    run_grouped_k(handle, [40, 0, 93], M, N, beta=beta)
+    run_grouped_k(handle, [40, 0, 93], M, N, beta=beta, d_type=BFloat16, c_type=F32, gap=8)
+
+
+def test_k_gaps_and_in_place(handle):
+    run_grouped_k(handle, [40, 0, 93], 136, 72, pad=8, gap=24, beta=1.0)
+    run_grouped_k(handle, [40, 0, 93], 136, 72, pad=3, gap=1, beta=1.0, expect=_lib.KERNEL_SIMPLE)
+    run_grouped_k(handle, [40, 0, 93], 136, 72, gap=1, beta=1.0, expect=_lib.KERNEL_TCGEN05)
+    run_grouped_k(handle, [40, 0, 93], 264, 200, beta=1.0, alias=True)
+    run_grouped_k(handle, [40, 0, 93], 136, 72, force_kernel=_lib.KERNEL_SIMPLE, beta=0.5, start=2, tail=1)
+
+
+@pytest.mark.parametrize("groups", [256, 1024])
+def test_k_many_groups(handle, groups):
+    sizes = np.random.default_rng(groups).integers(0, 20, groups).tolist()
+    run_grouped_k(handle, sizes, 40, 24, start=1, tail=1, beta=1.0)
+    run_grouped_k(handle, sizes, 264, 136)
+
+
+def test_k_a_neighbours_nan_stays_its_own(handle):
+    r = np.random.default_rng(5)
+    off = offsets_of([5, 40, 19])
+    X, Y = normal(r, (136, 64)), normal(r, (72, 64))
+    out = []
+    for bad in (None, np.nan, np.inf):
+        x, y = X.copy(), Y.copy()
+        if bad is not None:
+            x[:, 5:45] = y[:, 5:45] = bad
+        d = CuArray(np.zeros((136, 216), np.float32, order="F"))
+        handle.gemm_grouped_k(136, 72, 64, 1.0, CuArray(store(x, F16)), 136, CuArray(store(y, F16)), 72, F16, 0.0, None, 136, 136 * 72, F32, d, 136,
+                              136 * 72, F32, CuArray(off), 3)
+        sync(handle)
+        out.append(Array(d))
+    for o in out[1:]:
+        assert np.array_equal(o[:, :72], out[0][:, :72]) and np.array_equal(o[:, 144:], out[0][:, 144:])
+        assert not np.any(np.isfinite(o[:, 72:144]))
+
+
+def test_a_layer_forward_and_backward(handle):
+    """One layer of experts as a training step runs it: forward, input gradient, weight gradient added to what
+    is there, all on one stream without a word to the host in between."""
+    r = np.random.default_rng(9)
+    sizes, K, M = [70, 0, 33, 129], 136, 264
+    off, T = offsets_of(sizes), sum(sizes)
+    W, X, G = store(normal(r, (K, 4 * M), K ** -0.5), BFloat16), store(normal(r, (K, T)), BFloat16), store(normal(r, (M, T)), BFloat16)
+    acc = normal(r, (K, 4 * M))
+    Wd, Xd, Gd, od = CuArray(W), CuArray(X), CuArray(G), CuArray(off)
+    Y, dX, dW = CuArray(np.zeros((M, T), np.uint16, order="F")), CuArray(np.zeros((K, T), np.uint16, order="F")), CuArray(np.asfortranarray(acc))
+    handle.gemm_grouped(True, M, T, K, 1.0, Wd, K, K * M, Xd, K, BFloat16, 0.0, None, M, BFloat16, Y, M, BFloat16, od, 4)
+    handle.gemm_grouped(False, K, T, M, 1.0, Wd, K, K * M, Gd, M, BFloat16, 0.0, None, K, BFloat16, dX, K, BFloat16, od, 4)
+    handle.gemm_grouped_k(K, M, T, 1.0, Xd, K, Gd, M, BFloat16, 1.0, dW, K, K * M, F32, dW, K, K * M, F32, od, 4)
+    sync(handle)
+    w = [value(W[:, e * M:(e + 1) * M], BFloat16) for e in range(4)]
+    x, g = value(X, BFloat16), value(G, BFloat16)
+    close(value(Array(Y), BFloat16), *grouped_ref(w, x, None, off, 1.0, 0.0, True, np.zeros((M, T))), K, BFloat16, "forward")
+    close(value(Array(dX), BFloat16), *grouped_ref(w, g, None, off, 1.0, 0.0, False, np.zeros((K, T))), M, BFloat16, "input gradient")
+    exact, S = grouped_k_ref(x, g, [acc[:, e * M:(e + 1) * M].astype(np.float64) for e in range(4)], off, 1.0, 1.0)
+    close(value(Array(dW), F32), np.hstack(exact), np.hstack(S), max(sizes), F32, "weight gradient")
