@@ -49,6 +49,12 @@ SIGNATURES = {
     "b200_gemm_grouped": (_i, [_p, _p, _i, _i64, _i64, _i64, _f, _p, _i64, _i64, _p, _i64, _i, _f, _p, _i64, _i, _p, _i64, _i, _p, _i64]),
     "b200_gemm_grouped_k": (_i, [_p, _p, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _i, _f, _p, _i64, _i64, _i, _p, _i64, _i64, _i, _p,
                                  _i64]),
+    "b200_mxfp4_scale_bytes": (_i64, [_i64, _i64, _i64]),
+    "b200_mxfp4_quantize": (_i, [_p, _p, _i, _i64, _i64, _p, _i64, _i, _p, _i64, _p, _p, _i64]),
+    "b200_mxfp4_dequantize": (_i, [_p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i, _p, _i64]),
+    "b200_gemm_mxfp4": (_i, [_p, _p, _i64, _i64, _i64, _f, _p, _i64, _p, _p, _i64, _p, _f, _p, _i64, _i, _p, _i64, _i]),
+    "b200_gemm_mxfp4_grouped": (_i, [_p, _p, _i64, _i64, _i64, _f, _p, _i64, _i64, _p, _p, _i64, _p, _f, _p, _i64, _i, _p, _i64, _i, _p,
+                                     _i64]),
     "b200_gemm_f16f32_gated": (_i, [_p, _p, _i, _i, _i64, _i64, _i64, _f, _p, _i64, _p, _i64, _f, _p, _i64, _p, _i64, _p, _i64]),
     "b200_stream_write_u32": (_i, [_p, _p, C.c_uint32]),
     "b200_stream_wait_u32": (_i, [_p, _p, C.c_uint32]),

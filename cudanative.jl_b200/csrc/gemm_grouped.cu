@@ -133,10 +133,10 @@ struct Grouped {
     const int32_t* offsets;
 };
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
-int launch_grouped(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas>;
-    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas>;
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
+int launch_promote(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote>;
+    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
@@ -146,7 +146,7 @@ int launch_grouped(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid,
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(256, 1, 1);
+    cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
     cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -160,6 +160,13 @@ int launch_grouped(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid,
     cfg.numAttrs = pdl ? 2 : 1;
     B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p));
     return B200_OK;
+}
+
+// binary32 results add several accumulators with rounding to nearest (epilogue_sm100.cuh)
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
+int launch_grouped(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+    if (p.e.d_fmt == 0) return launch_promote<kBN, kAMn, kRaggedK, kCtas, true>(tm, p, grid, stream, pdl);
+    return launch_promote<kBN, kAMn, kRaggedK, kCtas, false>(tm, p, grid, stream, pdl);
 }
 
 template <int kBN, int kCtas>
@@ -210,24 +217,24 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     int tile_n, pair, rc;
     pick_tile(h, g, &tile_n, &pair);
     GroupedParams p = {};
-    p.M = static_cast<int>(g.M);
+    p.e.M = static_cast<int>(g.M);
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
     p.groups = static_cast<int>(g.groups);
     p.tiles_m = static_cast<int>((g.M + 128 * pair - 1) / (128 * pair));
     p.tiles_n = g.ragged_k ? static_cast<int>((g.N + tile_n - 1) / tile_n) : 0;
     p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
-    p.alpha = g.alpha;
-    p.beta = g.beta;
+    p.e.alpha = g.alpha;
+    p.e.beta = g.beta;
     p.offsets = g.offsets;
-    p.C = g.C;
-    p.D = g.D;
-    p.ldc = g.ldc;
-    p.ldd = g.ldd;
-    p.stride_c = g.stride_c;
-    p.stride_d = g.stride_d;
-    p.c_fmt = elem_fmt(g.c_type);
-    p.d_fmt = elem_fmt(g.d_type);
+    p.e.C = g.C;
+    p.e.D = g.D;
+    p.e.ldc = g.ldc;
+    p.e.ldd = g.ldd;
+    p.e.stride_c = g.stride_c;
+    p.e.stride_d = g.stride_d;
+    p.e.c_fmt = elem_fmt(g.c_type);
+    p.e.d_fmt = elem_fmt(g.d_type);
     p.a_per_group = g.stride_a != 0 ? 1 : 0;
     p.ab_bf16 = g.ab_type == B200_BF16 ? 1 : 0;
     p.status = h->status_word;
@@ -251,20 +258,21 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     auto strides_ok = [&](int64_t stride, int64_t ld, int type) {
         return !g.ragged_k || g.groups == 1 || (stride % (16 / elem_bytes(type)) == 0 && stride >= ld * g.N);
     };
+    const uint32_t chunk = g.ragged_k || g.d_type == B200_F32 ? 16 : 32;  // columns per bulk copy (GroupedCfg::Epi)
     auto out_map = [&](CUtensorMap* m, const void* ptr, int64_t ld, int64_t stride, int type, const char* what) {
         BatchDim b;
         if (g.ragged_k) {
             b.count = g.groups;
             b.stride = g.groups > 1 ? stride : ld * g.N;
         }
-        return make_map_2d(m, map_type(type), elem_bytes(type), ptr, g.M, g.N, ld, 128, 32, CU_TENSOR_MAP_SWIZZLE_NONE, what, b);
+        return make_map_2d(m, map_type(type), elem_bytes(type), ptr, g.M, g.N, ld, 128, chunk, CU_TENSOR_MAP_SWIZZLE_NONE, what, b);
     };
-    p.d_tma = bulk_matrix(g.D, g.ldd, g.M, g.d_type) && strides_ok(g.stride_d, g.ldd, g.d_type);
-    p.c_tma = g.ragged_k && g.beta != 0.0f && bulk_matrix(g.C, g.ldc, g.M, g.c_type) && strides_ok(g.stride_c, g.ldc, g.c_type);
+    p.e.d_tma = bulk_matrix(g.D, g.ldd, g.M, g.d_type) && strides_ok(g.stride_d, g.ldd, g.d_type);
+    p.e.c_tma = g.ragged_k && g.beta != 0.0f && bulk_matrix(g.C, g.ldc, g.M, g.c_type) && strides_ok(g.stride_c, g.ldc, g.c_type);
     tm[3] = tm[0];  // never dereferenced unless replaced
-    if (p.d_tma && (rc = out_map(&tm[3], g.D, g.ldd, g.stride_d, g.d_type, "D"))) return rc;
+    if (p.e.d_tma && (rc = out_map(&tm[3], g.D, g.ldd, g.stride_d, g.d_type, "D"))) return rc;
     tm[2] = tm[3];
-    if (p.c_tma && (rc = out_map(&tm[2], g.C, g.ldc, g.stride_c, g.c_type, "C"))) return rc;
+    if (p.e.c_tma && (rc = out_map(&tm[2], g.C, g.ldc, g.stride_c, g.c_type, "C"))) return rc;
 
     // ragged N: at most one partial tile column per group that has columns
     const int64_t cols = g.ragged_k ? g.groups * p.tiles_n : g.N / tile_n + std::min<int64_t>(g.groups, g.N);

@@ -20,10 +20,11 @@
 //             between the arrival of the tile and its use.
 //
 // Roles and barriers are those of gemm_sm100.cuh (warp 0 producer, warp 1 MMA issuer, warp 2 tensor
-// memory, warps 4-7 epilogue); every wait is bounded.  Offsets that decrease or leave [0, total] are
+// memory) with the epilogue of epilogue_sm100.cuh in warps 4-11; every wait is bounded.  Offsets that decrease or leave [0, total] are
 // reported in the device status word (kBadOffsets) and the launch writes nothing.
 #pragma once
 
+#include "epilogue_sm100.cuh"
 #include "ptx_sm100.cuh"
 
 namespace b200 {
@@ -31,25 +32,21 @@ namespace b200 {
 constexpr int kMaxGroups = 1024;
 
 struct GroupedParams {
-    int M, N, K;           // ragged N: N = columns of B, C, D; ragged K: K = columns of A and B
+    int N, K;              // ragged N: N = columns of B, C, D; ragged K: K = columns of A and B
     int groups;
     int tiles_m, tiles_n;  // tiles_n: ragged K only (tile columns of one D_e)
     int raster_group;
-    float alpha, beta;
     const int* offsets;
-    const void* C;
-    void* D;
-    long long ldc, ldd, stride_c, stride_d;  // strides: ragged K only
-    int c_fmt, d_fmt;      // 0 = binary32, 1 = binary16, 2 = bfloat16
-    int c_tma, d_tma;      // C / D may be moved by bulk copies
     int a_per_group;       // ragged N: 0 = one A for all groups
     int ab_bf16;
+    EpilogueParams e;
     int* status;
     unsigned long long wait_budget_ns;
 };
 
-template <int kBN, bool kRaggedK, int kCtas>
+template <int kBN, bool kRaggedK, int kCtas, bool kPromote>
 struct GroupedCfg {
+    static constexpr int THREADS = 384;
     static constexpr int BM = 128;
     static constexpr int BK = 64;
     static constexpr int BN_LOCAL = kBN / kCtas;
@@ -58,33 +55,31 @@ struct GroupedCfg {
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int BBOX = BN_LOCAL < 64 ? BN_LOCAL : 64;  // B rows per bulk load
     static constexpr int BBOX_BYTES = BBOX * BK * 2;
-    static constexpr int GRANULE = kCtas == 2 ? 32 : 16;         // of the instruction's N
-    static constexpr int EPI_COLS = 32;
-    static constexpr int EPI_BYTES = BM * EPI_COLS * 4;
-    static constexpr int EPI_BUFS = kRaggedK ? 5 : 3;
-    static constexpr int C_AHEAD = 3;                            // chunks of C in flight (ragged K)
-    static constexpr int TABLE_BYTES = 2 * (kMaxGroups + 4) * 4;
+    static constexpr int GRANULE = kCtas == 2 ? 32 : 16;        // of the instruction's N
+    static constexpr int PROMOTE_KB = 8;                        // k-blocks per accumulator of a binary32 D
+    using Epi = EpilogueCfg<kBN, (kRaggedK || kPromote) ? 16 : 32, kRaggedK>;
+    static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - EPI_BUFS * EPI_BYTES;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int TMEM_COLS = 2 * kBN < 32 ? 32 : 2 * kBN;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BUFS * EPI_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static_assert(!kRaggedK || C_AHEAD + 2 <= EPI_BUFS, "a buffer is refilled two stores after its own");
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int NBARS = 4 * STAGES + 4 + 2 * Epi::BUFS;
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
-    static_assert(8 * (4 * STAGES + 4 + EPI_BUFS) + 8 <= BAR_BYTES, "barriers");
+    static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
 };
 
 // Offsets into shared memory, checked and, for kTiles, with an exclusive scan of the tile columns per
-// group in `first` (groups + 1 entries).  All 256 threads; returns false when the offsets are no
+// group in `first` (groups + 1 entries).  All kThreads threads; returns false when the offsets are no
 // ascending sequence inside [0, total].
-template <bool kTiles>
+template <bool kTiles, int kThreads = 256>
 __device__ __forceinline__ bool load_groups(const int* offsets, int groups, int total, int tile, int* off, int* first,
                                             int* warp_sums) {
-    constexpr int PER = kMaxGroups / 256;
+    constexpr int PER = kMaxGroups / kThreads + 1;  // entries 0 .. groups
     const int t = threadIdx.x;
     bool bad = false;
-    for (int e = t; e <= groups; e += 256) off[e] = offsets[e];
+    for (int e = t; e <= groups; e += kThreads) off[e] = offsets ? offsets[e] : (e == 0 ? 0 : total);  // none: one group
     __syncthreads();
     int n[PER], sum = 0;
 #pragma unroll
@@ -116,7 +111,6 @@ __device__ __forceinline__ bool load_groups(const int* offsets, int groups, int 
             if (e <= groups) first[e] = base;
             base += n[i];
         }
-        if (t == 255 && groups == kMaxGroups) first[kMaxGroups] = base;
         __syncthreads();
     }
     return !bad;
@@ -134,19 +128,14 @@ __device__ __forceinline__ int find_group(const int* first, int groups, int q) {
     return lo;
 }
 
-struct GroupedUnit {
-    int group, m0, n0, cols;  // this CTA's first row; first column (absolute); columns of the tile that exist
-    int k0, k_len;            // first k and how many
-};
-
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
-__global__ void __launch_bounds__(256, 1)
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
+__global__ void __launch_bounds__(384, 1)
 gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
                      const GroupedParams p) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas>;
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote>;
     constexpr int STAGES = Cfg::STAGES;
-    constexpr int BUFS = Cfg::EPI_BUFS;
+    using Epi = typename Cfg::Epi;
     constexpr bool kPair = (kCtas == 2);
     constexpr bool kBMn = kRaggedK;  // ragged K: both operands have their columns along k
     static_assert(!kRaggedK || kAMn, "ragged K: A is M x K column-major");
@@ -155,7 +144,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t epi_base = smem_base + STAGES * Cfg::STAGE_BYTES;
-    constexpr int kTableAt = STAGES * Cfg::STAGE_BYTES + BUFS * Cfg::EPI_BYTES;
+    constexpr int kTableAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
     const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
     uint8_t* epi_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
     int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
@@ -169,8 +158,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
     auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + 2 + a); };
     auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 4 + b); };
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * (4 * STAGES + 4 + BUFS));
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * (4 * STAGES + 4 + BUFS) + 4);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -189,9 +178,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tmem_full_bar(a), 1);
-            mbar_init(tmem_empty_bar(a), 4 * kCtas);
+            mbar_init(tmem_empty_bar(a), 8 * kCtas);
         }
-        for (int b = 0; b < BUFS; ++b) mbar_init(cfull_bar(b), 1);
+        for (int b = 0; b < 2 * Epi::BUFS; ++b) mbar_init(cfull_bar(b), 1);
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
@@ -208,7 +197,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     griddep_wait();
 
     // the scan's scratch may lie in the epilogue buffers: nothing uses them yet
-    const bool offsets_ok = load_groups<!kRaggedK>(p.offsets, p.groups, kRaggedK ? p.K : p.N, kBN, off, first,
+    const bool offsets_ok = load_groups<!kRaggedK, Cfg::THREADS>(p.offsets, p.groups, kRaggedK ? p.K : p.N, kBN, off, first,
                                                    reinterpret_cast<int*>(epi_gen));
     if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
         p.status[1] = static_cast<int>(blockIdx.x);
@@ -219,7 +208,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * tiles_per_group : first[p.groups] * p.tiles_m;
 
     auto decode = [&](int unit) {
-        GroupedUnit u;
+        Unit u;
         int idx, tn_count;
         if constexpr (kRaggedK) {
             u.group = unit / tiles_per_group;
@@ -249,11 +238,12 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             u.k0 = 0;
             u.k_len = p.K;
         }
+        u.kb = (u.k_len + Cfg::BK - 1) / Cfg::BK;
         return u;
     };
-    auto inst_n = [&](const GroupedUnit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
+    auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
     // rows of a group's last k-block; a ragged 16-row step has to be padded with zeros
-    auto needs_tail = [&](const GroupedUnit& u) { return kRaggedK && (u.k_len % 16) != 0; };
+    auto needs_tail = [&](const Unit& u) { return kRaggedK && (u.k_len % 16) != 0; };
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -263,12 +253,12 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             bool ok = true;
             const uint64_t once = l2_policy_evict_first();
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const GroupedUnit u = decode(unit);
+                const Unit u = decode(unit);
                 const int ninst = inst_n(u);
                 const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
                 const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
                 const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
-                const int kb1 = (u.k_len + Cfg::BK - 1) / Cfg::BK;
+                const int kb1 = u.kb;
                 const int z = u.group * p.a_per_group;
                 // one tile column in this group: A is read once, B again and again
                 const bool a_once = !kRaggedK && first[u.group + 1] - first[u.group] == 1;
@@ -338,21 +328,21 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             uint32_t ph = 0, tail_ph = 0, ucount = 0;
             bool ok = true;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const GroupedUnit u = decode(unit);
-                if (kRaggedK && u.k_len == 0) continue;  // an empty group has no accumulator
+                const Unit u = decode(unit);
+                // an empty group has no accumulator
                 const uint32_t idesc = idesc0 | (static_cast<uint32_t>(inst_n(u) >> 3) << 17);
-                const uint32_t acc = ucount & 1u;
-                ok = mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty);
-                if (!ok) break;
-                tc_fence_after_sync();
-                const uint32_t d_tmem = tmem_base + acc * kBN;
-                uint32_t accumulate = 0;
-                const int kb1 = (u.k_len + Cfg::BK - 1) / Cfg::BK;
-                for (int kb = 0; kb < kb1; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    const uint32_t acc = ucount & 1u;
+                    const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
+                    const bool end = kb + 1 == u.kb || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
+                    if (begin) {
+                        ok = mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty);
+                        if (!ok) break;
+                    }
                     ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
                     if (!ok) break;
                     int steps = Cfg::BK / 16;
-                    if (kb + 1 == kb1) {
+                    if (kb + 1 == u.kb) {
                         steps = (u.k_len - kb * Cfg::BK + 15) / 16;
                         if (needs_tail(u)) {
                             ok = mbar_wait(tail_ready_bar(s), (tail_ph >> s) & 1u, wc, kWaitTail);
@@ -361,22 +351,20 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         }
                     }
                     tc_fence_after_sync();
+                    const uint32_t d_tmem = tmem_base + acc * kBN;
                     const uint64_t da = da0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
                     const uint64_t db = db0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < Cfg::BK / 16; ++k) {
-                        if (k < steps) {
-                            umma_f16<kCtas>(d_tmem, da + k * kStepA, db + k * kStepB, idesc, accumulate);
-                            accumulate = 1u;
-                        }
-                    }
+                    for (int k = 0; k < Cfg::BK / 16; ++k)
+                        if (k < steps) umma_f16<kCtas>(d_tmem, da + k * kStepA, db + k * kStepB, idesc, (begin && k == 0) ? 0u : 1u);
                     if constexpr (kPair) umma_commit_pair(empty_bar(s));
                     else umma_commit<kCtas>(empty_bar(s));
+                    if (end) {
+                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                        else umma_commit<kCtas>(tmem_full_bar(acc));
+                        ++ucount;
+                    }
                 }
-                if (!ok) break;
-                if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                else umma_commit<kCtas>(tmem_full_bar(acc));
-                ++ucount;
             }
         }
         __syncwarp();
@@ -386,8 +374,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         uint32_t tail_ph = 0;
         bool ok = true;
         for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-            const GroupedUnit u = decode(unit);
-            const int kb1 = (u.k_len + Cfg::BK - 1) / Cfg::BK;
+            const Unit u = decode(unit);
+            const int kb1 = u.kb;
             if (needs_tail(u)) {
                 const int st = (s + kb1 - 1) % STAGES;
                 ok = mbar_wait(tail_full_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail);
@@ -414,163 +402,11 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         __syncwarp();
     } else if (warp >= 4) {
-        // ------------------------------------------------------------------ epilogue
-        const int et = threadIdx.x - 128;
-        const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const bool elected = (et == 0);
-        const bool has_c = (p.beta != 0.0f);
-        const bool c_bulk = kRaggedK && has_c && p.c_tma;
-        const float alpha = p.alpha, beta = p.beta;
-        const bool c_half = p.c_fmt != 0, d_half = p.d_fmt != 0;
-        const uint32_t c_chunk_bytes = c_half ? Cfg::EPI_BYTES / 2 : Cfg::EPI_BYTES;
-        const bool two_phase = c_bulk && (c_half != d_half);
-        const uint64_t stream_policy = l2_policy_evict_first();
-        uint32_t g = 0, loaded = 0;  // chunks done; chunks of C asked for
-
-        // runs C_AHEAD chunks ahead of the epilogue through the same sequence of chunks
-        int pf_unit = unit_first, pf_j = 0;
-        GroupedUnit pf = {};
-        bool pf_new = true;
-        auto fetch_c = [&]() {
-            if (pf_unit >= num_units) return;
-            if (pf_new) pf = decode(pf_unit);
-            pf_new = false;
-            const uint32_t b = loaded % BUFS;
-            mbar_arrive_expect_tx(cfull_bar(b), c_chunk_bytes);
-            tma_load_3d_hint(epi_base + b * Cfg::EPI_BYTES, &tmC, pf.m0, pf.n0 + pf_j * Cfg::EPI_COLS, pf.group, cfull_bar(b),
-                             stream_policy);
-            ++loaded;
-            if (++pf_j * Cfg::EPI_COLS >= pf.cols) {
-                pf_j = 0;
-                pf_unit += unit_stride;
-                pf_new = true;
-            }
-        };
-        if (c_bulk && elected)
-            for (int i = 0; i < Cfg::C_AHEAD; ++i) fetch_c();
-
-        uint32_t ucount = 0;
-        bool fail = false;
-        for (int unit = unit_first; unit < num_units; unit += unit_stride) {
-            const GroupedUnit u = decode(unit);
-            const bool empty = kRaggedK && u.k_len == 0;
-            const int nchunks = (u.cols + Cfg::EPI_COLS - 1) / Cfg::EPI_COLS;
-            const uint32_t acc = ucount & 1u;
-            bool ok = empty || mbar_wait(tmem_full_bar(acc), (ucount >> 1) & 1u, wc, kWaitTmemFull);
-            tc_fence_after_sync();
-            const int m = u.m0 + et;
-            for (int j = 0; j < nchunks; ++j, ++g) {
-                const uint32_t buf = g % BUFS;
-                // a bulk store writes whole chunks: a chunk that ends in another group's columns is
-                // stored column by column (ragged K: D_e's own edge, which the tensor map clips)
-                const bool bulk = p.d_tma && (kRaggedK || (j + 1) * Cfg::EPI_COLS <= u.cols);
-                if (elected) {
-                    // at most BUFS - 2 stores may still read their buffers: the one that is refilled
-                    // (C) or overwritten next is free
-                    if (c_bulk) {
-                        tma_store_wait_read<1>();
-                        fetch_c();
-                    } else {
-                        tma_store_wait_read<BUFS - 1>();
-                    }
-                }
-                if (c_bulk) ok = ok && mbar_wait(cfull_bar(buf), (g / BUFS) & 1u, wc, kWaitCTile);
-                else named_bar_sync(1, 128);
-                ok = __all_sync(0xffffffffu, ok);
-                uint32_t r[32];
-                float* col = reinterpret_cast<float*>(epi_gen + buf * Cfg::EPI_BYTES) + et;
-                __half* colh = reinterpret_cast<__half*>(epi_gen + buf * Cfg::EPI_BYTES) + et;
-                __nv_bfloat16* colb = reinterpret_cast<__nv_bfloat16*>(colh);
-                if (ok) {
-                    if (empty) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = 0u;
-                    } else {
-                        tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + j * Cfg::EPI_COLS, r);
-                        tmem_wait_ld();
-                    }
-                    if (c_bulk) {
-                        if (p.c_fmt == 2) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * __bfloat162float(colb[i * Cfg::BM])));
-                        } else if (c_half) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * __half2float(colh[i * Cfg::BM])));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * col[i * Cfg::BM]));
-                        }
-                    } else if (has_c) {
-                        const long long at = (kRaggedK ? u.group * p.stride_c : 0) + m +
-                                             static_cast<long long>(u.n0 + j * Cfg::EPI_COLS) * p.ldc;
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float c = 0.0f;
-                            if (m < p.M && j * Cfg::EPI_COLS + i < u.cols) {
-                                const long long e = at + i * p.ldc;
-                                c = p.c_fmt == 2 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.C)[e])
-                                    : c_half     ? __half2float(static_cast<const __half*>(p.C)[e])
-                                                 : static_cast<const float*>(p.C)[e];
-                            }
-                            r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * c));
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(alpha * __uint_as_float(r[i]));
-                    }
-                }
-                if (two_phase) named_bar_sync(3, 128);
-                if (ok && bulk) {
-                    if (p.d_fmt == 2) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) colb[i * Cfg::BM] = __float2bfloat16_rn(__uint_as_float(r[i]));
-                    } else if (d_half) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) colh[i * Cfg::BM] = __float2half_rn(__uint_as_float(r[i]));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) col[i * Cfg::BM] = __uint_as_float(r[i]);
-                    }
-                    fence_proxy_async_smem();
-                } else if (ok && m < p.M) {
-                    const long long at = (kRaggedK ? u.group * p.stride_d : 0) + m +
-                                         static_cast<long long>(u.n0 + j * Cfg::EPI_COLS) * p.ldd;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        if (j * Cfg::EPI_COLS + i < u.cols) {
-                            const long long e = at + i * p.ldd;
-                            if (p.d_fmt == 2) static_cast<__nv_bfloat16*>(p.D)[e] = __float2bfloat16_rn(__uint_as_float(r[i]));
-                            else if (d_half) static_cast<__half*>(p.D)[e] = __float2half_rn(__uint_as_float(r[i]));
-                            else static_cast<float*>(p.D)[e] = __uint_as_float(r[i]);
-                        }
-                    }
-                }
-                fail = named_bar_or(2, 128, !ok);
-                if (fail) break;
-                if (elected) {
-                    if (bulk && u.m0 < p.M) {
-                        const int y = u.n0 + j * Cfg::EPI_COLS;
-                        if constexpr (kRaggedK) tma_store_3d_hint(&tmD, u.m0, y, u.group, epi_base + buf * Cfg::EPI_BYTES, stream_policy);
-                        else tma_store_2d(&tmD, u.m0, y, epi_base + buf * Cfg::EPI_BYTES);
-                    }
-                    tma_store_commit();  // an empty group keeps the count of buffers in step
-                }
-            }
-            if (fail) break;
-            if (!empty) {
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (kPair) mbar_arrive_cluster(tmem_empty_bar(acc), 0);
-                    else mbar_arrive(tmem_empty_bar(acc));
-                }
-                ++ucount;
-            }
-        }
-        if (elected) tma_store_wait_all<0>();
+        const int wg = (warp - 4) >> 2;
+        const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote, Cfg::PROMOTE_KB, kRaggedK>(p.e, &tmC, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+                                                                           tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
+                                                                           unit_first, unit_stride, num_units, decode);
     }
 
     // ---------------------------------------------------------------------- common exit

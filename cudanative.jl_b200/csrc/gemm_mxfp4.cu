@@ -1,0 +1,160 @@
+// Host side of the microscaled 4-bit products: b200_gemm_mxfp4 and b200_gemm_mxfp4_grouped.
+#include "gemm_mxfp4.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+#include "internal.h"
+#include "tensor_map.h"
+
+namespace b200 {
+namespace {
+
+struct MxProblem {
+    int64_t M, N, K, groups;
+    float alpha, beta;
+    const void *A, *SA, *B, *SB, *C;
+    void* D;
+    int64_t lda, stride_a, ldb, ldc, ldd;
+    int c_type, d_type;
+    const int32_t* offsets;
+};
+
+template <int kBN, int kCtas, bool kPromote>
+int launch(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+    using Cfg = MxCfg<kBN, kCtas, kPromote>;
+    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote>;
+    static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
+    int dev = 0;
+    B200_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !((done.load(std::memory_order_relaxed) >> dev) & 1u)) {
+        B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+        if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kCtas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], p));
+    return B200_OK;
+}
+
+template <int kBN, int kCtas>
+int launch_typed(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+    if (p.e.d_fmt == 0) {
+        if constexpr (MxCfg<kBN, kCtas, true>::ACCS == 2) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
+        else return fail(B200_UNSUPPORTED, "mxfp4: a binary32 D takes tiles of 128 columns at most");
+    }
+    return launch<kBN, kCtas, false>(tm, p, grid, stream, pdl);
+}
+
+int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
+    int tile_n = 128, pair = 1, rc;
+    MxGemmParams p = {};
+    p.N = static_cast<int>(g.N);
+    p.K = static_cast<int>(g.K);
+    p.groups = static_cast<int>(g.groups);
+    p.tiles_m = static_cast<int>((g.M + 128 * pair - 1) / (128 * pair));
+    p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
+    p.offsets = g.offsets;
+    p.a_per_group = g.stride_a != 0 ? 1 : 0;
+    p.sa = static_cast<const uint8_t*>(g.SA);
+    p.sb = static_cast<const uint8_t*>(g.SB);
+    p.sa_stride = (g.M + 127) / 128 * ((g.K + 127) / 128) * 512;
+    p.e.M = static_cast<int>(g.M);
+    p.e.alpha = g.alpha;
+    p.e.beta = g.beta;
+    p.e.C = g.C;
+    p.e.D = g.D;
+    p.e.ldc = g.ldc;
+    p.e.ldd = g.ldd;
+    p.e.c_fmt = elem_fmt(g.c_type);
+    p.e.d_fmt = elem_fmt(g.d_type);
+    p.status = h->status_word;
+    p.wait_budget_ns = h->wait_budget_ns;
+    const int q = 16 / elem_bytes(g.d_type);
+    p.e.d_tma = !(reinterpret_cast<uintptr_t>(g.D) & 15u) && g.ldd % q == 0 && g.M % q == 0;
+
+    const int bn_local = tile_n / pair, bbox = bn_local % 64 == 0 ? 64 : 32;
+    const int64_t k_bytes = (g.K + 1) / 2;
+    CUtensorMap tm[3];
+    BatchDim b;
+    b.count = g.stride_a != 0 ? g.groups : 1;
+    b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
+    if ((rc = make_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
+    if ((rc = make_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
+    tm[2] = tm[1];  // never dereferenced unless replaced
+    if (p.e.d_tma && (rc = make_map_2d(&tm[2], map_type(g.d_type), elem_bytes(g.d_type), g.D, g.M, g.N, g.ldd, 128, g.d_type == B200_F32 ? 16 : 32,
+                                       CU_TENSOR_MAP_SWIZZLE_NONE, "D")))
+        return rc;
+
+    const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * p.tiles_m;
+    if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
+    const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
+    const int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
+    if ((rc = launch_typed<128, 1>(tm, p, grid, stream, h->pdl != 0))) return rc;
+    h->last = {B200_KERNEL_TCGEN05, tile_n, 1, grid, pair};
+    return B200_OK;
+}
+
+bool is_elem_type(int t) { return t == B200_F16 || t == B200_F32 || t == B200_BF16; }
+
+int entry(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
+    auto bad = [&](const char* m) { return fail(B200_INVALID_ARG, std::string("mxfp4 gemm: ") + m); };
+    const int64_t most = 0x7fffff00ll, k32 = (g.K + 31) / 32 * 32;
+    if (!is_elem_type(g.c_type) || !is_elem_type(g.d_type)) return bad("C and D must be Float16, bfloat16 or Float32");
+    if (g.M < 0 || g.N < 0 || g.K < 0) return bad("negative dimension");
+    if (g.M > most || g.N > most || g.K > most) return bad("dimension exceeds 2^31");
+    if (g.groups < 0 || g.groups > kMaxGroups) return bad("groups must be in [0, 1024]");
+    if (g.lda < k32 || g.ldb < k32 || g.lda % 32 || g.ldb % 32) return bad("lda and ldb must be multiples of 32 and at least K rounded up to 32");
+    if (g.stride_a < 0 || g.stride_a % 32) return bad("stride_a must be a multiple of 32");
+    if (g.groups > 1 && g.stride_a != 0 && g.stride_a < g.lda * g.M) return bad("stride_a smaller than one matrix");
+    if (g.ldd < std::max<int64_t>(1, g.M)) return bad("ldd smaller than M");
+    if (g.beta != 0.0f && g.ldc < std::max<int64_t>(1, g.M)) return bad("ldc smaller than M");
+    if (g.M == 0 || g.N == 0 || g.groups == 0) return B200_OK;
+    if (g.K == 0) return bad("K must be positive");
+    if (!g.A || !g.B || !g.SA || !g.SB) return bad("A, B or a scale pointer is null");
+    if (!g.D) return bad("D is null");
+    if (g.beta != 0.0f && !g.C) return bad("C is null but beta != 0");
+    if ((reinterpret_cast<uintptr_t>(g.A) | reinterpret_cast<uintptr_t>(g.B) | reinterpret_cast<uintptr_t>(g.SA) | reinterpret_cast<uintptr_t>(g.SB)) & 15u)
+        return bad("elements and scales must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(g.offsets) % 4 || reinterpret_cast<uintptr_t>(g.D) % elem_bytes(g.d_type) ||
+        (g.beta != 0.0f && reinterpret_cast<uintptr_t>(g.C) % elem_bytes(g.c_type)))
+        return bad("a pointer is not aligned to its element type");
+    if (h->force_kernel == B200_KERNEL_SIMPLE) return fail(B200_UNSUPPORTED, "mxfp4 gemm: there is no simple kernel for 4-bit operands");
+    int rc;
+    if ((rc = poll_previous_launch(h)) || (rc = check_current_device(h))) return rc;
+    rc = run(h, stream, g);
+    return rc ? rc : note_launch(h, stream);
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" int b200_gemm_mxfp4(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha, const void* A, int64_t lda,
+                               const void* a_scales, const void* B, int64_t ldb, const void* b_scales, float beta, const void* C, int64_t ldc,
+                               int c_type, void* D, int64_t ldd, int d_type) {
+    if (!h) return b200::fail(B200_INVALID_ARG, "null handle");
+    const b200::MxProblem g = {M, N, K, 1, alpha, beta, A, a_scales, B, b_scales, C, D, lda, 0, ldb, ldc, ldd, c_type, d_type, nullptr};
+    return b200::entry(h, static_cast<cudaStream_t>(stream), g);
+}
+
+extern "C" int b200_gemm_mxfp4_grouped(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha, const void* A, int64_t lda,
+                                       int64_t stride_a, const void* a_scales, const void* B, int64_t ldb, const void* b_scales, float beta,
+                                       const void* C, int64_t ldc, int c_type, void* D, int64_t ldd, int d_type, const int32_t* offsets,
+                                       int64_t groups) {
+    if (!h) return b200::fail(B200_INVALID_ARG, "null handle");
+    if (!offsets && groups > 0 && M > 0 && N > 0) return b200::fail(B200_INVALID_ARG, "mxfp4 gemm: offsets is null");
+    const b200::MxProblem g = {M, N, K, groups, alpha, beta, A, a_scales, B, b_scales, C, D, lda, stride_a, ldb, ldc, ldd, c_type, d_type, offsets};
+    return b200::entry(h, static_cast<cudaStream_t>(stream), g);
+}

@@ -1,0 +1,289 @@
+// Product of two microscaled 4-bit matrices for sm_100a, plain or grouped with ragged columns:
+//
+//   D[:, s_e] = alpha * A_e^T * B[:, s_e] + beta * C[:, s_e]
+//
+// A_e is K x M and B is K x N, elements and scales as mxfp4.cu lays them out; without offsets there is one
+// group of all columns.
+//
+// The pipeline is that of gemm_grouped.cuh with 256 values of k (128 bytes of elements) per stage, four
+// tcgen05.mma.kind::mxf4.block_scale of K = 64 each, and the stage's scales: one 512-byte tile per 128 rows
+// and 128 values of k, brought by a plain bulk copy and moved to tensor memory by tcgen05.cp in front of the
+// products that use them.  Copies and products of one thread run in order, so a set of scale columns can be
+// written again without a barrier; kScaleSets sets keep a copy from waiting for the products before it.
+//
+// A tile's scales always come from whole tiles of 128 columns, counted from the group's first column, as
+// they were quantised.  A tile of kBN columns starts inside one where kBN is no multiple of 128: the
+// scales' first tensor-memory column is moved by (start % 128) / 32.
+//
+// What bounds it: 4-bit products run at four times the rate of 16-bit ones, with the same bytes per cycle.
+// For few columns (a token, a decode step) the elements of A, 17/32 byte per value, are the floor.
+#pragma once
+
+#include "gemm_grouped.cuh"
+
+namespace b200 {
+
+struct MxGemmParams {
+    int N, K;
+    int groups;
+    int tiles_m;
+    int raster_group;
+    const int* offsets;  // nullptr: one group, all columns
+    int a_per_group;
+    const uint8_t* sa;
+    const uint8_t* sb;
+    long long sa_stride;  // bytes between the scales of A_e and A_{e+1}
+    EpilogueParams e;
+    int* status;
+    unsigned long long wait_budget_ns;
+};
+
+template <int kBN, int kCtas, bool kPromote>
+struct MxCfg {
+    static constexpr int THREADS = 384;
+    static constexpr int BM = 128;
+    static constexpr int BK = 256;  // values of k per stage
+    static constexpr int BN_LOCAL = kBN / kCtas;
+    static constexpr int A_BYTES = BM * BK / 2;
+    static constexpr int B_BYTES = BN_LOCAL * BK / 2;
+    static constexpr int B_TILES = (kBN + 127) / 128;  // scale tiles that a tile of columns touches at most
+    static constexpr int SF_BYTES = 1024 * (1 + B_TILES);
+    static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES + SF_BYTES + 1023) / 1024 * 1024;
+    static constexpr int BBOX = BN_LOCAL % 64 == 0 ? 64 : 32;
+    static constexpr int BBOX_BYTES = BBOX * BK / 2;
+    static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
+    static constexpr int PROMOTE_KB = 8;
+    using Epi = EpilogueCfg<kBN, kPromote ? 16 : 32, false>;
+    static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
+    static constexpr int BAR_BYTES = 512;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES;
+    static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
+    static constexpr int ACCS = kBN <= 192 ? 2 : 1;
+    static constexpr int SCALE_COLS = 8 * (1 + B_TILES);  // per set: 2 x 4 for A, 2 x 4 per scale tile for B
+    static constexpr int SCALE_AT = ACCS * kBN;
+    static constexpr int SCALE_SETS = (512 - SCALE_AT) / SCALE_COLS >= 4 ? 4 : 2;
+    static constexpr int USED_COLS = SCALE_AT + SCALE_SETS * SCALE_COLS;
+    static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int NBARS = 2 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
+    static_assert(USED_COLS <= 512, "tensor memory");
+    static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
+    static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
+    static_assert(kBN <= 128 || kBN == 192 || kBN == 256, "columns per tile and the scale tiles they touch");
+};
+
+template <int kBN, int kCtas, bool kPromote>
+__global__ void __launch_bounds__(384, 1)
+gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmD, const MxGemmParams p) {
+    using Cfg = MxCfg<kBN, kCtas, kPromote>;
+    using Epi = typename Cfg::Epi;
+    constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS;
+    constexpr bool kPair = (kCtas == 2);
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t epi_base = smem_base + STAGES * Cfg::STAGE_BYTES;
+    uint8_t* epi_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
+    constexpr int kTableAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
+    int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
+    int* first = off + kMaxGroups + 4;
+    int* first128 = kBN == 128 ? first : first + kMaxGroups + 4;  // scale tiles before each group
+    uint8_t* bar_gen = smem_gen + kTableAt + Cfg::TABLE_BYTES;
+
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + ACCS + a); };
+    auto cfull_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + 2 * ACCS + b); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t cta_rank = kPair ? cluster_cta_rank() : 0u;
+    const int unit_stride = kPair ? (gridDim.x >> 1) : gridDim.x;
+    const int unit_first = kPair ? (blockIdx.x >> 1) : blockIdx.x;
+    WaitCtx wc{abort_flag, p.status, p.wait_budget_ns};
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int a = 0; a < ACCS; ++a) {
+            mbar_init(tmem_full_bar(a), 1);
+            mbar_init(tmem_empty_bar(a), 8 * kCtas);
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmD);
+    }
+    if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
+    tc_fence_before_sync();
+    __syncthreads();
+    if constexpr (kPair) cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    griddep_launch_dependents();
+    griddep_wait();
+
+    bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<int*>(epi_gen));
+    if constexpr (kBN != 128) load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, 128, off, first128, reinterpret_cast<int*>(epi_gen));
+    if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
+        p.status[1] = static_cast<int>(blockIdx.x);
+        p.status[2] = p.groups;
+        __threadfence();
+    }
+    const int num_units = offsets_ok ? first[p.groups] * p.tiles_m : 0;
+    const int kt = (p.K + 127) / 128;  // scale tiles along K
+
+    auto decode = [&](int unit) {
+        Unit u;
+        u.group = find_group(first, p.groups, unit / p.tiles_m);
+        const int idx = unit - first[u.group] * p.tiles_m;
+        const int tn_count = first[u.group + 1] - first[u.group];
+        const int band = idx / (p.raster_group * tn_count);
+        const int row0 = band * p.raster_group;
+        const int rows = min(p.raster_group, p.tiles_m - row0);
+        const int in = idx - band * p.raster_group * tn_count;
+        const int tn = in / rows;
+        u.m0 = (row0 + in - tn * rows) * (Cfg::BM * kCtas) + static_cast<int>(cta_rank) * Cfg::BM;
+        u.n0 = off[u.group] + tn * kBN;
+        u.cols = min(kBN, off[u.group + 1] - u.n0);
+        u.k0 = 0;
+        u.k_len = p.K;
+        u.kb = (p.K + Cfg::BK - 1) / Cfg::BK;
+        return u;
+    };
+    auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
+    // of a tile's first column among the 128 of its scale tile
+    auto scale_shift = [&](const Unit& u) { return (u.n0 - off[u.group]) & 127; };
+    auto scale_tiles = [&](const Unit& u) { return (scale_shift(u) + u.cols + 127) / 128; };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            const uint64_t once = l2_policy_evict_first();
+            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                const Unit u = decode(unit);
+                const int ninst = inst_n(u);
+                const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
+                const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
+                const int b_tiles = scale_tiles(u);
+                const bool a_once = first[u.group + 1] - first[u.group] == 1;
+                const int z = u.group * p.a_per_group;
+                // a CTA of a pair may own no rows of A: its scales are then those of the last rows
+                const int a_tile = min(u.m0, (p.e.M - 1) / 128 * 128) / 128;
+                const uint8_t* sa = p.sa + z * p.sa_stride + static_cast<long long>(a_tile) * kt * 512;
+                const uint8_t* sb = p.sb + static_cast<long long>(first128[u.group] + (u.n0 - off[u.group]) / 128) * kt * 512;
+                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
+                    if (!ok) break;
+                    const uint32_t at_a = smem_base + s * Cfg::STAGE_BYTES;
+                    const uint32_t at_b = at_a + Cfg::A_BYTES;
+                    const uint32_t at_sa = at_b + Cfg::B_BYTES, at_sb = at_sa + 1024;
+                    const uint32_t sf = 512u * min(2, kt - 2 * kb);  // one or two scale tiles along K in this stage
+                    const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES + sf * (1 + b_tiles);
+                    uint32_t fb = full_bar(s);
+                    if constexpr (kPair) fb = mapa_shared(fb, 0);
+                    if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
+                    if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, kb * 128, u.m0, z, fb);
+                    else if (a_once) tma_load_3d_hint(at_a, &tmA, kb * 128, u.m0, z, fb, once);
+                    else tma_load_3d(at_a, &tmA, kb * 128, u.m0, z, fb);
+                    for (int i = 0; i < boxes; ++i) {
+                        if constexpr (kPair) tma_load_2d_pair(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX, fb);
+                        else tma_load_2d(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX, fb);
+                    }
+                    bulk_load(at_sa, sa + kb * 1024, sf, fb);
+                    for (int i = 0; i < b_tiles; ++i) bulk_load(at_sb + i * 1024, sb + static_cast<long long>(i) * kt * 512 + kb * 1024, sf, fb);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (lane == 0 && cta_rank == 0) {
+            const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
+            const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
+            // 32 rows of 16 bytes, 8-row groups 128 bytes apart
+            const uint64_t ds0 = make_smem_desc(smem_base + Cfg::A_BYTES + Cfg::B_BYTES, 16, 128, kSwizzleNone);
+            int s = 0;
+            uint32_t ph = 0, ucount = 0, set = 0;
+            bool ok = true;
+            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                const Unit u = decode(unit);
+                const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, inst_n(u), 0);
+                const int b_tiles = scale_tiles(u);
+                const uint32_t shift = static_cast<uint32_t>(scale_shift(u)) / 32;
+                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    const uint32_t acc = ucount % ACCS;
+                    const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
+                    const bool end = kb + 1 == u.kb || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
+                    if (begin) {
+                        ok = mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty);
+                        if (!ok) break;
+                    }
+                    ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
+                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + set * Cfg::SCALE_COLS, sfb = sfa + 8;
+                    const int tiles_k = min(2, kt - 2 * kb);
+                    for (int j = 0; j < tiles_k; ++j) {
+                        tmem_cp_scales<kCtas>(sfa + 4 * j, ds0 + step + 32 * j);
+                        for (int i = 0; i < b_tiles; ++i)
+                            tmem_cp_scales<kCtas>(sfb + (j * Cfg::B_TILES + i) * 4, ds0 + step + 64 * (1 + i) + 32 * j);
+                    }
+                    const int steps = min(4, (p.K - kb * Cfg::BK + 63) / 64);
+                    const uint32_t d_tmem = tmem_base + acc * kBN;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (k < steps) {
+                            const uint32_t id = idesc0 | (k & 1 ? (2u << 4) | (2u << 29) : 0u);
+                            umma_mxf4<kCtas>(d_tmem, da0 + step + 2 * k, db0 + step + 2 * k, id, sfa + 4 * (k >> 1),
+                                             sfb + (k >> 1) * Cfg::B_TILES * 4 + shift, (begin && k == 0) ? 0u : 1u);
+                        }
+                    }
+                    set = set + 1 == Cfg::SCALE_SETS ? 0 : set + 1;
+                    if constexpr (kPair) umma_commit_pair(empty_bar(s));
+                    else umma_commit<kCtas>(empty_bar(s));
+                    if (end) {
+                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                        else umma_commit<kCtas>(tmem_full_bar(acc));
+                        ++ucount;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int wg = (warp - 4) >> 2;
+        const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
+        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, Cfg::PROMOTE_KB, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+                                                                           tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
+                                                                           unit_first, unit_stride, num_units, decode);
+    }
+
+    // ---------------------------------------------------------------------- common exit
+    tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag) {
+        const unsigned long long t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+    if constexpr (kPair) cluster_sync_all();
+    if (warp == 2) {
+        tc_fence_after_sync();
+        tmem_dealloc<kCtas>(tmem_base, Cfg::TMEM_COLS);
+    }
+}
+
+}  // namespace b200

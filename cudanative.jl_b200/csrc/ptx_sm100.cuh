@@ -298,6 +298,14 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(uint32_t dst_smem, const C
         : "memory");
 }
 
+// Untiled bulk load of `bytes` (a multiple of 16, both addresses 16-byte aligned) into this CTA's shared
+// memory.  The barrier may be the pair leader's (a shared::cluster address).
+__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, uint32_t bytes, uint32_t bar_cluster_addr) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_smem),
+                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar_cluster_addr)
+                 : "memory");
+}
+
 // 2-D tiled store shared -> global, tracked by this thread's bulk async-group.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, int x, int y,
                                              uint32_t src_smem) {
@@ -475,6 +483,53 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
             "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
             : "memory");
     }
+}
+
+// Instruction descriptor of tcgen05.mma.kind::mxf4.block_scale: 4-bit (E2M1) A and B, both K-major, with
+// one 8-bit power of two (UE8M0) per 32 values of a row, binary32 accumulator.  Bit layout (PTX ISA,
+// "Instruction descriptor" for .kind::mxf4): [4,6) which bytes of a B scale word, [7,10) A format (1 = E2M1),
+// [10,12) B format, [17,23) N >> 3, [23] scale type (1 = UE8M0), [27,29) M >> 7, [29,31) which bytes of
+// an A scale word (0 or 2: an instruction takes two of the four scales).
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int sf_id) {
+    return (static_cast<uint32_t>(sf_id) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+           (static_cast<uint32_t>(m >> 7) << 27) | (static_cast<uint32_t>(sf_id) << 29);
+}
+
+// D[tmem] (+)= (A * scale_a) * (B * scale_b), K = 64; scales in tensor memory (32 lanes x 4 bytes a column,
+// column c holding rows 32 c .. 32 c + 31); issued by ONE thread.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
+                                          uint32_t sfb_tmem, uint32_t accumulate) {
+    if constexpr (kCtaGroup == 1) {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+            : "memory");
+    }
+}
+
+// Shared -> tensor memory: 32 rows of 16 bytes to lanes 0 .. 31 x 4 columns, repeated in every warp's quarter
+// of the lanes.  Ordered before the tcgen05.mma that the same thread issues after it.  With a CTA pair each
+// CTA copies from its own shared memory to its own tensor memory.
+template <int kCtaGroup>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t s_desc) {
+    if constexpr (kCtaGroup == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
 }
 
 // Arrive on an mbarrier once every tcgen05 operation this thread issued so far has completed.

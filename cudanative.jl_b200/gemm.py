@@ -139,6 +139,37 @@ class Handle:
             self._h, stream, M, N, K, float(alpha), a, lda, b, ldb, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type),
             d, ldd, stride_d, _type_code(d_type), _addr(offsets), groups), "gemm_grouped_k")
 
+    def mxfp4_quantize(self, trans: bool, K: int, cols: int, X, ldx: int, x_type, Q, ldq: int, scales, offsets=None, groups: int = 0,
+                       stream=None) -> None:
+        """The K x cols matrix X (trans: its transpose is stored) in blocks of 32 down each column as 4-bit elements
+        ``Q`` with a shared 8-bit power of two each (b200_mxfp4_quantize).  ``scales`` takes
+        ``mxfp4_scale_bytes(K, cols, groups)`` bytes."""
+        _lib.check(_lib.lib().b200_mxfp4_quantize(self._h, stream, int(bool(trans)), K, cols, _addr(X), ldx, _type_code(x_type), _addr(Q), ldq,
+                                                  _addr(scales), _addr(offsets), groups), "mxfp4_quantize")
+
+    def mxfp4_dequantize(self, K: int, cols: int, Q, ldq: int, scales, Y, ldy: int, y_type, offsets=None, groups: int = 0, stream=None) -> None:
+        """The values a 4-bit matrix stands for (b200_mxfp4_dequantize)."""
+        _lib.check(_lib.lib().b200_mxfp4_dequantize(self._h, stream, K, cols, _addr(Q), ldq, _addr(scales), _addr(Y), ldy, _type_code(y_type),
+                                                    _addr(offsets), groups), "mxfp4_dequantize")
+
+    def gemm_mxfp4(self, M: int, N: int, K: int, alpha: float, A, lda: int, a_scales, B, ldb: int, b_scales, beta: float, Cm, ldc: int, c_type,
+                   D, ldd: int, d_type, stream=None) -> None:
+        """``D = alpha*A^T*B + beta*C`` with 4-bit A (K x M) and B (K x N) as ``mxfp4_quantize`` writes them
+        (b200_gemm_mxfp4)."""
+        c = _addr(Cm) if Cm is not None else None
+        _lib.check(_lib.lib().b200_gemm_mxfp4(
+            self._h, stream, M, N, K, float(alpha), _addr(A), lda, _addr(a_scales), _addr(B), ldb, _addr(b_scales), float(beta), c, ldc,
+            _type_code(c_type), _addr(D), ldd, _type_code(d_type)), "gemm_mxfp4")
+
+    def gemm_mxfp4_grouped(self, M: int, N: int, K: int, alpha: float, A, lda: int, stride_a: int, a_scales, B, ldb: int, b_scales, beta: float,
+                           Cm, ldc: int, c_type, D, ldd: int, d_type, offsets, groups: int, stream=None) -> None:
+        """``gemm_grouped`` with 4-bit matrices per group and 4-bit columns, quantised with the same offsets
+        (b200_gemm_mxfp4_grouped)."""
+        c = _addr(Cm) if Cm is not None else None
+        _lib.check(_lib.lib().b200_gemm_mxfp4_grouped(
+            self._h, stream, M, N, K, float(alpha), _addr(A), lda, stride_a, _addr(a_scales), _addr(B), ldb, _addr(b_scales), float(beta), c,
+            ldc, _type_code(c_type), _addr(D), ldd, _type_code(d_type), _addr(offsets), groups), "gemm_mxfp4_grouped")
+
     def gemm_gated(self, transA: bool, transB: bool, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int,
                    beta: float, Cm, ldc: int, D, ldd: int, panel_flags, panel_k: int, stream=None) -> None:
         """``gemm`` whose main loop reads columns [j*panel_k, (j+1)*panel_k) of op(A) only once the
@@ -161,6 +192,11 @@ class Handle:
             self._h, int(bool(transA)), int(bool(transB)), M, N, K, float(alpha), A.ctypes.data, lda,
             B.ctypes.data, ldb, float(beta), Cm.ctypes.data if Cm is not None else None, ldc, D.ctypes.data, ldd),
             "gemm_host")
+
+
+def mxfp4_scale_bytes(K: int, cols: int, groups: int = 0) -> int:
+    """Bytes of the scales of a K x cols 4-bit matrix (b200_mxfp4_scale_bytes)."""
+    return _lib.lib().b200_mxfp4_scale_bytes(K, cols, groups)
 
 
 def _addr(x):

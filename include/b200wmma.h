@@ -224,6 +224,58 @@ int b200_gemm_grouped_k(b200_handle* h, b200_stream stream, int64_t M, int64_t N
                         const void* C, int64_t ldc, int64_t stride_c, int c_type, void* D, int64_t ldd,
                         int64_t stride_d, int d_type, const int32_t* offsets, int64_t groups);
 
+/* ------------------------------------------------------------------------------------------ */
+/* microscaled 4-bit operands                                                                  */
+/* ------------------------------------------------------------------------------------------ */
+
+/* A K x cols matrix of 4-bit values, in blocks of 32 down each column (along K):
+ *   value(k, j) = element(k, j) * 2^(scale(k / 32, j) - 127)
+ * element: 4 bits, sign / 2 exponent / 1 fraction bits: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives;
+ * scale: 8 bits, 255 stands for NaN.  In memory
+ *   elements: column j at byte j * ldq / 2, two to a byte, the even k in the low half; ldq (elements) a
+ *     multiple of 32 and at least K rounded up to 32, 16-byte aligned; 0 behind K;
+ *   scales: tiles of 512 bytes for 128 columns x 4 blocks, column r and block b of a tile at byte
+ *     (r % 32) * 16 + (r / 32) * 4 + b; ceil(K / 128) tiles for columns 0 .. 127, then 128 .. 255, ...;
+ *     16-byte aligned; 0 where a tile has no column or block.
+ * With `offsets` (groups + 1 ascending int32 on the device, as in b200_gemm_grouped) the columns of every
+ * group begin a row of scale tiles of their own, in the order of the groups; elements stay where they are.
+ * Columns of no group are neither read nor written.  offsets = NULL and groups = 0: one plain matrix.
+ *
+ * b200_mxfp4_scale_bytes: bytes that `scales` takes (an upper bound, reached or not, with groups > 0).
+ * b200_mxfp4_quantize: trans = 0: X is K x cols column-major, trans = 1: X is cols x K column-major, i.e.
+ *   its transpose is quantised.  Float16, bfloat16 or Float32.  A block's scale is 2^(floor(log2 max) - 2),
+ *   at least 2^-127; elements are rounded to nearest, ties to even, and saturate at 6.  A block that holds
+ *   a NaN or an infinity gets scale 255.
+ * b200_mxfp4_dequantize: Y (K x cols column-major) = the values, rounded once to y_type. */
+int64_t b200_mxfp4_scale_bytes(int64_t K, int64_t cols, int64_t groups);
+int b200_mxfp4_quantize(b200_handle* h, b200_stream stream, int trans, int64_t K, int64_t cols, const void* X,
+                        int64_t ldx, int x_type, void* Q, int64_t ldq, void* scales, const int32_t* offsets,
+                        int64_t groups);
+int b200_mxfp4_dequantize(b200_handle* h, b200_stream stream, int64_t K, int64_t cols, const void* Q,
+                          int64_t ldq, const void* scales, void* Y, int64_t ldy, int y_type,
+                          const int32_t* offsets, int64_t groups);
+
+/* D = alpha * A^T * B + beta * C with 4-bit A (K x M) and B (K x N), both laid out as above; C and D are
+ * M x N column-major in any of the three types and at any alignment.  One weight matrix [out, in] and
+ * tokens [tokens, in], stored row by row and quantised with trans = 0, give [tokens, out].  lda and ldb
+ * count elements.  Products and sums of a block are exact in the tensor core's wider adder; accumulation
+ * is binary32.  A block with scale 255 makes its row or column of D NaN.  K > 0 unless M or N is 0.  There
+ * is no simple kernel for 4-bit operands: alignment that the layout above rules out is refused. */
+int b200_gemm_mxfp4(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha,
+                    const void* A, int64_t lda, const void* a_scales, const void* B, int64_t ldb,
+                    const void* b_scales, float beta, const void* C, int64_t ldc, int c_type, void* D,
+                    int64_t ldd, int d_type);
+
+/* b200_gemm_grouped with 4-bit operands: D[:, s_e] = alpha * A_e^T * B[:, s_e] + beta * C[:, s_e].
+ * A_e = A + e * stride_a elements (0: one matrix for all groups) with the scales of group e at
+ * a_scales + e * b200_mxfp4_scale_bytes(K, M, 0): as quantised one by one, or all at once as the K x
+ * (groups * M) matrix with offsets 0, M, 2 M, ...  B was quantised with the same offsets. */
+int b200_gemm_mxfp4_grouped(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha,
+                            const void* A, int64_t lda, int64_t stride_a, const void* a_scales,
+                            const void* B, int64_t ldb, const void* b_scales, float beta, const void* C,
+                            int64_t ldc, int c_type, void* D, int64_t ldd, int d_type,
+                            const int32_t* offsets, int64_t groups);
+
 /* b200_gemm_f16f32 whose main loop may start before all of A is in this GPU's memory: columns
  * [j*panel_k, (j+1)*panel_k) of op(A) are read only once the 32-bit word panel_flags[j] (device
  * memory) is non-zero.  panel_k is a multiple of 64; at most 32 panels.  The words are meant to
