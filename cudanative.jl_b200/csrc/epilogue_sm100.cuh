@@ -55,7 +55,7 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) 
 
 // Runs in warps 4 .. 11 (`wg` 0 or 1).  Barriers: tmem_full / tmem_empty [kAccs] at the given addresses,
 // 8 bytes apart; cfull [BUFS] of this warp group.
-template <class E, int kBN, int kAccs, int kCtas, bool kPromote, int kPromoteKb, bool kPerGroup, class Decode>
+template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, class Decode>
 __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUtensorMap* tmC, const CUtensorMap* tmD, int wg, uint32_t tmem_base,
                                              uint32_t epi_base, uint8_t* epi_gen, uint32_t tmem_full, uint32_t tmem_empty, uint32_t cfull,
                                              const WaitCtx& wc, int unit_first, int unit_stride, int num_units, Decode decode) {
@@ -68,7 +68,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
     const bool has_c = p.beta != 0.0f;
     const bool c_bulk = E::BULK_C && has_c && p.c_tma;
     const float alpha = p.alpha, beta = p.beta;
-    const int d_fmt = kPromote ? 0 : p.d_fmt;
+    const int d_fmt = kF32 ? 0 : p.d_fmt;
     const bool c_half = p.c_fmt != 0, d_half = d_fmt != 0;
     const uint32_t c_chunk_bytes = 128 * W * (c_half ? 2 : 4);
     const bool two_phase = c_bulk && (c_half != d_half);
@@ -206,7 +206,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
             }
         };
 
-        if constexpr (kPromote) {
+        if constexpr (kPromoteKb > 0) {
             float sum[E::COLS];
 #pragma unroll
             for (int i = 0; i < E::COLS; ++i) sum[i] = 0.0f;

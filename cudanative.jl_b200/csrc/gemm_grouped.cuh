@@ -404,7 +404,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     } else if (warp >= 4) {
         const int wg = (warp - 4) >> 2;
         const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, 2, kCtas, kPromote, Cfg::PROMOTE_KB, kRaggedK>(p.e, &tmC, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK>(p.e, &tmC, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
                                                                            tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
                                                                            unit_first, unit_stride, num_units, decode);
     }

@@ -21,7 +21,7 @@ struct MxProblem {
 };
 
 template <int kBN, int kCtas, bool kPromote>
-int launch(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     using Cfg = MxCfg<kBN, kCtas, kPromote>;
     auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
@@ -45,12 +45,12 @@ int launch(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cudaStre
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], p));
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], tm[4], p));
     return B200_OK;
 }
 
 template <int kBN, int kCtas>
-int launch_typed(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch_typed(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     if (p.e.d_fmt == 0) {
         if constexpr (MxCfg<kBN, kCtas, true>::ACCS == 2) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
         else return fail(B200_UNSUPPORTED, "mxfp4: a binary32 D takes tiles of 128 columns at most");
@@ -60,6 +60,9 @@ int launch_typed(const CUtensorMap (&tm)[3], const MxGemmParams& p, int grid, cu
 
 int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     int tile_n = 128, pair = 1, rc;
+    if (h->tile_n) tile_n = h->tile_n == 64 ? 192 : h->tile_n;
+    if (h->cta_pair) pair = h->cta_pair;
+    if (tile_n == 256 && g.d_type == B200_F32) tile_n = 128;
     MxGemmParams p = {};
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
@@ -68,9 +71,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
     p.offsets = g.offsets;
     p.a_per_group = g.stride_a != 0 ? 1 : 0;
-    p.sa = static_cast<const uint8_t*>(g.SA);
-    p.sb = static_cast<const uint8_t*>(g.SB);
-    p.sa_stride = (g.M + 127) / 128 * ((g.K + 127) / 128) * 512;
+    p.sa_tiles = static_cast<int>(b200_mxfp4_scale_bytes(g.K, g.M, 0) / 512);
     p.e.M = static_cast<int>(g.M);
     p.e.alpha = g.alpha;
     p.e.beta = g.beta;
@@ -87,14 +88,22 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
 
     const int bn_local = tile_n / pair, bbox = bn_local % 64 == 0 ? 64 : 32;
     const int64_t k_bytes = (g.K + 1) / 2;
-    CUtensorMap tm[3];
+    CUtensorMap tm[5];
     BatchDim b;
     b.count = g.stride_a != 0 ? g.groups : 1;
     b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
     if ((rc = make_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
     if ((rc = make_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
-    tm[2] = tm[1];  // never dereferenced unless replaced
-    if (p.e.d_tma && (rc = make_map_2d(&tm[2], map_type(g.d_type), elem_bytes(g.d_type), g.D, g.M, g.N, g.ldd, 128, g.d_type == B200_F32 ? 16 : 32,
+    // scales: one tile of 512 bytes per row of the map, two to a copy
+    const int64_t sa_tiles = static_cast<int64_t>(p.sa_tiles) * b.count;
+    const int64_t sb_tiles = b200_mxfp4_scale_bytes(g.K, g.N, g.offsets ? g.groups : 0) / 512;
+    if (sa_tiles > 0x7fffff00ll || sb_tiles > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many scale tiles");
+    auto scale_map = [&](CUtensorMap* m, const void* ptr, int64_t tiles, const char* what) {
+        return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, tiles, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what);
+    };
+    if ((rc = scale_map(&tm[2], g.SA, sa_tiles, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_tiles, "scales of B"))) return rc;
+    tm[4] = tm[1];  // never dereferenced unless replaced
+    if (p.e.d_tma && (rc = make_map_2d(&tm[4], map_type(g.d_type), elem_bytes(g.d_type), g.D, g.M, g.N, g.ldd, 128, g.d_type == B200_F32 ? 16 : 32,
                                        CU_TENSOR_MAP_SWIZZLE_NONE, "D")))
         return rc;
 
@@ -102,7 +111,10 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
     const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
-    if ((rc = launch_typed<128, 1>(tm, p, grid, stream, h->pdl != 0))) return rc;
+    const bool pdl = h->pdl != 0;
+    if (pair == 2) rc = tile_n == 256 ? launch_typed<256, 2>(tm, p, grid, stream, pdl) : tile_n == 192 ? launch_typed<192, 2>(tm, p, grid, stream, pdl) : launch_typed<128, 2>(tm, p, grid, stream, pdl);
+    else rc = tile_n == 256 ? launch_typed<256, 1>(tm, p, grid, stream, pdl) : launch_typed<128, 1>(tm, p, grid, stream, pdl);
+    if (rc) return rc;
     h->last = {B200_KERNEL_TCGEN05, tile_n, 1, grid, pair};
     return B200_OK;
 }

@@ -7,7 +7,7 @@
 //
 // The pipeline is that of gemm_grouped.cuh with 256 values of k (128 bytes of elements) per stage, four
 // tcgen05.mma.kind::mxf4.block_scale of K = 64 each, and the stage's scales: one 512-byte tile per 128 rows
-// and 128 values of k, brought by a plain bulk copy and moved to tensor memory by tcgen05.cp in front of the
+// and 128 values of k, brought by bulk copies of its own and moved to tensor memory by tcgen05.cp in front of the
 // products that use them.  Copies and products of one thread run in order, so a set of scale columns can be
 // written again without a barrier; kScaleSets sets keep a copy from waiting for the products before it.
 //
@@ -30,9 +30,7 @@ struct MxGemmParams {
     int raster_group;
     const int* offsets;  // nullptr: one group, all columns
     int a_per_group;
-    const uint8_t* sa;
-    const uint8_t* sb;
-    long long sa_stride;  // bytes between the scales of A_e and A_{e+1}
+    int sa_tiles;        // scale tiles (of 512 bytes) of one A_e
     EpilogueParams e;
     int* status;
     unsigned long long wait_budget_ns;
@@ -75,6 +73,7 @@ struct MxCfg {
 template <int kBN, int kCtas, bool kPromote>
 __global__ void __launch_bounds__(384, 1)
 gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                    const __grid_constant__ CUtensorMap tmD, const MxGemmParams p) {
     using Cfg = MxCfg<kBN, kCtas, kPromote>;
     using Epi = typename Cfg::Epi;
@@ -121,6 +120,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
+        tma_prefetch_desc(&tmSA);
+        tma_prefetch_desc(&tmSB);
         tma_prefetch_desc(&tmD);
     }
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
@@ -182,28 +183,29 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 const int z = u.group * p.a_per_group;
                 // a CTA of a pair may own no rows of A: its scales are then those of the last rows
                 const int a_tile = min(u.m0, (p.e.M - 1) / 128 * 128) / 128;
-                const uint8_t* sa = p.sa + z * p.sa_stride + static_cast<long long>(a_tile) * kt * 512;
-                const uint8_t* sb = p.sb + static_cast<long long>(first128[u.group] + (u.n0 - off[u.group]) / 128) * kt * 512;
+                const int sa = z * p.sa_tiles + a_tile * kt;
+                const int sb = (first128[u.group] + (u.n0 - off[u.group]) / 128) * kt;
+                // a stage's scales are two tiles along K; behind an odd last one stands a tile that is not used
+                const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES + 1024 * (1 + b_tiles);
                 for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
                     if (!ok) break;
                     const uint32_t at_a = smem_base + s * Cfg::STAGE_BYTES;
                     const uint32_t at_b = at_a + Cfg::A_BYTES;
                     const uint32_t at_sa = at_b + Cfg::B_BYTES, at_sb = at_sa + 1024;
-                    const uint32_t sf = 512u * min(2, kt - 2 * kb);  // one or two scale tiles along K in this stage
-                    const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES + sf * (1 + b_tiles);
                     uint32_t fb = full_bar(s);
                     if constexpr (kPair) fb = mapa_shared(fb, 0);
                     if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
                     if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, kb * 128, u.m0, z, fb);
                     else if (a_once) tma_load_3d_hint(at_a, &tmA, kb * 128, u.m0, z, fb, once);
                     else tma_load_3d(at_a, &tmA, kb * 128, u.m0, z, fb);
-                    for (int i = 0; i < boxes; ++i) {
-                        if constexpr (kPair) tma_load_2d_pair(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX, fb);
-                        else tma_load_2d(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX, fb);
-                    }
-                    bulk_load(at_sa, sa + kb * 1024, sf, fb);
-                    for (int i = 0; i < b_tiles; ++i) bulk_load(at_sb + i * 1024, sb + static_cast<long long>(i) * kt * 512 + kb * 1024, sf, fb);
+                    auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
+                        if constexpr (kPair) tma_load_2d_pair(dst, tm, x, y, fb);
+                        else tma_load_2d(dst, tm, x, y, fb);
+                    };
+                    for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX);
+                    load(at_sa, &tmSA, 0, sa + 2 * kb);
+                    for (int i = 0; i < b_tiles; ++i) load(at_sb + i * 1024, &tmSB, 0, sb + i * kt + 2 * kb);
                 }
             }
         }
@@ -267,7 +269,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     } else if (warp >= 4) {
         const int wg = (warp - 4) >> 2;
         const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, Cfg::PROMOTE_KB, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? (1 << 30) : 0, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
                                                                            tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
                                                                            unit_first, unit_stride, num_units, decode);
     }

@@ -298,14 +298,6 @@ __device__ __forceinline__ void tma_load_2d_pair_hint(uint32_t dst_smem, const C
         : "memory");
 }
 
-// Untiled bulk load of `bytes` (a multiple of 16, both addresses 16-byte aligned) into this CTA's shared
-// memory.  The barrier may be the pair leader's (a shared::cluster address).
-__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void* src, uint32_t bytes, uint32_t bar_cluster_addr) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_smem),
-                 "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar_cluster_addr)
-                 : "memory");
-}
-
 // 2-D tiled store shared -> global, tracked by this thread's bulk async-group.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, int x, int y,
                                              uint32_t src_smem) {
