@@ -7,9 +7,11 @@
 //
 // The pipeline is that of gemm_grouped.cuh with 256 values of k (128 bytes of elements) per stage, four
 // tcgen05.mma.kind::mxf4.block_scale of K = 64 each, and the stage's scales: one 512-byte tile per 128 rows
-// and 128 values of k, brought by bulk copies of its own and moved to tensor memory by tcgen05.cp in front of the
-// products that use them.  Copies and products of one thread run in order, so a set of scale columns can be
-// written again without a barrier; kScaleSets sets keep a copy from waiting for the products before it.
+// and 128 values of k, brought by bulk copies of its own.  The products read scales from tensor memory, the
+// same 32 lanes repeated in each warp's quarter: four more warps (12 - 15) carry them there, one quarter each,
+// a set of columns per stage.  (tcgen05.cp does the same from the MMA issuer's thread, but holds up the
+// products behind it by about 80 cycles a tile, six tiles to 512 cycles of products: 8192^3 took 370 us
+// instead of 224 us without it; issued one stage ahead 437 us.)
 //
 // A tile's scales always come from whole tiles of 128 columns, counted from the group's first column, as
 // they were quantised.  A tile of kBN columns starts inside one where kBN is no multiple of 128: the
@@ -38,7 +40,7 @@ struct MxGemmParams {
 
 template <int kBN, int kCtas, bool kPromote>
 struct MxCfg {
-    static constexpr int THREADS = 384;
+    static constexpr int THREADS = 512;
     static constexpr int BM = 128;
     static constexpr int BK = 256;  // values of k per stage
     static constexpr int BN_LOCAL = kBN / kCtas;
@@ -59,11 +61,10 @@ struct MxCfg {
     static constexpr int ACCS = kBN <= 192 ? 2 : 1;
     static constexpr int SCALE_COLS = 8 * (1 + B_TILES);  // per set: 2 x 4 for A, 2 x 4 per scale tile for B
     static constexpr int SCALE_AT = ACCS * kBN;
-    static constexpr int SCALE_SETS = (512 - SCALE_AT) / SCALE_COLS >= 4 ? 4 : 2;
-    static constexpr int USED_COLS = SCALE_AT + SCALE_SETS * SCALE_COLS;
+    static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 2 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
+    static constexpr int NBARS = 4 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
@@ -71,7 +72,7 @@ struct MxCfg {
 };
 
 template <int kBN, int kCtas, bool kPromote>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(512, 1)
 gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                    const __grid_constant__ CUtensorMap tmD, const MxGemmParams p) {
@@ -94,9 +95,11 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
-    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
-    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + ACCS + a); };
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (2 * STAGES + 2 * ACCS + b); };
+    auto scales_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };   // in this CTA's shared memory
+    auto scales_ready_bar = [&](int s) { return bar_base + 8u * (3 * STAGES + s); };  // in tensor memory (of both CTAs)
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + ACCS + a); };
+    auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 2 * ACCS + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
@@ -112,6 +115,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
+            mbar_init(scales_full_bar(s), 1);
+            mbar_init(scales_ready_bar(s), 4 * kCtas);
         }
         for (int a = 0; a < ACCS; ++a) {
             mbar_init(tmem_full_bar(a), 1);
@@ -186,7 +191,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 const int sa = z * p.sa_tiles + a_tile * kt;
                 const int sb = (first128[u.group] + (u.n0 - off[u.group]) / 128) * kt;
                 // a stage's scales are two tiles along K; behind an odd last one stands a tile that is not used
-                const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES + 1024 * (1 + b_tiles);
+                const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
                 for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
                     if (!ok) break;
@@ -204,8 +209,10 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         else tma_load_2d(dst, tm, x, y, fb);
                     };
                     for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX);
-                    load(at_sa, &tmSA, 0, sa + 2 * kb);
-                    for (int i = 0; i < b_tiles; ++i) load(at_sb + i * 1024, &tmSB, 0, sb + i * kt + 2 * kb);
+                    const uint32_t sf = scales_full_bar(s);
+                    mbar_arrive_expect_tx(sf, 1024 * (1 + b_tiles));
+                    tma_load_2d(at_sa, &tmSA, 0, sa + 2 * kb, sf);
+                    for (int i = 0; i < b_tiles; ++i) tma_load_2d(at_sb + i * 1024, &tmSB, 0, sb + i * kt + 2 * kb, sf);
                 }
             }
         }
@@ -215,15 +222,12 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (lane == 0 && cta_rank == 0) {
             const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
             const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
-            // 32 rows of 16 bytes, 8-row groups 128 bytes apart
-            const uint64_t ds0 = make_smem_desc(smem_base + Cfg::A_BYTES + Cfg::B_BYTES, 16, 128, kSwizzleNone);
             int s = 0;
-            uint32_t ph = 0, ucount = 0, set = 0;
+            uint32_t ph = 0, ucount = 0;
             bool ok = true;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
                 const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, inst_n(u), 0);
-                const int b_tiles = scale_tiles(u);
                 const uint32_t shift = static_cast<uint32_t>(scale_shift(u)) / 32;
                 for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     const uint32_t acc = ucount % ACCS;
@@ -233,17 +237,11 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         ok = mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty);
                         if (!ok) break;
                     }
-                    ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
+                    ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage) && mbar_wait(scales_ready_bar(s), ph, wc, kWaitScales);
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + set * Cfg::SCALE_COLS, sfb = sfa + 8;
-                    const int tiles_k = min(2, kt - 2 * kb);
-                    for (int j = 0; j < tiles_k; ++j) {
-                        tmem_cp_scales<kCtas>(sfa + 4 * j, ds0 + step + 32 * j);
-                        for (int i = 0; i < b_tiles; ++i)
-                            tmem_cp_scales<kCtas>(sfb + (j * Cfg::B_TILES + i) * 4, ds0 + step + 64 * (1 + i) + 32 * j);
-                    }
+                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
                     const int steps = min(4, (p.K - kb * Cfg::BK + 63) / 64);
                     const uint32_t d_tmem = tmem_base + acc * kBN;
 #pragma unroll
@@ -254,7 +252,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                                              sfb + (k >> 1) * Cfg::B_TILES * 4 + shift, (begin && k == 0) ? 0u : 1u);
                         }
                     }
-                    set = set + 1 == Cfg::SCALE_SETS ? 0 : set + 1;
                     if constexpr (kPair) umma_commit_pair(empty_bar(s));
                     else umma_commit<kCtas>(empty_bar(s));
                     if (end) {
@@ -262,6 +259,42 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         else umma_commit<kCtas>(tmem_full_bar(acc));
                         ++ucount;
                     }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------------ scales: shared -> tensor memory
+        const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        const int kb_total = (p.K + Cfg::BK - 1) / Cfg::BK;
+        for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+            for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                ok = mbar_wait(scales_full_bar(s), ph, wc, kWaitScales);
+                ok = __all_sync(0xffffffffu, ok);  // tcgen05.st is warp-collective
+                if (!ok) break;
+                // the stage's columns of tensor memory are free: its loads were issued after the products that
+                // last read them.  Tiles that were not loaded hold old bytes that no product reads.
+                const uint8_t* tiles = smem_gen + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES + lane * 16;
+                const uint32_t sfa = tmem_base + quarter + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
+                uint4 r[2 * (1 + Cfg::B_TILES)];
+#pragma unroll
+                for (int i = 0; i < 2 * (1 + Cfg::B_TILES); ++i) r[i] = *reinterpret_cast<const uint4*>(tiles + i * 512);
+                tmem_st_32x32b_x4(sfa, r[0]);
+                tmem_st_32x32b_x4(sfa + 4, r[1]);
+#pragma unroll
+                for (int i = 0; i < Cfg::B_TILES; ++i) {
+                    tmem_st_32x32b_x4(sfb + i * 4, r[2 + 2 * i]);
+                    tmem_st_32x32b_x4(sfb + (Cfg::B_TILES + i) * 4, r[3 + 2 * i]);
+                }
+                tmem_wait_st();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (kPair) mbar_arrive_cluster_relaxed(scales_ready_bar(s), 0);
+                    else mbar_arrive(scales_ready_bar(s));
                 }
             }
         }

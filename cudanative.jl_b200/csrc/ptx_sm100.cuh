@@ -65,6 +65,20 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t cta_r
         : "memory");
 }
 
+// The same without release semantics for memory: for a signal that says only that this warp's tensor-memory
+// stores have completed (tcgen05.wait::st, tcgen05.fence::before_thread_sync).  A release at cluster scope
+// waits for all of the thread's memory operations, about 0.5 us.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar, uint32_t cta_rank) {
+    asm volatile(
+        "{\n"
+        ".reg .b32 remote;\n"
+        "mapa.shared::cluster.u32 remote, %0, %1;\n"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [remote];\n"
+        "}" ::"r"(bar),
+        "r"(cta_rank)
+        : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
@@ -109,6 +123,7 @@ enum : int {
     kWaitSelftest = 107,     // the bounded-wait self test (nothing ever arrives)
     kWaitPanel = 108,        // producer waiting for a panel of A to arrive in this GPU's memory
     kWaitTail = 109,         // grouped product: the last k-block of a group, zeros behind its end
+    kWaitScales = 111,       // 4-bit product: a stage's scales, in shared or in tensor memory
     kBadOffsets = 110        // not a wait: a group's offsets decrease or leave the matrix
 };
 
@@ -513,17 +528,6 @@ __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint
     }
 }
 
-// Shared -> tensor memory: 32 rows of 16 bytes to lanes 0 .. 31 x 4 columns, repeated in every warp's quarter
-// of the lanes.  Ordered before the tcgen05.mma that the same thread issues after it.  With a CTA pair each
-// CTA copies from its own shared memory to its own tensor memory.
-template <int kCtaGroup>
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t s_desc) {
-    if constexpr (kCtaGroup == 1)
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
-    else
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
-}
-
 // Arrive on an mbarrier once every tcgen05 operation this thread issued so far has completed.
 // `bar` is a shared::cluster address: a plain shared::cta address names this CTA's own barrier,
 // a mapa-translated one names a peer CTA's.
@@ -595,6 +599,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
         "r"(r[15])
         : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x4(uint32_t taddr, uint4 r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tmem_wait_ld() {
