@@ -63,6 +63,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     if (h->tile_n) tile_n = h->tile_n == 64 ? 192 : h->tile_n;
     if (h->cta_pair) pair = h->cta_pair;
     if (tile_n == 256 && g.d_type == B200_F32) tile_n = 128;
+    if (tile_n == 192) pair = 2;
     MxGemmParams p = {};
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
@@ -71,7 +72,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
     p.offsets = g.offsets;
     p.a_per_group = g.stride_a != 0 ? 1 : 0;
-    p.sa_tiles = static_cast<int>(b200_mxfp4_scale_bytes(g.K, g.M, 0) / 512);
+    p.a_tile_rows = static_cast<int>((g.M + 127) / 128);
     p.e.M = static_cast<int>(g.M);
     p.e.alpha = g.alpha;
     p.e.beta = g.beta;
@@ -86,7 +87,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     const int q = 16 / elem_bytes(g.d_type);
     p.e.d_tma = !(reinterpret_cast<uintptr_t>(g.D) & 15u) && g.ldd % q == 0 && g.M % q == 0;
 
-    const int bn_local = tile_n / pair, bbox = bn_local % 64 == 0 ? 64 : 32;
+    const int bn_local = tile_n / pair, bbox = bn_local % 128 == 0 ? 128 : bn_local % 64 == 0 ? 64 : 32;
     const int64_t k_bytes = (g.K + 1) / 2;
     CUtensorMap tm[5];
     BatchDim b;
@@ -94,14 +95,18 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
     if ((rc = make_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
     if ((rc = make_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
-    // scales: one tile of 512 bytes per row of the map, two to a copy
-    const int64_t sa_tiles = static_cast<int64_t>(p.sa_tiles) * b.count;
-    const int64_t sb_tiles = b200_mxfp4_scale_bytes(g.K, g.N, g.offsets ? g.groups : 0) / 512;
-    if (sa_tiles > 0x7fffff00ll || sb_tiles > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many scale tiles");
-    auto scale_map = [&](CUtensorMap* m, const void* ptr, int64_t tiles, const char* what) {
-        return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, tiles, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what);
+    // scales: tiles of 128 words, K tiles, rows of tiles; a copy takes 2 along K
+    const int64_t kt = (g.K + 127) / 128, sa_rows = p.a_tile_rows * b.count;
+    const int64_t sb_rows = b200_mxfp4_scale_bytes(g.K, g.N, g.offsets ? g.groups : 0) / 512 / kt;
+    if (sa_rows > 0x7fffff00ll || sb_rows > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many scale tiles");
+    auto scale_map = [&](CUtensorMap* m, const void* ptr, int64_t rows, uint32_t box_rows, const char* what) {
+        BatchDim d;
+        d.count = rows;
+        d.stride = kt * 128;
+        d.box = box_rows;
+        return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
     };
-    if ((rc = scale_map(&tm[2], g.SA, sa_tiles, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_tiles, "scales of B"))) return rc;
+    if ((rc = scale_map(&tm[2], g.SA, sa_rows, 1, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, (tile_n + 127) / 128, "scales of B"))) return rc;
     tm[4] = tm[1];  // never dereferenced unless replaced
     if (p.e.d_tma && (rc = make_map_2d(&tm[4], map_type(g.d_type), elem_bytes(g.d_type), g.D, g.M, g.N, g.ldd, 128, g.d_type == B200_F32 ? 16 : 32,
                                        CU_TENSOR_MAP_SWIZZLE_NONE, "D")))

@@ -32,7 +32,7 @@ struct MxGemmParams {
     int raster_group;
     const int* offsets;  // nullptr: one group, all columns
     int a_per_group;
-    int sa_tiles;        // scale tiles (of 512 bytes) of one A_e
+    int a_tile_rows;     // rows of scale tiles of one A_e
     EpilogueParams e;
     int* status;
     unsigned long long wait_budget_ns;
@@ -49,7 +49,7 @@ struct MxCfg {
     static constexpr int B_TILES = (kBN + 127) / 128;  // scale tiles that a tile of columns touches at most
     static constexpr int SF_BYTES = 1024 * (1 + B_TILES);
     static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES + SF_BYTES + 1023) / 1024 * 1024;
-    static constexpr int BBOX = BN_LOCAL % 64 == 0 ? 64 : 32;
+    static constexpr int BBOX = BN_LOCAL % 128 == 0 ? 128 : BN_LOCAL % 64 == 0 ? 64 : 32;
     static constexpr int BBOX_BYTES = BBOX * BK / 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
     static constexpr int PROMOTE_KB = 8;
@@ -146,7 +146,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __threadfence();
     }
     const int num_units = offsets_ok ? first[p.groups] * p.tiles_m : 0;
-    const int kt = (p.K + 127) / 128;  // scale tiles along K
 
     auto decode = [&](int unit) {
         Unit u;
@@ -169,7 +168,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
     // of a tile's first column among the 128 of its scale tile
     auto scale_shift = [&](const Unit& u) { return (u.n0 - off[u.group]) & 127; };
-    auto scale_tiles = [&](const Unit& u) { return (scale_shift(u) + u.cols + 127) / 128; };
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -183,21 +181,14 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 const int ninst = inst_n(u);
                 const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
                 const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
-                const int b_tiles = scale_tiles(u);
                 const bool a_once = first[u.group + 1] - first[u.group] == 1;
                 const int z = u.group * p.a_per_group;
-                // a CTA of a pair may own no rows of A: its scales are then those of the last rows
-                const int a_tile = min(u.m0, (p.e.M - 1) / 128 * 128) / 128;
-                const int sa = z * p.sa_tiles + a_tile * kt;
-                const int sb = (first128[u.group] + (u.n0 - off[u.group]) / 128) * kt;
-                // a stage's scales are two tiles along K; behind an odd last one stands a tile that is not used
                 const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
                 for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
                     if (!ok) break;
                     const uint32_t at_a = smem_base + s * Cfg::STAGE_BYTES;
                     const uint32_t at_b = at_a + Cfg::A_BYTES;
-                    const uint32_t at_sa = at_b + Cfg::B_BYTES, at_sb = at_sa + 1024;
                     uint32_t fb = full_bar(s);
                     if constexpr (kPair) fb = mapa_shared(fb, 0);
                     if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
@@ -209,10 +200,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         else tma_load_2d(dst, tm, x, y, fb);
                     };
                     for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX);
-                    const uint32_t sf = scales_full_bar(s);
-                    mbar_arrive_expect_tx(sf, 1024 * (1 + b_tiles));
-                    tma_load_2d(at_sa, &tmSA, 0, sa + 2 * kb, sf);
-                    for (int i = 0; i < b_tiles; ++i) tma_load_2d(at_sb + i * 1024, &tmSB, 0, sb + i * kt + 2 * kb, sf);
                 }
             }
         }
@@ -263,6 +250,31 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             }
         }
         __syncwarp();
+    } else if (warp == 3) {
+        // ------------------------------------------------------------------ TMA producer of the scales
+        // A thread of its own: with the scales' copies in warp 0 its issue rate bounds the pipeline.
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                const Unit u = decode(unit);
+                // a CTA of a pair may own no rows of A: its scales are then those of the last rows
+                const int a_row = u.group * p.a_per_group * p.a_tile_rows + min(u.m0 / 128, p.a_tile_rows - 1);
+                const int b_row = first128[u.group] + (u.n0 - off[u.group]) / 128;
+                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
+                    if (!ok) break;
+                    const uint32_t at = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES;
+                    // two tiles along K (behind an odd last one: zeros), B_TILES along the columns; tiles that
+                    // this tile's columns do not touch are loaded and not used
+                    mbar_arrive_expect_tx(scales_full_bar(s), Cfg::SF_BYTES);
+                    tma_load_3d(at, &tmSA, 0, 2 * kb, a_row, scales_full_bar(s));
+                    tma_load_3d(at + 1024, &tmSB, 0, 2 * kb, b_row, scales_full_bar(s));
+                }
+            }
+        }
+        __syncwarp();
     } else if (warp >= 12) {
         // ------------------------------------------------------------------ scales: shared -> tensor memory
         const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -276,7 +288,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 ok = __all_sync(0xffffffffu, ok);  // tcgen05.st is warp-collective
                 if (!ok) break;
                 // the stage's columns of tensor memory are free: its loads were issued after the products that
-                // last read them.  Tiles that were not loaded hold old bytes that no product reads.
+                // last read them
                 const uint8_t* tiles = smem_gen + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES + lane * 16;
                 const uint32_t sfa = tmem_base + quarter + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
                 uint4 r[2 * (1 + Cfg::B_TILES)];

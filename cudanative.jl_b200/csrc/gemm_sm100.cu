@@ -35,11 +35,11 @@ EncodeFn get_encode_fn() {
 struct MapKey {
     const void* base;
     int64_t inner, outer, ld, batch_count, batch_stride;
-    uint32_t box_inner, box_outer;
+    uint32_t box_inner, box_outer, box_batch;
     int dt, sw;
     bool operator==(const MapKey& o) const {
         return base == o.base && inner == o.inner && outer == o.outer && ld == o.ld && batch_count == o.batch_count &&
-               batch_stride == o.batch_stride && box_inner == o.box_inner && box_outer == o.box_outer && dt == o.dt && sw == o.sw;
+               batch_stride == o.batch_stride && box_inner == o.box_inner && box_outer == o.box_outer && box_batch == o.box_batch && dt == o.dt && sw == o.sw;
     }
 };
 struct MapCache {
@@ -81,7 +81,7 @@ thread_local MapCache g_map_cache;
 int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
                 int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
                 const char* what, BatchDim batch) {
-    const MapKey mk{base, inner, outer, ld, batch.count, batch.stride, box_inner, box_outer, static_cast<int>(dt), static_cast<int>(sw)};
+    const MapKey mk{base, inner, outer, ld, batch.count, batch.stride, box_inner, box_outer, batch.box, static_cast<int>(dt), static_cast<int>(sw)};
     if (const CUtensorMap* hit = g_map_cache.find(mk)) {
         *tm = *hit;
         return B200_OK;
@@ -91,7 +91,7 @@ int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const v
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer),
                           static_cast<cuuint64_t>(batch.count)};
     cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * elem_bytes, static_cast<cuuint64_t>(batch.stride) * elem_bytes};
-    cuuint32_t box[3] = {box_inner, box_outer, 1};
+    cuuint32_t box[3] = {box_inner, box_outer, batch.box};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(tm, dt, batch.count > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE,
