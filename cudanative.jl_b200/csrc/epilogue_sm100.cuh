@@ -53,6 +53,8 @@ struct EpilogueCfg {
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
 __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 
+constexpr int kDrain = 1 << 30;  // kPromoteKb: one accumulator per tile, moved to registers before the rest
+
 // Runs in warps 4 .. 11 (`wg` 0 or 1).  Barriers: tmem_full / tmem_empty [kAccs] at the given addresses,
 // 8 bytes apart; cfull [BUFS] of this warp group.
 template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, class Decode>
@@ -206,7 +208,30 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
             }
         };
 
-        if constexpr (kPromoteKb > 0) {
+        if constexpr (kPromoteKb >= kDrain) {
+            // one accumulator in tensor memory: read it out at once and let the next tile begin
+            uint32_t r[E::COLS / W][W];
+            const uint32_t acc = acc_count % kAccs;
+            ok = ok && mbar_wait(tmem_full + 8 * acc, (acc_count / kAccs) & 1u, wc, kWaitTmemFull);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after_sync();
+            if (ok) {
+#pragma unroll
+                for (int q = 0; q < E::COLS / W; ++q)
+                    if (q * W < cols) tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
+                tmem_wait_ld();
+            }
+            release(acc);
+            ++acc_count;
+#pragma unroll
+            for (int q = 0; q < E::COLS / W; ++q) {
+                if (!fail && q * W < cols) {
+                    buffer_ready();
+                    finish(q, r[q]);
+                }
+            }
+            if (fail) break;
+        } else if constexpr (kPromoteKb > 0) {
             float sum[E::COLS];
 #pragma unroll
             for (int i = 0; i < E::COLS; ++i) sum[i] = 0.0f;

@@ -64,7 +64,7 @@ struct MxCfg {
     static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 4 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
+    static constexpr int NBARS = 3 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
@@ -96,10 +96,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     auto full_bar = [&](int s) { return bar_base + 8u * s; };
     auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
     auto scales_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };   // in this CTA's shared memory
-    auto scales_ready_bar = [&](int s) { return bar_base + 8u * (3 * STAGES + s); };  // in tensor memory (of both CTAs)
-    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
-    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + ACCS + a); };
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 2 * ACCS + b); };
+    auto tmem_full_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + a); };
+    auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + ACCS + a); };
+    auto cfull_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
@@ -113,10 +112,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(full_bar(s), 1);
+            mbar_init(full_bar(s), 1 + 4 * kCtas);  // the leader's producer; the warps that carry scales
             mbar_init(empty_bar(s), 1);
             mbar_init(scales_full_bar(s), 1);
-            mbar_init(scales_ready_bar(s), 4 * kCtas);
         }
         for (int a = 0; a < ACCS; ++a) {
             mbar_init(tmem_full_bar(a), 1);
@@ -169,6 +167,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     // of a tile's first column among the 128 of its scale tile
     auto scale_shift = [&](const Unit& u) { return (u.n0 - off[u.group]) & 127; };
 
+    // registers: 4 x 128 a thread at launch = 2 x 56 + 2 x 200; the epilogue holds half a tile row in them
+    if (warp < 4) {
+    regs_dec<56>();
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
         if (lane == 0) {
@@ -211,7 +212,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
             int s = 0;
             uint32_t ph = 0, ucount = 0;
-            bool ok = true;
+            bool ok = true, ready = false;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
                 const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, inst_n(u), 0);
@@ -224,9 +225,12 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         ok = mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty);
                         if (!ok) break;
                     }
-                    ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage) && mbar_wait(scales_ready_bar(s), ph, wc, kWaitScales);
+                    if (!ready) ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
                     if (!ok) break;
                     tc_fence_after_sync();
+                    // look at the next stage now: the answer arrives while this one's products are issued
+                    const int s1 = s + 1 == STAGES ? 0 : s + 1;
+                    ready = mbar_test(full_bar(s1), ph ^ (s1 == 0));
                     const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
                     const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
                     const int steps = min(4, (p.K - kb * Cfg::BK + 63) / 64);
@@ -275,7 +279,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             }
         }
         __syncwarp();
+    }
     } else if (warp >= 12) {
+        regs_dec<56>();
         // ------------------------------------------------------------------ scales: shared -> tensor memory
         const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
         int s = 0;
@@ -305,16 +311,17 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (kPair) mbar_arrive_cluster_relaxed(scales_ready_bar(s), 0);
-                    else mbar_arrive(scales_ready_bar(s));
+                    if constexpr (kPair) mbar_arrive_cluster_relaxed(full_bar(s), 0);
+                    else mbar_arrive(full_bar(s));
                 }
             }
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else {
+        regs_inc<200>();
         const int wg = (warp - 4) >> 2;
         const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? (1 << 30) : 0, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? kDrain : 0, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
                                                                            tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
                                                                            unit_first, unit_stride, num_units, decode);
     }
