@@ -38,11 +38,11 @@ struct Unit {
 };
 
 // kW: 16 columns of up to 4 bytes, or 32 columns of 2 bytes (16-bit D without bulk loads of C).
-template <int kBN, int kW, bool kBulkC>
+template <int kBN, int kW, bool kBulkC, int kBufs = 3>
 struct EpilogueCfg {
     static constexpr int COLS = kBN >= 64 ? kBN / 2 : kBN;  // per warp group; the second is idle below 64
     static constexpr int W = kW;
-    static constexpr int BUFS = 3;
+    static constexpr int BUFS = kBufs;
     static constexpr int BUF_BYTES = 8192;
     static constexpr int C_AHEAD = BUFS - 1;
     static constexpr bool BULK_C = kBulkC;

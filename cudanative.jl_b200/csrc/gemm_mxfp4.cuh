@@ -53,7 +53,7 @@ struct MxCfg {
     static constexpr int BBOX_BYTES = BBOX * BK / 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
     static constexpr int PROMOTE_KB = 8;
-    using Epi = EpilogueCfg<kBN, kPromote ? 16 : 32, false>;
+    using Epi = EpilogueCfg<kBN, kPromote ? 16 : 32, false, 2>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES;
@@ -207,49 +207,51 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0 && cta_rank == 0) {
+        if (cta_rank == 0) {
+            const uint32_t lead = elect_lane();
             const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
             const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
+            const int kb_total = (p.K + Cfg::BK - 1) / Cfg::BK;
             int s = 0;
             uint32_t ph = 0, ucount = 0;
             bool ok = true, ready = false;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
-                const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, inst_n(u), 0);
-                const uint32_t shift = static_cast<uint32_t>(scale_shift(u)) / 32;
-                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
+                const uint32_t shift = __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0);
+                for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     const uint32_t acc = ucount % ACCS;
                     const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
-                    const bool end = kb + 1 == u.kb || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
-                    if (begin) {
-                        ok = mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty);
-                        if (!ok) break;
-                    }
-                    if (!ready) ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
+                    const bool end = kb + 1 == kb_total || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
+                    if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    if (ok && !ready) ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage));
                     if (!ok) break;
                     tc_fence_after_sync();
                     // look at the next stage now: the answer arrives while this one's products are issued
                     const int s1 = s + 1 == STAGES ? 0 : s + 1;
-                    ready = mbar_test(full_bar(s1), ph ^ (s1 == 0));
+                    const bool next = mbar_test(full_bar(s1), ph ^ (s1 == 0));
                     const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
+                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8 + shift;
                     const int steps = min(4, (p.K - kb * Cfg::BK + 63) / 64);
                     const uint32_t d_tmem = tmem_base + acc * kBN;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if (k < steps) {
                             const uint32_t id = idesc0 | (k & 1 ? (2u << 4) | (2u << 29) : 0u);
-                            umma_mxf4<kCtas>(d_tmem, da0 + step + 2 * k, db0 + step + 2 * k, id, sfa + 4 * (k >> 1),
-                                             sfb + (k >> 1) * Cfg::B_TILES * 4 + shift, (begin && k == 0) ? 0u : 1u);
+                            umma_mxf4<kCtas>(lead, d_tmem, da0 + step + 2 * k, db0 + step + 2 * k, id, sfa + 4 * (k >> 1),
+                                             sfb + (k >> 1) * Cfg::B_TILES * 4, (begin && k == 0) ? 0u : 1u);
                         }
                     }
-                    if constexpr (kPair) umma_commit_pair(empty_bar(s));
-                    else umma_commit<kCtas>(empty_bar(s));
-                    if (end) {
-                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                        else umma_commit<kCtas>(tmem_full_bar(acc));
-                        ++ucount;
+                    if (lead) {
+                        if constexpr (kPair) umma_commit_pair(empty_bar(s));
+                        else umma_commit<kCtas>(empty_bar(s));
+                        if (end) {
+                            if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                            else umma_commit<kCtas>(tmem_full_bar(acc));
+                        }
                     }
+                    ucount += end ? 1u : 0u;
+                    ready = __all_sync(0xffffffffu, next);
                 }
             }
         }

@@ -529,29 +529,47 @@ __host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int sf_id) 
 }
 
 // D[tmem] (+)= (A * scale_a) * (B * scale_b), K = 64; scales in tensor memory (32 lanes x 4 bytes a column,
-// column c holding rows 32 c .. 32 c + 31); issued by ONE thread.
+// column c holding rows 32 c .. 32 c + 31).
+// Executed by a whole converged warp with `lead` set in one lane: the operands are then the same in every lane
+// and sit in uniform registers from the start.  From one lane's own branch each of them has to be moved there
+// for every instruction, which took as long as the product itself.
 template <int kCtaGroup>
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
+__device__ __forceinline__ void umma_mxf4(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa_tmem,
                                           uint32_t sfb_tmem, uint32_t accumulate) {
     if constexpr (kCtaGroup == 1) {
         asm volatile(
             "{\n"
-            ".reg .pred p;\n"
+            ".reg .pred p, q;\n"
             "setp.ne.b32 p, %6, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "setp.ne.b32 q, %7, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
             "}" ::"r"(d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate), "r"(lead)
             : "memory");
     } else {
         asm volatile(
             "{\n"
-            ".reg .pred p;\n"
+            ".reg .pred p, q;\n"
             "setp.ne.b32 p, %6, 0;\n"
-            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "setp.ne.b32 q, %7, 0;\n"
+            "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
             "}" ::"r"(d_tmem),
-            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate), "r"(lead)
             : "memory");
     }
+}
+
+// 1 in one lane of a converged warp, 0 in the others.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}"
+        : "=r"(r));
+    return r;
 }
 
 // Arrive on an mbarrier once every tcgen05 operation this thread issued so far has completed.
