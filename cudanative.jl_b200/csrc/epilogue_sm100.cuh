@@ -31,10 +31,19 @@ struct EpilogueParams {
     int c_tma, d_tma;                        // may be moved by bulk copies
 };
 
-// A tile of work: this CTA's first row, the tile's first column, the columns that exist, k-blocks of 64
-// (or 256) in the inner dimension.
+// A tile of work: this CTA's first row, the tile's first column, the columns that exist; the inner dimension
+// from k0 on, of which this CTA takes k-blocks (of 64 or 256) kb0 .. kb0 + kb - 1.
 struct Unit {
-    int group, m0, n0, cols, k0, k_len, kb;
+    int group, m0, n0, cols, k0, k_len, kb0, kb;
+};
+
+// With few tiles the two CTAs of a cluster take half of a tile's inner dimension each: CTA 1 sends its sums
+// into CTA 0's shared memory, CTA 0 adds them to its own (always in this order) and stores.
+struct SplitParams {
+    int role = -1;       // -1: whole tiles, 0: receives and stores, 1: sends
+    const float* recv;   // [columns][128]
+    uint32_t recv_addr;
+    uint32_t full_bar, empty_bar;
 };
 
 // kW: 16 columns of up to 4 bytes, or 32 columns of 2 bytes (16-bit D without bulk loads of C).
@@ -57,10 +66,10 @@ constexpr int kDrain = 1 << 30;  // kPromoteKb: one accumulator per tile, moved 
 
 // Runs in warps 4 .. 11 (`wg` 0 or 1).  Barriers: tmem_full / tmem_empty [kAccs] at the given addresses,
 // 8 bytes apart; cfull [BUFS] of this warp group.
-template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, class Decode>
+template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, bool kSplit, class Decode>
 __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUtensorMap* tmC, const CUtensorMap* tmD, int wg, uint32_t tmem_base,
                                              uint32_t epi_base, uint8_t* epi_gen, uint32_t tmem_full, uint32_t tmem_empty, uint32_t cfull,
-                                             const WaitCtx& wc, int unit_first, int unit_stride, int num_units, Decode decode) {
+                                             const WaitCtx& wc, int unit_first, int unit_stride, int num_units, const SplitParams& split, Decode decode) {
     constexpr int W = E::W, BUFS = E::BUFS;
     const int et = static_cast<int>(threadIdx.x & 127);
     const int lane = static_cast<int>(threadIdx.x & 31);
@@ -101,8 +110,32 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
     if (c_bulk && elected)
         for (int i = 0; i < E::C_AHEAD; ++i) fetch_c();
 
-    uint32_t acc_count = 0;
+    uint32_t acc_count = 0, split_count = 0;
     bool fail = false, ok = true;
+    const bool sends = kSplit && split.role == 1, receives = kSplit && split.role == 0;
+    const uint32_t remote = kSplit ? mapa_shared(split.recv_addr, 0) : 0u;
+    // room in the receiver's buffer, or the sender's sums in it
+    auto split_begin = [&]() {
+        if (sends) ok = ok && mbar_wait_cluster(split.empty_bar, (split_count & 1u) ^ 1u, wc, kWaitPartial);
+        if (receives) ok = ok && mbar_wait_cluster(split.full_bar, split_count & 1u, wc, kWaitPartial);
+        ok = __all_sync(0xffffffffu, ok);
+    };
+    auto split_chunk = [&](int j, uint32_t (&r)[W]) {
+        if (!ok) return;
+        if (sends) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) st_cluster_u32(remote + ((j * W + i) * 128 + et) * 4, r[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + split.recv[(j * W + i) * 128 + et]);
+        }
+    };
+    auto split_end = [&]() {
+        __syncwarp();
+        if (lane == 0 && sends) mbar_arrive_cluster(split.full_bar, 0);
+        if (lane == 0 && receives) mbar_arrive_cluster(split.empty_bar, 1);
+        ++split_count;
+    };
     for (int unit = unit_first; unit < num_units; unit += unit_stride) {
         const Unit u = decode(unit);
         const int cols = own_cols(u);
@@ -254,24 +287,29 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
                 }
                 release(acc);
             }
+            if (kSplit && (sends || receives) && cols > 0) split_begin();
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q) {
                 if (!fail && q * W < cols) {
                     uint32_t r[W];
-                    buffer_ready();
+                    if (!sends) buffer_ready();
 #pragma unroll
                     for (int i = 0; i < W; ++i) r[i] = __float_as_uint(sum[q * W + i]);
-                    finish(q, r);
+                    if (kSplit && (sends || receives)) split_chunk(q, r);
+                    if (!sends) finish(q, r);
                 }
             }
-            if (fail) break;
+            if (kSplit && (sends || receives) && cols > 0) split_end();
+            if (fail || (sends && !ok)) break;
         } else {
             const bool empty = u.kb == 0;
             const uint32_t acc = acc_count % kAccs;
             if (!empty) ok = ok && mbar_wait(tmem_full + 8 * acc, (acc_count / kAccs) & 1u, wc, kWaitTmemFull);
             tc_fence_after_sync();
+            if (kSplit && (sends || receives) && cols > 0) split_begin();
             for (int j = 0; j * W < cols; ++j) {
-                buffer_ready();
+                if (sends) ok = __all_sync(0xffffffffu, ok);
+                else buffer_ready();
                 uint32_t r[W];
                 if (ok && !empty) {
                     tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
@@ -280,9 +318,11 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, const CUte
 #pragma unroll
                     for (int i = 0; i < W; ++i) r[i] = 0u;
                 }
-                if (!finish(j, r)) break;
+                if (kSplit && (sends || receives)) split_chunk(j, r);
+                if (!sends && !finish(j, r)) break;
             }
-            if (fail) break;
+            if (kSplit && (sends || receives) && cols > 0) split_end();
+            if (fail || (sends && !ok)) break;
             if (!empty) {
                 release(acc);
                 ++acc_count;

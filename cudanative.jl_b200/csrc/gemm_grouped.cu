@@ -135,8 +135,9 @@ struct Grouped {
 
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
 int launch_promote(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote>;
-    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote>;
+    constexpr bool kSplit = kBN == 32;  // few columns per group: pairs of CTAs that may share a tile's inner dimension
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
+    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote, kSplit>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
@@ -151,7 +152,7 @@ int launch_promote(const CUtensorMap (&tm)[4], const GroupedParams& p, int grid,
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCtas;
+    attr[0].val.clusterDim.x = kSplit ? 2 : kCtas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -280,6 +281,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "grouped gemm: too many tiles for one launch");
     int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
     int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
+    if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
     if (pair == 2) rc = tile_n == 256 ? launch_kind<256, 2>(g, tm, p, grid, stream, pdl) : launch_kind<128, 2>(g, tm, p, grid, stream, pdl);
     else if (tile_n == 128) rc = launch_kind<128, 1>(g, tm, p, grid, stream, pdl);

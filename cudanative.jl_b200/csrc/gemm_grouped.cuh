@@ -44,7 +44,7 @@ struct GroupedParams {
     unsigned long long wait_budget_ns;
 };
 
-template <int kBN, bool kRaggedK, int kCtas, bool kPromote>
+template <int kBN, bool kRaggedK, int kCtas, bool kPromote, bool kSplit>
 struct GroupedCfg {
     static constexpr int THREADS = 384;
     static constexpr int BM = 128;
@@ -60,11 +60,13 @@ struct GroupedCfg {
     using Epi = EpilogueCfg<kBN, (kRaggedK || kPromote) ? 16 : 32, kRaggedK>;
     static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES;
+    static constexpr int RECV_BYTES = kSplit ? 128 * Epi::COLS * 4 : 0;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int TMEM_COLS = 2 * kBN < 32 ? 32 : 2 * kBN;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 4 * STAGES + 4 + 2 * Epi::BUFS;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int NBARS = 4 * STAGES + 6 + 2 * Epi::BUFS;
+    static_assert(!kSplit || (kCtas == 1 && !kRaggedK && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
@@ -128,12 +130,12 @@ __device__ __forceinline__ int find_group(const int* first, int groups, int q) {
     return lo;
 }
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, bool kSplit>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
                      const GroupedParams p) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote>;
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
     constexpr int STAGES = Cfg::STAGES;
     using Epi = typename Cfg::Epi;
     constexpr bool kPair = (kCtas == 2);
@@ -144,7 +146,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t epi_base = smem_base + STAGES * Cfg::STAGE_BYTES;
-    constexpr int kTableAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kTableAt = kRecvAt + Cfg::RECV_BYTES;
     const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
     uint8_t* epi_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
     int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
@@ -157,15 +160,16 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     auto tail_ready_bar = [&](int s) { return bar_base + 8u * (3 * STAGES + s); };  // ... and its foreign rows are zero
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
     auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + 2 + a); };
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 4 + b); };
+    auto split_bar = [&](int i) { return bar_base + 8u * (4 * STAGES + 4 + i); };  // partial sums: full, empty
+    auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 6 + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t cta_rank = kPair ? cluster_cta_rank() : 0u;
-    const int unit_stride = kPair ? (gridDim.x >> 1) : gridDim.x;
-    const int unit_first = kPair ? (blockIdx.x >> 1) : blockIdx.x;
+    int unit_stride = kPair ? (gridDim.x >> 1) : gridDim.x;
+    int unit_first = kPair ? (blockIdx.x >> 1) : blockIdx.x;
     WaitCtx wc{abort_flag, p.status, p.wait_budget_ns};
 
     if (threadIdx.x == 0) {
@@ -179,6 +183,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         for (int a = 0; a < 2; ++a) {
             mbar_init(tmem_full_bar(a), 1);
             mbar_init(tmem_empty_bar(a), 8 * kCtas);
+            mbar_init(split_bar(a), 4);
         }
         for (int b = 0; b < 2 * Epi::BUFS; ++b) mbar_init(cfull_bar(b), 1);
         fence_mbar_init();
@@ -190,7 +195,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     tc_fence_before_sync();
     __syncthreads();
-    if constexpr (kPair) cluster_sync_all();
+    if constexpr (kPair || kSplit) cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     griddep_launch_dependents();
@@ -206,6 +211,22 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     }
     const int tiles_per_group = p.tiles_m * p.tiles_n;  // ragged K
     const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * tiles_per_group : first[p.groups] * p.tiles_m;
+
+    // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).
+    SplitParams split;
+    if constexpr (kSplit) {
+        const int ctas = gridDim.x, kb_all = (p.K + Cfg::BK - 1) / Cfg::BK;
+        const int whole = (num_units + ctas - 1) / ctas, halves = (num_units + ctas / 2 - 1) / (ctas / 2);
+        if (kb_all >= 4 && halves < 2 * whole) {
+            split.role = static_cast<int>(cluster_cta_rank());
+            unit_first = blockIdx.x >> 1;
+            unit_stride = ctas >> 1;
+        }
+        split.recv = reinterpret_cast<const float*>(smem_gen + kRecvAt);
+        split.recv_addr = smem_base + kRecvAt;
+        split.full_bar = split_bar(0);
+        split.empty_bar = split_bar(1);
+    }
 
     auto decode = [&](int unit) {
         Unit u;
@@ -238,7 +259,13 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             u.k0 = 0;
             u.k_len = p.K;
         }
+        u.kb0 = 0;
         u.kb = (u.k_len + Cfg::BK - 1) / Cfg::BK;
+        if (kSplit && split.role >= 0) {
+            const int half = (u.kb + 1) / 2;
+            u.kb0 = split.role * half;
+            u.kb = split.role ? u.kb - half : half;
+        }
         return u;
     };
     auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
@@ -267,7 +294,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     if (!ok) break;
                     const uint32_t sa = smem_base + s * Cfg::STAGE_BYTES;
                     const uint32_t sb = sa + Cfg::A_BYTES;
-                    const int k0 = u.k0 + kb * Cfg::BK;
+                    const int k0 = u.k0 + (u.kb0 + kb) * Cfg::BK;
                     if constexpr (kRaggedK) {
                         const bool tail = needs_tail(u) && kb + 1 == kb1;
                         if (tail) {
@@ -343,7 +370,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     if (!ok) break;
                     int steps = Cfg::BK / 16;
                     if (kb + 1 == u.kb) {
-                        steps = (u.k_len - kb * Cfg::BK + 15) / 16;
+                        steps = min(steps, (u.k_len - (u.kb0 + kb) * Cfg::BK + 15) / 16);
                         if (needs_tail(u)) {
                             ok = mbar_wait(tail_ready_bar(s), (tail_ph >> s) & 1u, wc, kWaitTail);
                             if (!ok) break;
@@ -404,9 +431,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     } else if (warp >= 4) {
         const int wg = (warp - 4) >> 2;
         const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK>(p.e, &tmC, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(p.e, &tmC, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
                                                                            tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
-                                                                           unit_first, unit_stride, num_units, decode);
+                                                                           unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit
@@ -416,7 +443,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-    if constexpr (kPair) cluster_sync_all();
+    if constexpr (kPair || kSplit) cluster_sync_all();
     if (warp == 2) {
         tc_fence_after_sync();
         tmem_dealloc<kCtas>(tmem_base, Cfg::TMEM_COLS);

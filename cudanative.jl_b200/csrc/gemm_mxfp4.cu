@@ -22,8 +22,9 @@ struct MxProblem {
 
 template <int kBN, int kCtas, bool kPromote>
 int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
-    using Cfg = MxCfg<kBN, kCtas, kPromote>;
-    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote>;
+    constexpr bool kSplit = kBN == 32;  // few columns: pairs of CTAs that may share a tile's inner dimension
+    using Cfg = MxCfg<kBN, kCtas, kPromote, kSplit>;
+    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote, kSplit>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
@@ -38,7 +39,7 @@ int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStre
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kCtas;
+    attr[0].val.clusterDim.x = kSplit ? 2 : kCtas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -52,18 +53,24 @@ int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStre
 template <int kBN, int kCtas>
 int launch_typed(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     if (p.e.d_fmt == 0) {
-        if constexpr (MxCfg<kBN, kCtas, true>::ACCS == 2) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
+        if constexpr (kBN <= 128) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
         else return fail(B200_UNSUPPORTED, "mxfp4: a binary32 D takes tiles of 128 columns at most");
     }
     return launch<kBN, kCtas, false>(tm, p, grid, stream, pdl);
 }
 
+// Tile columns, by the mean length of the groups.  Two CTAs on 256 columns need a 16-bit D: a binary32 one
+// takes two accumulators (epilogue_sm100.cuh), for which tensor memory has no room beside the scales.
+void pick_tile(const b200_handle* h, const MxProblem& g, int* tile_n, int* pair) {
+    const int64_t n = (g.N + g.groups - 1) / g.groups;
+    *tile_n = h->tile_n ? std::max(h->tile_n, 128) : n > 128 ? 256 : n > 32 ? 128 : 32;
+    if (*tile_n == 256 && (g.d_type == B200_F32 || g.M <= 128 || h->cta_pair == 1)) *tile_n = 128;
+    *pair = *tile_n == 256 ? 2 : 1;
+}
+
 int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
-    int tile_n = 128, pair = 1, rc;
-    if (h->tile_n) tile_n = h->tile_n == 64 ? 192 : h->tile_n;
-    if (h->cta_pair) pair = h->cta_pair;
-    if (tile_n == 256 && g.d_type == B200_F32) tile_n = 128;
-    if (tile_n == 192) pair = 2;
+    int tile_n, pair, rc;
+    pick_tile(h, g, &tile_n, &pair);
     MxGemmParams p = {};
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
@@ -87,7 +94,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     const int q = 16 / elem_bytes(g.d_type);
     p.e.d_tma = !(reinterpret_cast<uintptr_t>(g.D) & 15u) && g.ldd % q == 0 && g.M % q == 0;
 
-    const int bn_local = tile_n / pair, bbox = bn_local % 128 == 0 ? 128 : bn_local % 64 == 0 ? 64 : 32;
+    const int bn_local = tile_n / pair, bbox = std::min(bn_local, 128);
     const int64_t k_bytes = (g.K + 1) / 2;
     CUtensorMap tm[5];
     BatchDim b;
@@ -115,10 +122,12 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * p.tiles_m;
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
     const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
-    const int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
+    int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
+    if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
-    if (pair == 2) rc = tile_n == 256 ? launch_typed<256, 2>(tm, p, grid, stream, pdl) : tile_n == 192 ? launch_typed<192, 2>(tm, p, grid, stream, pdl) : launch_typed<128, 2>(tm, p, grid, stream, pdl);
-    else rc = tile_n == 256 ? launch_typed<256, 1>(tm, p, grid, stream, pdl) : launch_typed<128, 1>(tm, p, grid, stream, pdl);
+    if (tile_n == 256) rc = launch_typed<256, 2>(tm, p, grid, stream, pdl);
+    else if (tile_n == 128) rc = launch_typed<128, 1>(tm, p, grid, stream, pdl);
+    else rc = launch_typed<32, 1>(tm, p, grid, stream, pdl);
     if (rc) return rc;
     h->last = {B200_KERNEL_TCGEN05, tile_n, 1, grid, pair};
     return B200_OK;

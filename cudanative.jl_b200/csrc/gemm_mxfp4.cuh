@@ -14,8 +14,9 @@
 // instead of 224 us without it; issued one stage ahead 437 us.)
 //
 // A tile's scales always come from whole tiles of 128 columns, counted from the group's first column, as
-// they were quantised.  A tile of kBN columns starts inside one where kBN is no multiple of 128: the
-// scales' first tensor-memory column is moved by (start % 128) / 32.
+// they were quantised.  A tile of 32 columns may begin inside one: the warps that carry its scales put the
+// rows that it starts with into the first column (the products' scale addresses stay multiples of 4 columns;
+// an odd one is a misaligned address).
 //
 // What bounds it: 4-bit products run at four times the rate of 16-bit ones, with the same bytes per cycle.
 // For few columns (a token, a decode step) the elements of A, 17/32 byte per value, are the floor.
@@ -38,7 +39,7 @@ struct MxGemmParams {
     unsigned long long wait_budget_ns;
 };
 
-template <int kBN, int kCtas, bool kPromote>
+template <int kBN, int kCtas, bool kPromote, bool kSplit>
 struct MxCfg {
     static constexpr int THREADS = 512;
     static constexpr int BM = 128;
@@ -49,34 +50,36 @@ struct MxCfg {
     static constexpr int B_TILES = (kBN + 127) / 128;  // scale tiles that a tile of columns touches at most
     static constexpr int SF_BYTES = 1024 * (1 + B_TILES);
     static constexpr int STAGE_BYTES = (A_BYTES + B_BYTES + SF_BYTES + 1023) / 1024 * 1024;
-    static constexpr int BBOX = BN_LOCAL % 128 == 0 ? 128 : BN_LOCAL % 64 == 0 ? 64 : 32;
+    static constexpr int BBOX = BN_LOCAL < 128 ? BN_LOCAL : 128;
     static constexpr int BBOX_BYTES = BBOX * BK / 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
     static constexpr int PROMOTE_KB = 8;
     using Epi = EpilogueCfg<kBN, kPromote ? 16 : 32, false, 2>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES;
+    static constexpr int RECV_BYTES = kSplit ? 128 * Epi::COLS * 4 : 0;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int ACCS = kBN <= 192 ? 2 : 1;
     static constexpr int SCALE_COLS = 8 * (1 + B_TILES);  // per set: 2 x 4 for A, 2 x 4 per scale tile for B
     static constexpr int SCALE_AT = ACCS * kBN;
     static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 3 * STAGES + 2 * ACCS + 2 * Epi::BUFS;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int NBARS = 3 * STAGES + 2 + 2 * ACCS + 2 * Epi::BUFS;
+    static_assert(!kSplit || (kCtas == 1 && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
-    static_assert(kBN <= 128 || kBN == 192 || kBN == 256, "columns per tile and the scale tiles they touch");
+    static_assert(kBN == 32 || kBN == 128 || kBN == 256, "a tile of columns begins on a multiple of 32 inside its scale tile");
 };
 
-template <int kBN, int kCtas, bool kPromote>
+template <int kBN, int kCtas, bool kPromote, bool kSplit>
 __global__ void __launch_bounds__(512, 1)
 gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
                    const __grid_constant__ CUtensorMap tmD, const MxGemmParams p) {
-    using Cfg = MxCfg<kBN, kCtas, kPromote>;
+    using Cfg = MxCfg<kBN, kCtas, kPromote, kSplit>;
     using Epi = typename Cfg::Epi;
     constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS;
     constexpr bool kPair = (kCtas == 2);
@@ -86,7 +89,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t epi_base = smem_base + STAGES * Cfg::STAGE_BYTES;
     uint8_t* epi_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
-    constexpr int kTableAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kTableAt = kRecvAt + Cfg::RECV_BYTES;
     const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
     int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
     int* first = off + kMaxGroups + 4;
@@ -98,15 +102,16 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     auto scales_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };   // in this CTA's shared memory
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + a); };
     auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + ACCS + a); };
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + b); };
+    auto split_bar = [&](int i) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + i); };  // partial sums: full, empty
+    auto cfull_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + 2 + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t cta_rank = kPair ? cluster_cta_rank() : 0u;
-    const int unit_stride = kPair ? (gridDim.x >> 1) : gridDim.x;
-    const int unit_first = kPair ? (blockIdx.x >> 1) : blockIdx.x;
+    int unit_stride = kPair ? (gridDim.x >> 1) : gridDim.x;
+    int unit_first = kPair ? (blockIdx.x >> 1) : blockIdx.x;
     WaitCtx wc{abort_flag, p.status, p.wait_budget_ns};
 
     if (threadIdx.x == 0) {
@@ -120,6 +125,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             mbar_init(tmem_full_bar(a), 1);
             mbar_init(tmem_empty_bar(a), 8 * kCtas);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(split_bar(i), 4);
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
@@ -130,7 +136,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     tc_fence_before_sync();
     __syncthreads();
-    if constexpr (kPair) cluster_sync_all();
+    if constexpr (kPair || kSplit) cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     griddep_launch_dependents();
@@ -144,6 +150,27 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __threadfence();
     }
     const int num_units = offsets_ok ? first[p.groups] * p.tiles_m : 0;
+
+    // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).
+    SplitParams split;
+    const int kb_all = (p.K + Cfg::BK - 1) / Cfg::BK;
+    if constexpr (kSplit) {
+        const int ctas = gridDim.x;
+        const int whole = (num_units + ctas - 1) / ctas, halves = (num_units + ctas / 2 - 1) / (ctas / 2);
+        if (kb_all >= 4 && halves < 2 * whole) {
+            split.role = static_cast<int>(cluster_cta_rank());
+            unit_first = blockIdx.x >> 1;
+            unit_stride = ctas >> 1;
+        }
+        split.recv = reinterpret_cast<const float*>(smem_gen + kRecvAt);
+        split.recv_addr = smem_base + kRecvAt;
+        split.full_bar = split_bar(0);
+        split.empty_bar = split_bar(1);
+    }
+    // this CTA's k-blocks of every tile
+    const int kb_half = (kb_all + 1) / 2;
+    const int kb_first = kSplit && split.role == 1 ? kb_half : 0;
+    const int kb_total = !kSplit || split.role < 0 ? kb_all : split.role ? kb_all - kb_half : kb_half;
 
     auto decode = [&](int unit) {
         Unit u;
@@ -160,7 +187,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         u.cols = min(kBN, off[u.group + 1] - u.n0);
         u.k0 = 0;
         u.k_len = p.K;
-        u.kb = (p.K + Cfg::BK - 1) / Cfg::BK;
+        u.kb0 = kb_first;
+        u.kb = kb_total;
         return u;
     };
     auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
@@ -193,14 +221,14 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     uint32_t fb = full_bar(s);
                     if constexpr (kPair) fb = mapa_shared(fb, 0);
                     if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
-                    if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, kb * 128, u.m0, z, fb);
-                    else if (a_once) tma_load_3d_hint(at_a, &tmA, kb * 128, u.m0, z, fb, once);
-                    else tma_load_3d(at_a, &tmA, kb * 128, u.m0, z, fb);
+                    if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
+                    else if (a_once) tma_load_3d_hint(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb, once);
+                    else tma_load_3d(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
                     auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
                         if constexpr (kPair) tma_load_2d_pair(dst, tm, x, y, fb);
                         else tma_load_2d(dst, tm, x, y, fb);
                     };
-                    for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, kb * 128, nb0 + i * Cfg::BBOX);
+                    for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, (kb_first + kb) * 128, nb0 + i * Cfg::BBOX);
                 }
             }
         }
@@ -211,14 +239,12 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             const uint32_t lead = elect_lane();
             const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
             const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
-            const int kb_total = (p.K + Cfg::BK - 1) / Cfg::BK;
             int s = 0;
             uint32_t ph = 0, ucount = 0;
             bool ok = true, ready = false;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
                 const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
-                const uint32_t shift = __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0);
                 for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     const uint32_t acc = ucount % ACCS;
                     const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
@@ -231,8 +257,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     const int s1 = s + 1 == STAGES ? 0 : s + 1;
                     const bool next = mbar_test(full_bar(s1), ph ^ (s1 == 0));
                     const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8 + shift;
-                    const int steps = min(4, (p.K - kb * Cfg::BK + 63) / 64);
+                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
+                    const int steps = min(4, (p.K - (kb_first + kb) * Cfg::BK + 63) / 64);
                     const uint32_t d_tmem = tmem_base + acc * kBN;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -275,8 +301,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     // two tiles along K (behind an odd last one: zeros), B_TILES along the columns; tiles that
                     // this tile's columns do not touch are loaded and not used
                     mbar_arrive_expect_tx(scales_full_bar(s), Cfg::SF_BYTES);
-                    tma_load_3d(at, &tmSA, 0, 2 * kb, a_row, scales_full_bar(s));
-                    tma_load_3d(at + 1024, &tmSB, 0, 2 * kb, b_row, scales_full_bar(s));
+                    tma_load_3d(at, &tmSA, 0, 2 * (kb_first + kb), a_row, scales_full_bar(s));
+                    tma_load_3d(at + 1024, &tmSB, 0, 2 * (kb_first + kb), b_row, scales_full_bar(s));
                 }
             }
         }
@@ -289,8 +315,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
-        const int kb_total = (p.K + Cfg::BK - 1) / Cfg::BK;
         for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+            const int turn = kBN < 128 ? scale_shift(decode(unit)) / 32 : 0;
             for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                 ok = mbar_wait(scales_full_bar(s), ph, wc, kWaitScales);
                 ok = __all_sync(0xffffffffu, ok);  // tcgen05.st is warp-collective
@@ -302,6 +328,10 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                 uint4 r[2 * (1 + Cfg::B_TILES)];
 #pragma unroll
                 for (int i = 0; i < 2 * (1 + Cfg::B_TILES); ++i) r[i] = *reinterpret_cast<const uint4*>(tiles + i * 512);
+                if constexpr (kBN < 128) {  // one column of 32 rows is all that the tile uses
+#pragma unroll
+                    for (int i = 2; i < 4; ++i) r[i].x = turn == 0 ? r[i].x : turn == 1 ? r[i].y : turn == 2 ? r[i].z : r[i].w;
+                }
                 tmem_st_32x32b_x4(sfa, r[0]);
                 tmem_st_32x32b_x4(sfa + 4, r[1]);
 #pragma unroll
@@ -323,9 +353,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         regs_inc<200>();
         const int wg = (warp - 4) >> 2;
         const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? kDrain : 0, false>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
+        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? kDrain : 0, false, kSplit>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
                                                                            tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
-                                                                           unit_first, unit_stride, num_units, decode);
+                                                                           unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit
@@ -335,7 +365,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-    if constexpr (kPair) cluster_sync_all();
+    if constexpr (kPair || kSplit) cluster_sync_all();
     if (warp == 2) {
         tc_fence_after_sync();
         tmem_dealloc<kCtas>(tmem_base, Cfg::TMEM_COLS);

@@ -150,6 +150,7 @@ enum : int {
     kWaitPanel = 108,        // producer waiting for a panel of A to arrive in this GPU's memory
     kWaitTail = 109,         // grouped product: the last k-block of a group, zeros behind its end
     kWaitScales = 111,       // 4-bit product: a stage's scales, in shared or in tensor memory
+    kWaitPartial = 112,      // split inner dimension: the other CTA's partial sums, or room to send them
     kBadOffsets = 110        // not a wait: a group's offsets decrease or leave the matrix
 };
 
@@ -193,6 +194,36 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const W
             return false;
         }
     }
+}
+
+// mbar_wait for a barrier that the other CTA of the cluster arrives on after it has written this CTA's shared
+// memory: the wait acquires at cluster scope.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, const WaitCtx& w, int where) {
+    const long long t0 = clock64();
+    const long long budget_cycles = static_cast<long long>(w.budget_ns) * 2;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(50000u)
+            : "memory");
+        if (ok) return true;
+        if (*w.abort_flag) return false;
+        if (clock64() - t0 > budget_cycles) {
+            report_timeout(w, where, static_cast<int>(parity));
+            return false;
+        }
+    }
+}
+
+// Store to the shared memory of a CTA of this cluster (an address from mapa_shared).
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // Bounded wait for a 32-bit word in global memory to become non-zero.  The word is written by a
