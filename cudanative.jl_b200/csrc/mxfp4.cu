@@ -61,19 +61,38 @@ __device__ __forceinline__ uint32_t to_elements(const float* v) {
     return r;
 }
 
-// 32 values -> scale code and elements.
-__device__ __forceinline__ uint32_t quantize_block(float (&v)[32], uint4* q) {
-    uint32_t top = 0;  // binary32 magnitudes order like integers
+// Eight elements times x.
+template <typename T>
+__device__ __forceinline__ void from_elements(uint32_t bits, float x, T (&out)[8]) {
+    uint32_t h[4];  // two binary16 each: every element is exact in it
+    asm("{\n"
+        ".reg .b8 t0, t1, t2, t3;\n"
+        "mov.b32 {t0, t1, t2, t3}, %4;\n"
+        "cvt.rn.f16x2.e2m1x2 %0, t0;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, t1;\n"
+        "cvt.rn.f16x2.e2m1x2 %2, t2;\n"
+        "cvt.rn.f16x2.e2m1x2 %3, t3;\n"
+        "}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(bits));
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    const uint32_t e = top >> 23;  // biased exponent; 0 for zero and subnormals
-    const uint32_t s = e == 255 ? 255u : (e > 2 ? e - 2 : 0u);
-    const float inv = __uint_as_float((e == 255 ? 0u : 254u - s) << 23);  // 2^(127 - s), normal for every s <= 252
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= inv;
-    *q = make_uint4(to_elements(v), to_elements(v + 8), to_elements(v + 16), to_elements(v + 24));
-    return s;
+    for (int j = 0; j < 4; ++j) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        out[2 * j] = from_float<T>(v.x * x);
+        out[2 * j + 1] = from_float<T>(v.y * x);
+    }
 }
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // orders like the values
+
+// Scale code of a block whose largest magnitude is `top` (binary32 bits).
+__device__ __forceinline__ uint32_t scale_code(uint32_t top) {
+    const uint32_t e = top >> 23;  // biased exponent; 0 for zero and subnormals
+    return e == 255 ? 255u : (e > 2 ? e - 2 : 0u);
+}
+
+// 1 / X = 2^(127 - s), a normal number for every s <= 252; 0 for a block of NaN.
+__device__ __forceinline__ float inverse(uint32_t s) { return __uint_as_float((s == 255 ? 0u : 254u - s) << 23); }
 
 __device__ __forceinline__ long long scale_at(long long tile_row, int kt, int kblock, int r) {
     return (tile_row * kt + kblock / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + kblock % 4;
@@ -91,113 +110,205 @@ __device__ __forceinline__ TileRow tile_row(const MxParams& p, const int* off, c
     return {v0, static_cast<int>(min(128ll, off[e + 1] - v0))};
 }
 
-// One block of 32 values per thread.  kTrans = 0: a vector's values are contiguous, four neighbouring
-// threads take four blocks of one vector (and write its four scales as one word); kTrans = 1: vectors are
-// contiguous across, a warp takes one block of 32 vectors.
-template <typename T, bool kTrans>
+// What every block of a launch needs: the groups' rows of scale tiles, and how many there are; 0 for bad offsets.
+__device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off, int* first, int* sums) {
+    if (!p.offsets) return (p.cols + 127) / 128;
+    if (!load_groups<true>(p.offsets, p.groups, p.cols, 128, off, first, sums)) {
+        if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
+        return 0;
+    }
+    return first[p.groups];
+}
+
+// Vectors whose values are contiguous.  A tile is 128 vectors x 128 values: 16 lanes take a vector's 128, eight
+// values (16 bytes of a 16-bit type) each, so that a warp reads and writes whole lines; four lanes find a
+// block's largest magnitude with two shuffles.  A thread has eight vectors in flight.
+template <typename T>
 __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxParams p) {
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
-    long long tile_rows = (p.cols + 127) / 128;
-    if (p.offsets) {
-        if (!load_groups<true>(p.offsets, p.groups, p.cols, 128, off, first, sums)) {
-            if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
-            return;
-        }
-        tile_rows = first[p.groups];
-    }
+    griddep_launch_dependents();
+    griddep_wait();
+    const long long tile_rows = scale_tile_rows(p, off, first, sums);
     const int kt = (p.K + 127) / 128;
     const T* X = static_cast<const T*>(p.X);
-    const long long work = tile_rows * kt;  // a tile of 128 vectors x 128 values: 512 blocks, two per thread
+    const long long work = tile_rows * kt;
+    const int lane = threadIdx.x & 31, part = lane & 15;
+    const int r0 = (threadIdx.x >> 5) * 2 + (lane >> 4);
+    const bool wide = p.ldx % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(X) & 15u) == 0;
     for (long long w = blockIdx.x; w < work; w += gridDim.x) {
         const long long q = w / kt;
         const int k_tile = static_cast<int>(w - q * kt);
         const TileRow t = tile_row(p, off, first, q);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-            const int i = threadIdx.x + half * 256;
-            const int r = kTrans ? (i & 31) + (i >> 7) * 32 : i >> 2;
-            const int b = kTrans ? (i >> 5) & 3 : i & 3;
-            const int k0 = k_tile * 128 + b * 32;
-            uint32_t s = 0;
-            if (r < t.count && k0 < p.K) {
-                const long long vec = t.first + r;
-                float v[32];
-                const T* src = kTrans ? X + vec + static_cast<long long>(k0) * p.ldx : X + vec * p.ldx + k0;
-                const long long step = kTrans ? p.ldx : 1;
-                constexpr int kVec = 16 / sizeof(T);
-                if (!kTrans && k0 + 32 <= p.K && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+        const int k0 = k_tile * 128 + part * 8;
+        constexpr int kVec = 8 * sizeof(T) / 16;
+        uint4 raw[8][kVec];
+        const T* src = X + (t.first + r0) * p.ldx + k0;
+        if (wide && k_tile * 128 + 128 <= p.K) {  // all loads before the first use
 #pragma unroll
-                    for (int j = 0; j < 32 / kVec; ++j) {
-                        const uint4 raw = reinterpret_cast<const uint4*>(src)[j];
-                        const T* e = reinterpret_cast<const T*>(&raw);
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-                        for (int x = 0; x < kVec; ++x) v[j * kVec + x] = as_float(e[x]);
-                    }
-                } else {
+                for (int j = 0; j < kVec; ++j)
+                    raw[i][j] = r0 + 16 * i < t.count ? reinterpret_cast<const uint4*>(src + 16 * i * p.ldx)[j] : make_uint4(0, 0, 0, 0);
+        } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = k0 + j < p.K ? as_float(src[j * step]) : 0.0f;
-                }
-                uint4 elements;
-                s = quantize_block(v, &elements);
-                *reinterpret_cast<uint4*>(p.Q + (vec * p.ldq + k0) / 2) = elements;
+            for (int i = 0; i < 8; ++i) {
+                T* e = reinterpret_cast<T*>(raw[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = r0 + 16 * i < t.count && k0 + j < p.K ? src[16 * i * p.ldx + j] : from_float<T>(0.0f);
             }
-            if constexpr (kTrans) {
-                p.S[scale_at(q, kt, k_tile * 4 + b, r)] = static_cast<uint8_t>(s);
-            } else {
-                s <<= 8 * b;
-                s |= __shfl_xor_sync(0xffffffffu, s, 1);
-                s |= __shfl_xor_sync(0xffffffffu, s, 2);
-                if (b == 0) *reinterpret_cast<uint32_t*>(p.S + scale_at(q, kt, k_tile * 4, r)) = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 16 * i;
+            const T* e = reinterpret_cast<const T*>(raw[i]);
+            float v[8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = as_float(e[j]);
+                top = max(top, magnitude(v[j]));
             }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            uint32_t s = scale_code(top);
+            const float inv = inverse(s);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= inv;
+            if (r < t.count && k0 < (p.K + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(p.Q + ((t.first + r) * p.ldq + k0) / 2) = to_elements(v);
+            // a vector's four scales as one word; vectors and blocks that do not exist were read as zeros: s = 0
+            s <<= 8 * (part / 4);
+            s |= __shfl_xor_sync(0xffffffffu, s, 4);
+            s |= __shfl_xor_sync(0xffffffffu, s, 8);
+            if (part == 0) *reinterpret_cast<uint32_t*>(p.S + scale_at(q, kt, k_tile * 4, r)) = s;
         }
     }
 }
 
+// Vectors that lie across (X is cols x K): a thread takes one block of two neighbouring vectors, so that a warp
+// reads 64 vectors' values of one k as a line; elements and scales of the tile go out through shared memory.
 template <typename T>
-__global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const MxParams p) {
+__global__ void __launch_bounds__(256) mxfp4_quantize_across_kernel(const MxParams p) {
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
-    long long tile_rows = (p.cols + 127) / 128;
-    if (p.offsets) {
-        if (!load_groups<true>(p.offsets, p.groups, p.cols, 128, off, first, sums)) {
-            if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
-            return;
-        }
-        tile_rows = first[p.groups];
-    }
+    __shared__ __align__(16) uint8_t elements[128][64 + 16];
+    __shared__ __align__(16) uint8_t scales[512];
+    griddep_launch_dependents();
+    griddep_wait();
+    const long long tile_rows = scale_tile_rows(p, off, first, sums);
     const int kt = (p.K + 127) / 128;
-    T* Y = static_cast<T*>(p.Y);
+    const T* X = static_cast<const T*>(p.X);
     const long long work = tile_rows * kt;
+    const int r = (threadIdx.x & 63) * 2, b = threadIdx.x >> 6;
+    struct alignas(2 * sizeof(T)) Pair { T a, b; };
     for (long long w = blockIdx.x; w < work; w += gridDim.x) {
         const long long q = w / kt;
         const int k_tile = static_cast<int>(w - q * kt);
         const TileRow t = tile_row(p, off, first, q);
-        // eight elements (4 bytes) per thread and step: 16 threads to a vector's 128
-#pragma unroll 2
-        for (int i = threadIdx.x; i < 128 * 16; i += 256) {
-            const int r = i >> 4, k0 = k_tile * 128 + (i & 15) * 8;
-            if (r >= t.count || k0 >= p.K) continue;
-            const long long vec = t.first + r;
-            const uint32_t bits = *reinterpret_cast<const uint32_t*>(p.Q + (vec * p.ldq + k0) / 2);
-            const uint32_t s = p.S[scale_at(q, kt, k0 / 32, r)];
-            const float x = __uint_as_float(s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23);
-            T out[8];
+        const int k0 = k_tile * 128 + b * 32;
+        const T* src = X + t.first + r + static_cast<long long>(k0) * p.ldx;
+        const bool pairs = p.ldx % 2 == 0 && (reinterpret_cast<uintptr_t>(src) % sizeof(Pair)) == 0;
+        Pair raw[32];
+        if (pairs && r + 1 < t.count && k0 + 32 <= p.K) {  // all loads before the first use
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t c = (bits >> (4 * j)) & 15u, m = c & 7u;
-                // magnitude: 0, .5, then (1 + .5 f) 2^(e - 1) with e = m >> 1, f = m & 1
-                const float a = m < 2 ? 0.5f * m : __uint_as_float(((126u + (m >> 1)) << 23) | ((m & 1u) << 22));
-                out[j] = from_float<T>((c & 8u ? -a : a) * x);
+            for (int j = 0; j < 32; ++j) raw[j] = *reinterpret_cast<const Pair*>(src + j * p.ldx);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                raw[j].a = r < t.count && k0 + j < p.K ? src[j * p.ldx] : from_float<T>(0.0f);
+                raw[j].b = r + 1 < t.count && k0 + j < p.K ? src[j * p.ldx + 1] : from_float<T>(0.0f);
             }
-            T* dst = Y + vec * p.ldy + k0;
-            if (k0 + 8 <= p.K && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+        }
 #pragma unroll
-                for (int j = 0; j < static_cast<int>(8 * sizeof(T) / 16); ++j)
-                    reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(out)[j];
-            } else {
+        for (int x = 0; x < 2; ++x) {
+            uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k0 + j < p.K) dst[j] = out[j];
+            for (int j = 0; j < 32; ++j) top = max(top, magnitude(as_float(x ? raw[j].b : raw[j].a)));
+            const uint32_t s = scale_code(top);
+            const float inv = inverse(s);
+            uint32_t e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = as_float(x ? raw[i * 8 + j].b : raw[i * 8 + j].a) * inv;
+                e[i] = to_elements(v);
             }
+            *reinterpret_cast<uint4*>(&elements[r + x][b * 16]) = make_uint4(e[0], e[1], e[2], e[3]);
+            scales[((r + x) % 32) * 16 + (r + x) / 32 * 4 + b] = static_cast<uint8_t>(s);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = threadIdx.x; i < 512; i += 256) {
+            const int row = i >> 2, part = i & 3;
+            const int k = k_tile * 128 + part * 32;
+            if (row < t.count && k < p.K)
+                *reinterpret_cast<uint4*>(p.Q + ((t.first + row) * p.ldq + k) / 2) = *reinterpret_cast<const uint4*>(&elements[row][part * 16]);
+        }
+        if (threadIdx.x < 32)
+            reinterpret_cast<uint4*>(p.S + (q * kt + k_tile) * 512)[threadIdx.x] = reinterpret_cast<const uint4*>(scales)[threadIdx.x];
+        __syncthreads();
+    }
+}
+
+// Eight elements to a thread, 16 lanes to a vector's 128, eight vectors in flight.  Rows of Y that do not begin
+// on 16 bytes are put together in shared memory and leave as 4-byte (or single) values, lane next to lane.
+template <typename T>
+__global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const MxParams p) {
+    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
+    __shared__ __align__(16) T rows[16][128 + 16 / sizeof(T)];
+    griddep_launch_dependents();
+    griddep_wait();
+    const long long tile_rows = scale_tile_rows(p, off, first, sums);
+    const int kt = (p.K + 127) / 128;
+    T* Y = static_cast<T*>(p.Y);
+    const long long work = tile_rows * kt;
+    const int lane = threadIdx.x & 31, part = lane & 15, r0 = (threadIdx.x >> 5) * 2 + (lane >> 4);
+    const bool wide = p.ldy % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(Y) & 15u) == 0;
+    const bool words = p.ldy * sizeof(T) % 4 == 0 && (reinterpret_cast<uintptr_t>(Y) & 3u) == 0;
+    for (long long w = blockIdx.x; w < work; w += gridDim.x) {
+        const long long q = w / kt;
+        const int k_tile = static_cast<int>(w - q * kt);
+        const TileRow t = tile_row(p, off, first, q);
+        const int k0 = k_tile * 128 + part * 8;
+        uint32_t bits[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 16 * i;
+            const bool there = r < t.count && k0 < p.K;
+            bits[i] = there ? *reinterpret_cast<const uint32_t*>(p.Q + ((t.first + r) * p.ldq + k0) / 2) : 0u;
+            s[i] = there ? p.S[scale_at(q, kt, k_tile * 4 + part / 4, r)] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 16 * i;
+            const float x = __uint_as_float(s[i] == 0 ? 0x00400000u : s[i] == 255 ? 0x7fc00000u : s[i] << 23);
+            alignas(16) T out[8];
+            from_elements(bits[i], x, out);
+            constexpr int kVec = 8 * sizeof(T) / 16;
+            if (wide && k_tile * 128 + 128 <= p.K) {
+                if (r < t.count) {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) reinterpret_cast<uint4*>(Y + (t.first + r) * p.ldy + k0)[j] = reinterpret_cast<const uint4*>(out)[j];
+                }
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) reinterpret_cast<uint4*>(&rows[r0][part * 8])[j] = reinterpret_cast<const uint4*>(out)[j];
+            __syncwarp();
+            const int n = min(128, p.K - k_tile * 128);
+#pragma unroll
+            for (int x2 = 0; x2 < 2; ++x2) {  // the warp's two vectors
+                const int rr = (threadIdx.x >> 5) * 2 + x2;
+                if (rr + 16 * i >= t.count) continue;
+                T* dst = Y + (t.first + rr + 16 * i) * p.ldy + k_tile * 128;
+                if (words && sizeof(T) == 2 && n % 2 == 0) {
+#pragma unroll
+                    for (int j = lane * 2; j < 128; j += 64)
+                        if (j < n) *reinterpret_cast<uint32_t*>(dst + j) = *reinterpret_cast<const uint32_t*>(&rows[rr][j]);
+                } else {
+                    for (int j = lane; j < n; j += 32) dst[j] = rows[rr][j];
+                }
+            }
+            __syncwarp();
         }
     }
 }
@@ -223,9 +334,19 @@ int check_mx(const char* what, int64_t K, int64_t cols, int64_t groups, const vo
     return B200_OK;
 }
 
-int grid_for(const b200_handle* h, int64_t K, int64_t cols, int64_t groups) {
-    const int64_t tiles = (cols / 128 + std::max<int64_t>(1, std::min(groups, cols))) * ((K + 127) / 128);
-    return static_cast<int>(std::min<int64_t>(tiles, static_cast<int64_t>(h->sm_count) * 8));
+int launch_mx(const b200_handle* h, void (*kern)(MxParams), const MxParams& p, cudaStream_t stream) {
+    const int64_t tiles = (p.cols / 128 + std::max<int64_t>(1, std::min(p.groups, p.cols))) * ((p.K + 127) / 128);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, static_cast<int64_t>(h->sm_count) * 8)), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = h->pdl ? 1 : 0;
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p));
+    return B200_OK;
 }
 
 }  // namespace
@@ -248,19 +369,11 @@ extern "C" int b200_mxfp4_quantize(b200_handle* h, b200_stream stream, int trans
     if ((rc = poll_previous_launch(h)) || (rc = check_current_device(h))) return rc;
     const MxParams p = {X, ldx, static_cast<uint8_t*>(Q), ldq, static_cast<uint8_t*>(S), nullptr, 0, static_cast<int>(K), static_cast<int>(cols),
                         static_cast<int>(groups), offsets, h->status_word};
-    const int grid = grid_for(h, K, cols, groups);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define B200_QUANTIZE(T)                                                    \
-    do {                                                                    \
-        if (trans) mxfp4_quantize_kernel<T, true><<<grid, 256, 0, st>>>(p); \
-        else mxfp4_quantize_kernel<T, false><<<grid, 256, 0, st>>>(p);      \
-    } while (0)
-    if (x_type == B200_F32) B200_QUANTIZE(float);
-    else if (x_type == B200_F16) B200_QUANTIZE(__half);
-    else B200_QUANTIZE(__nv_bfloat16);
-#undef B200_QUANTIZE
-    B200_CUDA_TRY(cudaGetLastError());
-    return note_launch(h, st);
+    if (x_type == B200_F32) rc = launch_mx(h, trans ? mxfp4_quantize_across_kernel<float> : mxfp4_quantize_kernel<float>, p, st);
+    else if (x_type == B200_F16) rc = launch_mx(h, trans ? mxfp4_quantize_across_kernel<__half> : mxfp4_quantize_kernel<__half>, p, st);
+    else rc = launch_mx(h, trans ? mxfp4_quantize_across_kernel<__nv_bfloat16> : mxfp4_quantize_kernel<__nv_bfloat16>, p, st);
+    return rc ? rc : note_launch(h, st);
 }
 
 extern "C" int b200_mxfp4_dequantize(b200_handle* h, b200_stream stream, int64_t K, int64_t cols, const void* Q, int64_t ldq, const void* S, void* Y,
@@ -271,11 +384,9 @@ extern "C" int b200_mxfp4_dequantize(b200_handle* h, b200_stream stream, int64_t
     if ((rc = poll_previous_launch(h)) || (rc = check_current_device(h))) return rc;
     const MxParams p = {nullptr, 0, const_cast<uint8_t*>(static_cast<const uint8_t*>(Q)), ldq, const_cast<uint8_t*>(static_cast<const uint8_t*>(S)),
                         Y, ldy, static_cast<int>(K), static_cast<int>(cols), static_cast<int>(groups), offsets, h->status_word};
-    const int grid = grid_for(h, K, cols, groups);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (y_type == B200_F32) mxfp4_dequantize_kernel<float><<<grid, 256, 0, st>>>(p);
-    else if (y_type == B200_F16) mxfp4_dequantize_kernel<__half><<<grid, 256, 0, st>>>(p);
-    else mxfp4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
-    B200_CUDA_TRY(cudaGetLastError());
-    return note_launch(h, st);
+    if (y_type == B200_F32) rc = launch_mx(h, mxfp4_dequantize_kernel<float>, p, st);
+    else if (y_type == B200_F16) rc = launch_mx(h, mxfp4_dequantize_kernel<__half>, p, st);
+    else rc = launch_mx(h, mxfp4_dequantize_kernel<__nv_bfloat16>, p, st);
+    return rc ? rc : note_launch(h, st);
 }

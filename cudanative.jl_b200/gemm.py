@@ -21,10 +21,13 @@ from .array import CuHostArray, DevicePtr
 from .bfloat16 import BFloat16
 
 
+_TYPE_CODES = {BFloat16: _lib.BF16, np.float16: _lib.F16, np.float32: _lib.F32}
+
+
 def _type_code(t) -> int:
     """numpy dtype (float16 / float32) or the ``BFloat16`` tag -> the library's element tag."""
-    if t is BFloat16:
-        return _lib.BF16
+    if isinstance(t, type) and t in _TYPE_CODES:
+        return _TYPE_CODES[t]
     dt = np.dtype(t)
     if dt == np.float16:
         return _lib.F16
