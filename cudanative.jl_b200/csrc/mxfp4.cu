@@ -124,7 +124,7 @@ __device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off
 // values (16 bytes of a 16-bit type) each, so that a warp reads and writes whole lines; four lanes find a
 // block's largest magnitude with two shuffles.  A thread has eight vectors in flight.
 template <typename T>
-__global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxParams p) {
+__global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p) {
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
     griddep_launch_dependents();
     griddep_wait();
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxParams p) {
     const T* X = static_cast<const T*>(p.X);
     const long long work = tile_rows * kt;
     const int lane = threadIdx.x & 31, part = lane & 15;
-    const int r0 = (threadIdx.x >> 5) * 2 + (lane >> 4);
+    const int first_row = (threadIdx.x >> 5) * 2 + (lane >> 4);
     const bool wide = p.ldx % (16 / sizeof(T)) == 0 && (reinterpret_cast<uintptr_t>(X) & 15u) == 0;
     for (long long w = blockIdx.x; w < work; w += gridDim.x) {
         const long long q = w / kt;
@@ -141,24 +141,27 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxParams p) {
         const TileRow t = tile_row(p, off, first, q);
         const int k0 = k_tile * 128 + part * 8;
         constexpr int kVec = 8 * sizeof(T) / 16;
-        uint4 raw[8][kVec];
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+        const int r0 = first_row + 64 * half;
+        uint4 raw[4][kVec];
         const T* src = X + (t.first + r0) * p.ldx + k0;
         if (wide && k_tile * 128 + 128 <= p.K) {  // all loads before the first use
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < kVec; ++j)
                     raw[i][j] = r0 + 16 * i < t.count ? reinterpret_cast<const uint4*>(src + 16 * i * p.ldx)[j] : make_uint4(0, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
                 T* e = reinterpret_cast<T*>(raw[i]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) e[j] = r0 + 16 * i < t.count && k0 + j < p.K ? src[16 * i * p.ldx + j] : from_float<T>(0.0f);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const int r = r0 + 16 * i;
             const T* e = reinterpret_cast<const T*>(raw[i]);
             float v[8];
@@ -180,6 +183,7 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_kernel(const MxParams p) {
             s |= __shfl_xor_sync(0xffffffffu, s, 4);
             s |= __shfl_xor_sync(0xffffffffu, s, 8);
             if (part == 0) *reinterpret_cast<uint32_t*>(p.S + scale_at(q, kt, k_tile * 4, r)) = s;
+        }
         }
     }
 }
