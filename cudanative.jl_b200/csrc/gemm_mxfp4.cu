@@ -21,7 +21,7 @@ struct MxProblem {
 };
 
 template <int kBN, int kCtas, bool kPromote>
-int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     constexpr bool kSplit = kBN == 32;  // few columns: pairs of CTAs that may share a tile's inner dimension
     using Cfg = MxCfg<kBN, kCtas, kPromote, kSplit>;
     auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote, kSplit>;
@@ -46,12 +46,12 @@ int launch(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStre
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], tm[4], p));
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p));
     return B200_OK;
 }
 
 template <int kBN, int kCtas>
-int launch_typed(const CUtensorMap (&tm)[5], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch_typed(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     if (p.e.d_fmt == 0) {
         if constexpr (kBN <= 128) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
         else return fail(B200_UNSUPPORTED, "mxfp4: a binary32 D takes tiles of 128 columns at most");
@@ -91,12 +91,11 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     p.e.d_fmt = elem_fmt(g.d_type);
     p.status = h->status_word;
     p.wait_budget_ns = h->wait_budget_ns;
-    const int q = 16 / elem_bytes(g.d_type);
-    p.e.d_tma = !(reinterpret_cast<uintptr_t>(g.D) & 15u) && g.ldd % q == 0 && g.M % q == 0;
+    p.e.d_pairs = !(reinterpret_cast<uintptr_t>(g.D) & 3u) && g.ldd % 2 == 0;
 
     const int bn_local = tile_n / pair, bbox = std::min(bn_local, 128);
     const int64_t k_bytes = (g.K + 1) / 2;
-    CUtensorMap tm[5];
+    CUtensorMap tm[4];
     BatchDim b;
     b.count = g.stride_a != 0 ? g.groups : 1;
     b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
@@ -114,11 +113,6 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
         return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
     };
     if ((rc = scale_map(&tm[2], g.SA, sa_rows, 1, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, (tile_n + 127) / 128, "scales of B"))) return rc;
-    tm[4] = tm[1];  // never dereferenced unless replaced
-    if (p.e.d_tma && (rc = make_map_2d(&tm[4], map_type(g.d_type), elem_bytes(g.d_type), g.D, g.M, g.N, g.ldd, 128, g.d_type == B200_F32 ? 16 : 32,
-                                       CU_TENSOR_MAP_SWIZZLE_NONE, "D")))
-        return rc;
-
     const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * p.tiles_m;
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
     const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;

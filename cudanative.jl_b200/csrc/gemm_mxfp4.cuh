@@ -54,7 +54,7 @@ struct MxCfg {
     static constexpr int BBOX_BYTES = BBOX * BK / 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
     static constexpr int PROMOTE_KB = 8;
-    using Epi = EpilogueCfg<kBN, kPromote ? 16 : 32, false, 2>;
+    using Epi = EpilogueCfg<kBN, 0>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
     static constexpr int RECV_BYTES = kSplit ? 128 * Epi::COLS * 4 : 0;
@@ -66,7 +66,7 @@ struct MxCfg {
     static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 3 * STAGES + 2 + 2 * ACCS + 2 * Epi::BUFS;
+    static constexpr int NBARS = 3 * STAGES + 2 + 2 * ACCS;
     static_assert(!kSplit || (kCtas == 1 && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
@@ -77,8 +77,7 @@ struct MxCfg {
 template <int kBN, int kCtas, bool kPromote, bool kSplit>
 __global__ void __launch_bounds__(512, 1)
 gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                   const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
-                   const __grid_constant__ CUtensorMap tmD, const MxGemmParams p) {
+                   const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const MxGemmParams p) {
     using Cfg = MxCfg<kBN, kCtas, kPromote, kSplit>;
     using Epi = typename Cfg::Epi;
     constexpr int STAGES = Cfg::STAGES, ACCS = Cfg::ACCS;
@@ -87,9 +86,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-    const uint32_t epi_base = smem_base + STAGES * Cfg::STAGE_BYTES;
-    uint8_t* epi_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
-    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES;
     constexpr int kTableAt = kRecvAt + Cfg::RECV_BYTES;
     const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
     int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
@@ -103,7 +100,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + a); };
     auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (3 * STAGES + ACCS + a); };
     auto split_bar = [&](int i) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + i); };  // partial sums: full, empty
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (3 * STAGES + 2 * ACCS + 2 + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
@@ -131,7 +127,6 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         tma_prefetch_desc(&tmB);
         tma_prefetch_desc(&tmSA);
         tma_prefetch_desc(&tmSB);
-        tma_prefetch_desc(&tmD);
     }
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     tc_fence_before_sync();
@@ -142,8 +137,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     griddep_launch_dependents();
     griddep_wait();
 
-    bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<int*>(epi_gen));
-    if constexpr (kBN != 128) load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, 128, off, first128, reinterpret_cast<int*>(epi_gen));
+    bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<int*>(smem_gen));
+    if constexpr (kBN != 128) load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, 128, off, first128, reinterpret_cast<int*>(smem_gen));
     if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
         p.status[1] = static_cast<int>(blockIdx.x);
         p.status[2] = p.groups;
@@ -352,10 +347,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     } else {
         regs_inc<200>();
         const int wg = (warp - 4) >> 2;
-        const int at = wg * Epi::BUFS * Epi::BUF_BYTES;
-        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? kDrain : 0, false, kSplit>(p.e, &tmD, &tmD, wg, tmem_base, epi_base + at, epi_gen + at,
-                                                                           tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::BUFS), wc,
-                                                                           unit_first, unit_stride, num_units, split, decode);
+        run_epilogue<Epi, kBN, ACCS, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : ACCS == 1 ? -1 : 0, false, kSplit>(
+            p.e, wg, tmem_base, nullptr, tmem_full_bar(0), tmem_empty_bar(0), 0, 0, wc, unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit
