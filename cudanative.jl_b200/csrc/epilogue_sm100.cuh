@@ -96,7 +96,8 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                                              uint32_t tmem_empty, uint32_t cfull, uint32_t cempty, const WaitCtx& wc, int unit_first,
                                              int unit_stride, int num_units, const SplitParams& split, Decode decode) {
     constexpr int W = E::W, RING = E::RING > 0 ? E::RING : 1;
-    constexpr int kDrain = kPromoteKb < 0;  // one accumulator: read it out at once so that the next tile may begin
+    constexpr bool kDrain = kPromoteKb < 0;  // one accumulator: read it out at once so that the next tile may begin
+    constexpr bool kAhead = kPromoteKb <= 0 && E::RING == 0;
     const int et = static_cast<int>(threadIdx.x & 127);
     const int lane = static_cast<int>(threadIdx.x & 31);
     const uint32_t lane_base = static_cast<uint32_t>(((threadIdx.x >> 5) & 3) * 32) << 16;
@@ -142,6 +143,37 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld is warp-collective
             tc_fence_after_sync();
         };
+        // C read directly: W columns ahead, the first before the accumulator is waited for, where the registers
+        // are there for it (kAhead)
+        float c_next[W];
+        auto load_c = [&](int j) {
+            const int left = cols - j * W;
+            const long long at = (kPerGroup ? u.group * p.stride_c : 0) + m + (u.n0 + col0 + j * W) * p.ldc;
+            if (p.c_fmt == 0) {
+                const float* c = static_cast<const float*>(p.C) + at;
+                if (whole_rows && left >= W) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) c_next[i] = c[i * p.ldc];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) c_next[i] = m < p.M && i < left ? c[i * p.ldc] : 0.0f;
+                }
+            } else {
+                const unsigned short* c = static_cast<const unsigned short*>(p.C) + at;
+                unsigned short raw[W];
+                if (whole_rows && left >= W) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) raw[i] = c[i * p.ldc];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) raw[i] = m < p.M && i < left ? c[i * p.ldc] : static_cast<unsigned short>(0);
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    c_next[i] = p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(raw[i]) << 16) : __half2float(__ushort_as_half(raw[i]));
+            }
+        };
+        if (kAhead && has_c && !c_bulk && !sends && cols > 0) load_c(0);
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
             if constexpr (kSplit) {
@@ -178,18 +210,10 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 if (lane == 0) mbar_arrive(cempty + 8 * b);
                 ++c_count;
             } else if (has_c) {
-                const long long at = (kPerGroup ? u.group * p.stride_c : 0) + m + n * p.ldc;
+                if (!kAhead) load_c(j);
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    float c = 0.0f;
-                    if (m < p.M && i < left) {
-                        const long long e = at + i * p.ldc;
-                        c = p.c_fmt == 2   ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.C)[e])
-                            : p.c_fmt == 1 ? __half2float(static_cast<const __half*>(p.C)[e])
-                                           : static_cast<const float*>(p.C)[e];
-                    }
-                    r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * c));
-                }
+                for (int i = 0; i < W; ++i) r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * c_next[i]));
+                if (kAhead && (j + 1) * W < cols) load_c(j + 1);
             } else {
 #pragma unroll
                 for (int i = 0; i < W; ++i) r[i] = __float_as_uint(alpha * __uint_as_float(r[i]));
@@ -240,7 +264,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             float sum[E::COLS];
 #pragma unroll
             for (int i = 0; i < E::COLS; ++i) sum[i] = 0.0f;
-            for (int kb = 0; ok && kb < u.kb; kb += kPromoteKb, ++acc_count) {
+            for (int kb = 0; ok && kb < u.kb; kb += (kPromoteKb > 0 ? kPromoteKb : 1), ++acc_count) {
                 const uint32_t acc = acc_count % kAccs;
                 wait_acc(acc);
                 if (!ok) break;

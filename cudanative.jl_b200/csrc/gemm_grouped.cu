@@ -143,6 +143,10 @@ int launch_promote(const CUtensorMap (&tm)[3], const GroupedParams& p, int grid,
     B200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 64 || !((done.load(std::memory_order_relaxed) >> dev) & 1u)) {
         B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+        // the kernel deals out 168 registers a thread among its warpgroups: one built with fewer would wait for more
+        cudaFuncAttributes at;
+        B200_CUDA_TRY(cudaFuncGetAttributes(&at, kern));
+        if (at.numRegs != 168) return fail(B200_UNSUPPORTED, "grouped gemm: kernel built with " + std::to_string(at.numRegs) + " registers, not 168");
         if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};

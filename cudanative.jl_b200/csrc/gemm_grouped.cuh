@@ -272,6 +272,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     // rows of a group's last k-block; a ragged 16-row step has to be padded with zeros
     auto needs_tail = [&](const Unit& u) { return kRaggedK && (u.k_len % 16) != 0; };
 
+    // registers: 3 x 168 a thread at launch = 56 + 2 x 224; a binary32 result's sums stay in them
+    if (warp < 4) {
+    regs_dec<56>();
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
         if (lane == 0) {
@@ -428,11 +431,6 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             s = (s + kb1) % STAGES;
         }
         __syncwarp();
-    } else if (warp >= 4) {
-        const int wg = (warp - 4) >> 2;
-        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
-            p.e, wg, tmem_base, ring_gen + wg * Epi::RING * Epi::BUF_BYTES, tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::RING),
-            cfull_bar((2 + wg) * Epi::RING), wc, unit_first, unit_stride, num_units, split, decode);
     } else if (kRaggedK && warp == 2) {
         if constexpr (kRaggedK) {
             if (lane == 0 && p.e.beta != 0.0f && p.e.c_tma)
@@ -440,6 +438,13 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                                 unit_stride, num_units, decode);
         }
         __syncwarp();
+    }
+    } else {
+        regs_inc<224>();
+        const int wg = (warp - 4) >> 2;
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
+            p.e, wg, tmem_base, ring_gen + wg * Epi::RING * Epi::BUF_BYTES, tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::RING),
+            cfull_bar((2 + wg) * Epi::RING), wc, unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit

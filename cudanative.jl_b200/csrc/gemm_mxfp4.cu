@@ -20,16 +20,20 @@ struct MxProblem {
     const int32_t* offsets;
 };
 
-template <int kBN, int kCtas, bool kPromote>
+template <int kBN, int kCtas>
 int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     constexpr bool kSplit = kBN == 32;  // few columns: pairs of CTAs that may share a tile's inner dimension
-    using Cfg = MxCfg<kBN, kCtas, kPromote, kSplit>;
-    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kPromote, kSplit>;
+    using Cfg = MxCfg<kBN, kCtas, kSplit>;
+    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kSplit>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
     if (dev >= 64 || !((done.load(std::memory_order_relaxed) >> dev) & 1u)) {
         B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+        // the kernel deals out 128 registers a thread among its warpgroups: one built with fewer would wait for more
+        cudaFuncAttributes at;
+        B200_CUDA_TRY(cudaFuncGetAttributes(&at, kern));
+        if (at.numRegs != 128) return fail(B200_UNSUPPORTED, "mxfp4 gemm: kernel built with " + std::to_string(at.numRegs) + " registers, not 128");
         if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
@@ -50,21 +54,11 @@ int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStre
     return B200_OK;
 }
 
-template <int kBN, int kCtas>
-int launch_typed(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
-    if (p.e.d_fmt == 0) {
-        if constexpr (kBN <= 128) return launch<kBN, kCtas, true>(tm, p, grid, stream, pdl);
-        else return fail(B200_UNSUPPORTED, "mxfp4: a binary32 D takes tiles of 128 columns at most");
-    }
-    return launch<kBN, kCtas, false>(tm, p, grid, stream, pdl);
-}
-
-// Tile columns, by the mean length of the groups.  Two CTAs on 256 columns need a 16-bit D: a binary32 one
-// takes two accumulators (epilogue_sm100.cuh), for which tensor memory has no room beside the scales.
+// Tile columns, by the mean length of the groups.
 void pick_tile(const b200_handle* h, const MxProblem& g, int* tile_n, int* pair) {
     const int64_t n = (g.N + g.groups - 1) / g.groups;
     *tile_n = h->tile_n ? std::max(h->tile_n, 128) : n > 128 ? 256 : n > 32 ? 128 : 32;
-    if (*tile_n == 256 && (g.d_type == B200_F32 || g.M <= 128 || h->cta_pair == 1)) *tile_n = 128;
+    if (*tile_n == 256 && (g.M <= 128 || h->cta_pair == 1)) *tile_n = 128;
     *pair = *tile_n == 256 ? 2 : 1;
 }
 
@@ -119,9 +113,9 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
     if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
-    if (tile_n == 256) rc = launch_typed<256, 2>(tm, p, grid, stream, pdl);
-    else if (tile_n == 128) rc = launch_typed<128, 1>(tm, p, grid, stream, pdl);
-    else rc = launch_typed<32, 1>(tm, p, grid, stream, pdl);
+    if (tile_n == 256) rc = launch<256, 2>(tm, p, grid, stream, pdl);
+    else if (tile_n == 128) rc = launch<128, 1>(tm, p, grid, stream, pdl);
+    else rc = launch<32, 1>(tm, p, grid, stream, pdl);
     if (rc) return rc;
     h->last = {B200_KERNEL_TCGEN05, tile_n, 1, grid, pair};
     return B200_OK;
