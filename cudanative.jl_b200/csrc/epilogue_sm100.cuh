@@ -57,9 +57,10 @@ struct SplitParams {
 template <int kBN, int kRing>
 struct EpilogueCfg {
     static constexpr int COLS = kBN >= 64 ? kBN / 2 : kBN;  // per warp group; the second is idle below 64
-    static constexpr int W = 16;                            // columns per step
+    static constexpr int W = 32;                            // columns per step
+    static constexpr int CW = 16;                           // columns per copy of C
     static constexpr int RING = kRing;
-    static constexpr int BUF_BYTES = 128 * W * 4;
+    static constexpr int BUF_BYTES = 128 * CW * 4;
     static constexpr int BYTES = 2 * kRing * BUF_BYTES;
     static_assert(COLS % W == 0, "steps");
 };
@@ -70,19 +71,19 @@ __device__ __forceinline__ int columns_of(int tile_cols, int wg, int cols) { ret
 template <class E, class Decode>
 __device__ __forceinline__ void c_producer(const EpilogueParams& p, const CUtensorMap* tmC, uint32_t ring, uint32_t cfull, uint32_t cempty,
                                            const WaitCtx& wc, int unit_first, int unit_stride, int num_units, Decode decode) {
-    const uint32_t bytes = 128 * E::W * (p.c_fmt ? 2 : 4);
+    const uint32_t bytes = 128 * E::CW * (p.c_fmt ? 2 : 4);
     const uint64_t once = l2_policy_evict_first();
     uint32_t count[2] = {0, 0};
     for (int unit = unit_first; unit < num_units; unit += unit_stride) {
         const Unit u = decode(unit);
-        for (int j = 0; j * E::W < min(u.cols, E::COLS); ++j) {
+        for (int j = 0; j * E::CW < min(u.cols, E::COLS); ++j) {
 #pragma unroll
             for (int wg = 0; wg < 2; ++wg) {
-                if (j * E::W >= columns_of(u.cols, wg, E::COLS)) continue;
+                if (j * E::CW >= columns_of(u.cols, wg, E::COLS)) continue;
                 const uint32_t b = wg * E::RING + count[wg] % E::RING;
                 if (!mbar_wait(cempty + 8 * b, ((count[wg] / E::RING) & 1u) ^ 1u, wc, kWaitCTile)) return;
                 mbar_arrive_expect_tx(cfull + 8 * b, bytes);
-                tma_load_3d_hint(ring + b * E::BUF_BYTES, tmC, u.m0, u.n0 + wg * E::COLS + j * E::W, u.group, cfull + 8 * b, once);
+                tma_load_3d_hint(ring + b * E::BUF_BYTES, tmC, u.m0, u.n0 + wg * E::COLS + j * E::CW, u.group, cfull + 8 * b, once);
                 ++count[wg];
             }
         }
@@ -95,9 +96,9 @@ template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, boo
 __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, uint32_t tmem_base, const uint8_t* ring, uint32_t tmem_full,
                                              uint32_t tmem_empty, uint32_t cfull, uint32_t cempty, const WaitCtx& wc, int unit_first,
                                              int unit_stride, int num_units, const SplitParams& split, Decode decode) {
-    constexpr int W = E::W, RING = E::RING > 0 ? E::RING : 1;
+    constexpr int W = E::W, CW = E::CW, RING = E::RING > 0 ? E::RING : 1;
     constexpr bool kDrain = kPromoteKb < 0;  // one accumulator: read it out at once so that the next tile may begin
-    constexpr bool kAhead = kPromoteKb <= 0 && E::RING == 0;
+    constexpr bool kAhead = kPromoteKb == 0 && E::RING == 0;
     const int et = static_cast<int>(threadIdx.x & 127);
     const int lane = static_cast<int>(threadIdx.x & 31);
     const uint32_t lane_base = static_cast<uint32_t>(((threadIdx.x >> 5) & 3) * 32) << 16;
@@ -189,26 +190,26 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             }
             const int n = u.n0 + col0 + j * W, left = cols - j * W;
             if (c_bulk) {
-                const uint32_t b = c_count % RING;
-                ok = mbar_wait(cfull + 8 * b, (c_count / RING) & 1u, wc, kWaitCTile);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                const float* c = reinterpret_cast<const float*>(ring + b * E::BUF_BYTES) + et;
-                const unsigned short* ch = reinterpret_cast<const unsigned short*>(ring + b * E::BUF_BYTES) + et;
-                if (p.c_fmt == 2) {
 #pragma unroll
-                    for (int i = 0; i < W; ++i)
-                        r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * __uint_as_float(static_cast<uint32_t>(ch[i * 128]) << 16)));
-                } else if (p.c_fmt == 1) {
+                for (int half = 0; half < W / CW; ++half) {
+                    if (half * CW >= left) break;
+                    const uint32_t b = c_count % RING;
+                    ok = mbar_wait(cfull + 8 * b, (c_count / RING) & 1u, wc, kWaitCTile);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    const float* c = reinterpret_cast<const float*>(ring + b * E::BUF_BYTES) + et;
+                    const unsigned short* ch = reinterpret_cast<const unsigned short*>(ring + b * E::BUF_BYTES) + et;
 #pragma unroll
-                    for (int i = 0; i < W; ++i) r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * __half2float(__ushort_as_half(ch[i * 128]))));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * c[i * 128]));
+                    for (int i = 0; i < CW; ++i) {
+                        const float v = p.c_fmt == 0   ? c[i * 128]
+                                        : p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(ch[i * 128]) << 16)
+                                                       : __half2float(__ushort_as_half(ch[i * 128]));
+                        r[half * CW + i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[half * CW + i]), beta * v));
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(cempty + 8 * b);
+                    ++c_count;
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(cempty + 8 * b);
-                ++c_count;
             } else if (has_c) {
                 if (!kAhead) load_c(j);
 #pragma unroll
@@ -269,17 +270,13 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 wait_acc(acc);
                 if (!ok) break;
 #pragma unroll
-                for (int q = 0; q < E::COLS / W; q += 2) {
+                for (int q = 0; q < E::COLS / W; ++q) {
                     if (q * W < cols) {
-                        uint32_t r[2][W];
-                        tmem_ld_32x32b_x16(tmem_base + lane_base + acc * kBN + col0 + q * W, r[0]);
-                        if (q + 1 < E::COLS / W) tmem_ld_32x32b_x16(tmem_base + lane_base + acc * kBN + col0 + (q + 1) * W, r[1]);
+                        uint32_t r[W];
+                        tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < W; ++i) {
-                            sum[q * W + i] += __uint_as_float(r[0][i]);
-                            if (q + 1 < E::COLS / W) sum[(q + 1) * W + i] += __uint_as_float(r[1][i]);
-                        }
+                        for (int i = 0; i < W; ++i) sum[q * W + i] += __uint_as_float(r[i]);
                     }
                 }
                 release(acc);
@@ -302,7 +299,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             if (!ok) break;
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q)
-                if (q * W < cols) tmem_ld_32x32b_x16(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
+                if (q * W < cols) tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
             tmem_wait_ld();
             release(acc);
             ++acc_count;
@@ -318,7 +315,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             for (int j = 0; ok && j * W < cols; ++j) {
                 uint32_t r[W];
                 if (!empty) {
-                    tmem_ld_32x32b_x16(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
+                    tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
                     tmem_wait_ld();
                 } else {
 #pragma unroll

@@ -87,7 +87,8 @@ __device__ __forceinline__ void plain_store(const PlainParams& p, const float (&
 template <bool kTransA>
 __global__ void __launch_bounds__(256) grouped_plain_kernel(const PlainParams p) {
     __shared__ float sA[kTileK][kTile + 1], sB[kTileK][kTile + 1];
-    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
+    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
+    __shared__ unsigned long long sums[8];
     if (!load_groups<true>(p.offsets, p.groups, static_cast<int>(p.N), kTile, off, first, sums)) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
         return;

@@ -73,47 +73,61 @@ struct GroupedCfg {
 };
 
 // Offsets into shared memory, checked and, for kTiles, with an exclusive scan of the tile columns per
-// group in `first` (groups + 1 entries).  All kThreads threads; returns false when the offsets are no
+// group in `first` (groups + 1 entries); `first128`, where given, gets the same for tiles of 128.  No
+// offsets: one group of all columns.  All kThreads threads; returns false when the offsets are no
 // ascending sequence inside [0, total].
 template <bool kTiles, int kThreads = 256>
 __device__ __forceinline__ bool load_groups(const int* offsets, int groups, int total, int tile, int* off, int* first,
-                                            int* warp_sums) {
+                                            unsigned long long* warp_sums, int* first128 = nullptr) {
     constexpr int PER = kMaxGroups / kThreads + 1;  // entries 0 .. groups
     const int t = threadIdx.x;
+    if (!offsets) {
+        if (t < 2) {
+            off[t] = t ? total : 0;
+            if (kTiles) first[t] = t ? (total + tile - 1) / tile : 0;
+            if (first128) first128[t] = t ? (total + 127) / 128 : 0;
+        }
+        __syncthreads();
+        return true;
+    }
     bool bad = false;
-    for (int e = t; e <= groups; e += kThreads) off[e] = offsets ? offsets[e] : (e == 0 ? 0 : total);  // none: one group
-    __syncthreads();
-    int n[PER], sum = 0;
+    unsigned long long n[PER], sum = 0;  // tiles in the low half, tiles of 128 in the high one
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = t * PER + i;
         n[i] = 0;
+        if (e <= groups) off[e] = offsets[e];
         if (e < groups) {
-            const int a = off[e], b = off[e + 1];
+            const int a = offsets[e], b = offsets[e + 1];
             if (a < 0 || b < a || b > total) bad = true;
-            else n[i] = (b - a) / tile + ((b - a) % tile != 0);
+            else if (kTiles) n[i] = static_cast<unsigned long long>((b - a) / 128 + ((b - a) % 128 != 0)) << 32 | static_cast<unsigned>((b - a) / tile + ((b - a) % tile != 0));
         }
         sum += n[i];
     }
-    bad = __syncthreads_or(bad) != 0;
     if constexpr (kTiles) {
-        int incl = sum;
+        unsigned long long incl = sum;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, incl, d);
+            const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, d);
             if ((t & 31) >= d) incl += v;
         }
         if ((t & 31) == 31) warp_sums[t >> 5] = incl;
-        __syncthreads();
-        int base = incl - sum;
-        for (int w = 0; w < (t >> 5); ++w) base += warp_sums[w];
+        bad = __syncthreads_or(bad) != 0;
+        unsigned long long base = incl - sum;
+#pragma unroll
+        for (int w = 0; w < kThreads / 32 - 1; ++w) base += w < (t >> 5) ? warp_sums[w] : 0ull;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = t * PER + i;
-            if (e <= groups) first[e] = base;
+            if (e <= groups) {
+                first[e] = static_cast<int>(base);
+                if (first128) first128[e] = static_cast<int>(base >> 32);
+            }
             base += n[i];
         }
         __syncthreads();
+    } else {
+        bad = __syncthreads_or(bad) != 0;
     }
     return !bad;
 }
@@ -203,7 +217,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
     // the scan's scratch may lie in the first stage: nothing uses it yet
     const bool offsets_ok = load_groups<!kRaggedK, Cfg::THREADS>(p.offsets, p.groups, kRaggedK ? p.K : p.N, kBN, off, first,
-                                                   reinterpret_cast<int*>(smem_gen));
+                                                   reinterpret_cast<unsigned long long*>(smem_gen));
     if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
         p.status[1] = static_cast<int>(blockIdx.x);
         p.status[2] = p.groups;

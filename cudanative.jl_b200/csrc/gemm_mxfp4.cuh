@@ -140,8 +140,9 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     griddep_launch_dependents();
     griddep_wait();
 
-    bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<int*>(smem_gen));
-    if constexpr (kBN != 128) load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, 128, off, first128, reinterpret_cast<int*>(smem_gen));
+    // the scan's scratch may lie in the first stage: nothing uses it yet
+    const bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<unsigned long long*>(smem_gen),
+                                                            kBN == 128 ? nullptr : first128);
     if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
         p.status[1] = static_cast<int>(blockIdx.x);
         p.status[2] = p.groups;

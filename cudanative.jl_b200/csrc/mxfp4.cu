@@ -111,7 +111,7 @@ __device__ __forceinline__ TileRow tile_row(const MxParams& p, const int* off, c
 }
 
 // What every block of a launch needs: the groups' rows of scale tiles, and how many there are; 0 for bad offsets.
-__device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off, int* first, int* sums) {
+__device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off, int* first, unsigned long long* sums) {
     if (!p.offsets) return (p.cols + 127) / 128;
     if (!load_groups<true>(p.offsets, p.groups, p.cols, 128, off, first, sums)) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
@@ -125,7 +125,8 @@ __device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off
 // block's largest magnitude with two shuffles.  A thread has eight vectors in flight.
 template <typename T>
 __global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p) {
-    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
+    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
+    __shared__ unsigned long long sums[8];
     griddep_launch_dependents();
     griddep_wait();
     const long long tile_rows = scale_tile_rows(p, off, first, sums);
@@ -192,7 +193,8 @@ __global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p
 // reads 64 vectors' values of one k as a line; elements and scales of the tile go out through shared memory.
 template <typename T>
 __global__ void __launch_bounds__(256) mxfp4_quantize_across_kernel(const MxParams p) {
-    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
+    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
+    __shared__ unsigned long long sums[8];
     __shared__ __align__(16) uint8_t elements[128][64 + 16];
     __shared__ __align__(16) uint8_t scales[512];
     griddep_launch_dependents();
@@ -257,7 +259,8 @@ __global__ void __launch_bounds__(256) mxfp4_quantize_across_kernel(const MxPara
 // on 16 bytes are put together in shared memory and leave as 4-byte (or single) values, lane next to lane.
 template <typename T>
 __global__ void __launch_bounds__(256) mxfp4_dequantize_kernel(const MxParams p) {
-    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1], sums[8];
+    __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
+    __shared__ unsigned long long sums[8];
     __shared__ __align__(16) T rows[16][128 + 16 / sizeof(T)];
     griddep_launch_dependents();
     griddep_wait();
