@@ -54,16 +54,19 @@ struct SplitParams {
 };
 
 // kRing: chunks of C in flight per warp group; 0 where C is read directly.
-template <int kBN, int kRing>
+template <int kBN, int kRing, int kW = 32>
 struct EpilogueCfg {
     static constexpr int COLS = kBN >= 64 ? kBN / 2 : kBN;  // per warp group; the second is idle below 64
-    static constexpr int W = 32;                            // columns per step
+    static constexpr int W = kW;                            // columns per step
     static constexpr int CW = 16;                           // columns per copy of C
     static constexpr int RING = kRing;
     static constexpr int BUF_BYTES = 128 * CW * 4;
     static constexpr int BYTES = 2 * kRing * BUF_BYTES;
     static_assert(COLS % W == 0, "steps");
 };
+
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
 
 __device__ __forceinline__ int columns_of(int tile_cols, int wg, int cols) { return min(cols, max(0, tile_cols - wg * cols)); }
 
@@ -273,7 +276,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 for (int q = 0; q < E::COLS / W; ++q) {
                     if (q * W < cols) {
                         uint32_t r[W];
-                        tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r);
+                        tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + q * W, r);
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < W; ++i) sum[q * W + i] += __uint_as_float(r[i]);
@@ -299,7 +302,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             if (!ok) break;
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q)
-                if (q * W < cols) tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
+                if (q * W < cols) tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
             tmem_wait_ld();
             release(acc);
             ++acc_count;
@@ -315,7 +318,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             for (int j = 0; ok && j * W < cols; ++j) {
                 uint32_t r[W];
                 if (!empty) {
-                    tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
+                    tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
                     tmem_wait_ld();
                 } else {
 #pragma unroll

@@ -361,7 +361,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0 && cta_rank == 0) {
+        // The whole warp walks the loop and one lane issues: see umma_mxf4 in ptx_sm100.cuh.
+        if (cta_rank == 0) {
+            const uint32_t lead = elect_lane();
             const uint32_t idesc0 = make_idesc_f16_f32(Cfg::BM * kCtas, 0, kAMn ? 1 : 0, kBMn ? 1 : 0, p.ab_bf16 ? 1 : 0);
             const uint64_t da0 = kAMn ? make_smem_desc(smem_base, 8192, 1024, kSwizzle128B)
                                       : make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
@@ -370,44 +372,48 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             constexpr uint32_t kStepA = (kAMn ? 2048 : 32) >> 4, kStepB = (kBMn ? 2048 : 32) >> 4;
             int s = 0;
             uint32_t ph = 0, tail_ph = 0, ucount = 0;
-            bool ok = true;
+            bool ok = true, ready = false;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
                 // an empty group has no accumulator
-                const uint32_t idesc = idesc0 | (static_cast<uint32_t>(inst_n(u) >> 3) << 17);
-                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                const int kb_total = __shfl_sync(0xffffffffu, u.kb, 0);
+                const uint32_t idesc = idesc0 | (static_cast<uint32_t>(__shfl_sync(0xffffffffu, inst_n(u), 0) >> 3) << 17);
+                // 16-row steps of the last k-block; whether it has to be padded with zeros first
+                const int last_steps = min(Cfg::BK / 16, (u.k_len - (u.kb0 + kb_total - 1) * Cfg::BK + 15) / 16);
+                const bool tail = needs_tail(u);
+                for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     const uint32_t acc = ucount & 1u;
+                    const bool last = kb + 1 == kb_total;
                     const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
-                    const bool end = kb + 1 == u.kb || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
-                    if (begin) {
-                        ok = mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty);
-                        if (!ok) break;
+                    const bool end = last || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
+                    if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    if (ok && !ready) ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage));
+                    if (ok && last && tail) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(s), (tail_ph >> s) & 1u, wc, kWaitTail));
+                        tail_ph ^= 1u << s;
                     }
-                    ok = mbar_wait(full_bar(s), ph, wc, kWaitFullStage);
                     if (!ok) break;
-                    int steps = Cfg::BK / 16;
-                    if (kb + 1 == u.kb) {
-                        steps = min(steps, (u.k_len - (u.kb0 + kb) * Cfg::BK + 15) / 16);
-                        if (needs_tail(u)) {
-                            ok = mbar_wait(tail_ready_bar(s), (tail_ph >> s) & 1u, wc, kWaitTail);
-                            if (!ok) break;
-                            tail_ph ^= 1u << s;
-                        }
-                    }
                     tc_fence_after_sync();
+                    // look at the next stage now: the answer arrives while this one's products are issued
+                    const int s1 = s + 1 == STAGES ? 0 : s + 1;
+                    const bool next = mbar_test(full_bar(s1), ph ^ (s1 == 0));
                     const uint32_t d_tmem = tmem_base + acc * kBN;
                     const uint64_t da = da0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
                     const uint64_t db = db0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
+                    const int steps = last ? last_steps : Cfg::BK / 16;
 #pragma unroll
                     for (int k = 0; k < Cfg::BK / 16; ++k)
-                        if (k < steps) umma_f16<kCtas>(d_tmem, da + k * kStepA, db + k * kStepB, idesc, (begin && k == 0) ? 0u : 1u);
-                    if constexpr (kPair) umma_commit_pair(empty_bar(s));
-                    else umma_commit<kCtas>(empty_bar(s));
-                    if (end) {
-                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                        else umma_commit<kCtas>(tmem_full_bar(acc));
-                        ++ucount;
+                        if (k < steps) umma_f16_warp<kCtas>(lead, d_tmem, da + k * kStepA, db + k * kStepB, idesc, (begin && k == 0) ? 0u : 1u);
+                    if (lead) {
+                        if constexpr (kPair) umma_commit_pair(empty_bar(s));
+                        else umma_commit<kCtas>(empty_bar(s));
+                        if (end) {
+                            if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                            else umma_commit<kCtas>(tmem_full_bar(acc));
+                        }
                     }
+                    ucount += end ? 1u : 0u;
+                    ready = __all_sync(0xffffffffu, next);
                 }
             }
         }

@@ -590,6 +590,33 @@ __device__ __forceinline__ void umma_mxf4(uint32_t lead, uint32_t d_tmem, uint64
     }
 }
 
+// umma_f16 in that form.
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_f16_warp(uint32_t lead, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+    if constexpr (kCtaGroup == 1) {
+        asm volatile(
+            "{\n"
+            ".reg .pred p, q;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "setp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+            "}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n"
+            ".reg .pred p, q;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "setp.ne.b32 q, %5, 0;\n"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+            "}" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lead)
+            : "memory");
+    }
+}
+
 // 1 in one lane of a converged warp, 0 in the others.
 __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t r;
