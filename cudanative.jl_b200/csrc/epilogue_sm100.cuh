@@ -46,9 +46,10 @@ struct Unit {
 
 // With few tiles the two CTAs of a cluster take half of a tile's inner dimension each: CTA 1 sends its sums
 // into CTA 0's shared memory, CTA 0 adds them to its own (always in this order) and stores.
+constexpr int kSplitRow = 36;  // words per row of the receiver's buffer: 32 columns, and 4 against bank conflicts
 struct SplitParams {
     int role = -1;       // -1: whole tiles, 0: receives and stores, 1: sends
-    const float* recv;   // [columns][128]
+    const float* recv;   // [128][kSplitRow]
     uint32_t recv_addr;
     uint32_t full_bar, empty_bar;
 };
@@ -113,7 +114,9 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
     uint32_t acc_count = 0, split_count = 0, c_count = 0;
     bool ok = true;
     const bool sends = kSplit && split.role == 1, receives = kSplit && split.role == 0;
-    const uint32_t remote = kSplit ? mapa_shared(split.recv_addr, 0) : 0u;
+    const uint32_t remote = kSplit ? mapa_shared(split.recv_addr + et * kSplitRow * 4, 0) : 0u;
+    const uint32_t remote_bar = kSplit ? mapa_shared(split.full_bar, 0) : 0u;
+    static_assert(!kSplit || (E::COLS == W && W == 32), "partial sums are one step of columns");
 
     for (int unit = unit_first; unit < num_units; unit += unit_stride) {
         const Unit u = decode(unit);
@@ -121,16 +124,32 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
         const int m = u.m0 + et;
         const bool whole_rows = u.m0 + (et & ~31) + 32 <= p.M;  // of this warp
 
-        // room in the receiver's buffer, or the sender's sums in it
-        auto split_begin = [&]() {
-            if (sends) ok = ok && mbar_wait_cluster(split.empty_bar, (split_count & 1u) ^ 1u, wc, kWaitPartial);
-            if (receives) ok = ok && mbar_wait_cluster(split.full_bar, split_count & 1u, wc, kWaitPartial);
-            ok = __all_sync(0xffffffffu, ok);
-        };
-        auto split_end = [&]() {
-            __syncwarp();
-            if (lane == 0 && sends) mbar_arrive_cluster(split.full_bar, 0);
-            if (lane == 0 && receives) mbar_arrive_cluster(split.empty_bar, 1);
+        // partial sums of the tile's columns, rounded up to four
+        auto exchange = [&](uint32_t (&r)[W]) {
+            if (sends) {
+                ok = mbar_wait_cluster(split.empty_bar, (split_count & 1u) ^ 1u, wc, kWaitPartial);  // room over there
+                ok = __all_sync(0xffffffffu, ok);
+#pragma unroll
+                for (int i = 0; i < W; i += 4)
+                    if (ok && i < cols) st_async_cluster(remote + i * 4, r + i, remote_bar);
+            } else {
+                if (et == 0) mbar_arrive_expect_tx(split.full_bar, 128 * ((cols + 3) / 4 * 4) * 4);
+                ok = mbar_wait_cluster(split.full_bar, split_count & 1u, wc, kWaitPartial);
+                ok = __all_sync(0xffffffffu, ok);
+                const float* in = split.recv + et * kSplitRow;
+#pragma unroll
+                for (int i = 0; i < W; i += 4) {
+                    if (ok && i < cols) {
+                        const float4 v = *reinterpret_cast<const float4*>(in + i);
+                        r[i] = __float_as_uint(__uint_as_float(r[i]) + v.x);
+                        r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) + v.y);
+                        r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) + v.z);
+                        r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) + v.w);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(split.empty_bar, 1);
+            }
             ++split_count;
         };
         // the accumulator has been read: the arrival carries no data, only that
@@ -178,18 +197,19 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             }
         };
         if (kAhead && has_c && !c_bulk && !sends && cols > 0) load_c(0);
+        if (!kAhead && has_c && !c_bulk) {
+            // no registers to hold them: bring the warp's lines of C into L2 meanwhile, a lane to a column
+            const int bytes = p.c_fmt == 0 ? 4 : 2, row = u.m0 + (et & ~31);
+            for (int j = lane; j < cols; j += 32) {
+                const long long at = (kPerGroup ? u.group * p.stride_c : 0) + row + (u.n0 + col0 + j) * p.ldc;
+                if (row < p.M) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.C) + at * bytes));
+            }
+        }
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
             if constexpr (kSplit) {
-                if (sends) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) st_cluster_u32(remote + ((j * W + i) * 128 + et) * 4, r[i]);
-                    return;
-                }
-                if (receives) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + split.recv[(j * W + i) * 128 + et]);
-                }
+                if (sends || receives) exchange(r);
+                if (sends || !ok) return;
             }
             const int n = u.n0 + col0 + j * W, left = cols - j * W;
             if (c_bulk) {
@@ -235,32 +255,34 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 }
                 return;
             }
-            uint32_t v[W / 2];  // columns 2 i and 2 i + 1, rounded
-#pragma unroll
-            for (int i = 0; i < W; i += 2) {
-                if (d_fmt == 2) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                    v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                } else {
-                    const __half2 h = __floats2half2_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
-                    v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
-            unsigned short* d = static_cast<unsigned short*>(p.D) + at;
-            if (whole_rows && left >= W && p.d_pairs) {
-                // the even lane stores rows m, m + 1 of the first column of two, the odd lane m - 1, m of the second
-                const int odd = lane & 1;
-                const uint32_t pick = odd ? 0x3276u : 0x5410u;
-                d += odd * (p.ldd - 1);
+            if constexpr (!kF32) {
+                uint32_t v[W / 2];  // columns 2 i and 2 i + 1, rounded
 #pragma unroll
                 for (int i = 0; i < W; i += 2) {
-                    const uint32_t x = __shfl_xor_sync(0xffffffffu, v[i / 2], 1);
-                    *reinterpret_cast<uint32_t*>(d + i * p.ldd) = __byte_perm(v[i / 2], x, pick);
+                    if (d_fmt == 2) {
+                        const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                        v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        const __half2 h = __floats2half2_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+                        v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
                 }
-            } else if (m < p.M) {
+                unsigned short* d = static_cast<unsigned short*>(p.D) + at;
+                if (whole_rows && left >= W && p.d_pairs) {
+                    // the even lane stores rows m, m + 1 of the first column of two, the odd lane m - 1, m of the second
+                    const int odd = lane & 1;
+                    const uint32_t pick = odd ? 0x3276u : 0x5410u;
+                    d += odd * (p.ldd - 1);
 #pragma unroll
-                for (int i = 0; i < W; ++i)
-                    if (i < left) d[i * p.ldd] = static_cast<unsigned short>(v[i / 2] >> (16 * (i & 1)));
+                    for (int i = 0; i < W; i += 2) {
+                        const uint32_t x = __shfl_xor_sync(0xffffffffu, v[i / 2], 1);
+                        *reinterpret_cast<uint32_t*>(d + i * p.ldd) = __byte_perm(v[i / 2], x, pick);
+                    }
+                } else if (m < p.M) {
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        if (i < left) d[i * p.ldd] = static_cast<unsigned short>(v[i / 2] >> (16 * (i & 1)));
+                }
             }
         };
 
@@ -284,7 +306,6 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 }
                 release(acc);
             }
-            if (kSplit && (sends || receives) && cols > 0) split_begin();
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q) {
                 if (ok && q * W < cols) {
@@ -294,7 +315,6 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                     finish(q, r);
                 }
             }
-            if (kSplit && ok && (sends || receives) && cols > 0) split_end();
         } else if constexpr (kDrain) {
             uint32_t r[E::COLS / W][W];
             const uint32_t acc = acc_count % kAccs;
@@ -314,7 +334,6 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             const uint32_t acc = acc_count % kAccs;
             if (!empty) wait_acc(acc);
             if (!ok) break;
-            if (kSplit && (sends || receives) && cols > 0) split_begin();
             for (int j = 0; ok && j * W < cols; ++j) {
                 uint32_t r[W];
                 if (!empty) {
@@ -326,7 +345,6 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 }
                 finish(j, r);
             }
-            if (kSplit && ok && (sends || receives) && cols > 0) split_end();
             if (!empty) {
                 release(acc);
                 ++acc_count;

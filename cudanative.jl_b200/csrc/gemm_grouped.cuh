@@ -60,7 +60,7 @@ struct GroupedCfg {
     using Epi = EpilogueCfg<kBN, kRaggedK ? 3 : 0>;
     static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int RECV_BYTES = kSplit ? 128 * Epi::COLS * 4 : 0;
+    static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int TMEM_COLS = 2 * kBN < 32 ? 32 : 2 * kBN;
@@ -195,8 +195,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         for (int a = 0; a < 2; ++a) {
             mbar_init(tmem_full_bar(a), 1);
             mbar_init(tmem_empty_bar(a), 8 * kCtas);
-            mbar_init(split_bar(a), 4);
         }
+        mbar_init(split_bar(0), 1);  // the receiver's arrive; it expects the sender's bytes
+        mbar_init(split_bar(1), 4);  // the receiver's four warps
         for (int b = 0; b < 2 * Epi::RING; ++b) {
             mbar_init(cfull_bar(b), 1);
             mbar_init(cfull_bar(2 * Epi::RING + b), 4);  // free again: the warp group's four warps

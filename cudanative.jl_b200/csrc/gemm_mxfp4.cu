@@ -54,12 +54,19 @@ int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStre
     return B200_OK;
 }
 
-// Tile columns, by the mean length of the groups.
+// Tile columns, by the mean length of the groups.  256 columns leave tensor memory for one accumulator: its
+// reading out is not hidden, nor is C read ahead.  192 have two.  Measured, 256 against 192: 8192 x 8192, K =
+// 8192 210 / 250 us, K = 512 50 / 48 us; with a Float32 C, 8192 x 8192, K = 1024 118 / 111 us, K = 4096 149 / 160 us,
+// and where two rounds of tiles are all there is, 4100 x 1111, K = 4096 33 / 24 us.
 void pick_tile(const b200_handle* h, const MxProblem& g, int* tile_n, int* pair) {
     const int64_t n = (g.N + g.groups - 1) / g.groups;
     *tile_n = h->tile_n ? std::max(h->tile_n, 128) : n > 128 ? 256 : n > 32 ? 128 : 32;
     if (*tile_n == 256 && (g.M <= 128 || h->cta_pair == 1)) *tile_n = 128;
-    *pair = *tile_n == 256 ? 2 : 1;
+    if (*tile_n == 256) {
+        const int64_t units = (g.M + 255) / 256 * (g.N / 256 + std::min(g.groups, g.N));
+        if (g.beta != 0.0f ? (g.K <= 2048 || units <= h->sm_count) : g.K <= 512) *tile_n = 192;
+    }
+    *pair = *tile_n >= 192 ? 2 : 1;
 }
 
 int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
@@ -114,6 +121,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
     if (tile_n == 256) rc = launch<256, 2>(tm, p, grid, stream, pdl);
+    else if (tile_n == 192) rc = launch<192, 2>(tm, p, grid, stream, pdl);
     else if (tile_n == 128) rc = launch<128, 1>(tm, p, grid, stream, pdl);
     else rc = launch<32, 1>(tm, p, grid, stream, pdl);
     if (rc) return rc;

@@ -14,9 +14,9 @@
 // instead of 224 us without it; issued one stage ahead 437 us.)
 //
 // A tile's scales always come from whole tiles of 128 columns, counted from the group's first column, as
-// they were quantised.  A tile of 32 columns may begin inside one: the warps that carry its scales put the
-// rows that it starts with into the first column (the products' scale addresses stay multiples of 4 columns;
-// an odd one is a misaligned address).
+// they were quantised.  A tile of 32 columns may begin at row 32, 64 or 96 of one: the warps that carry its
+// scales put those rows into the first column, since an odd column is no legal scale address.  A tile of 192
+// begins at row 0 or 64, which is column 0 or 2.
 //
 // One accumulator takes the whole sum in every case: the products have so few bits that the tensor core's
 // truncation hardly meets one (K = 8192: exact on normal data, 1.7e-7 of the result with values spread over
@@ -60,12 +60,13 @@ struct MxCfg {
     using Epi = EpilogueCfg<kBN, 0>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int RECV_BYTES = kSplit ? 128 * Epi::COLS * 4 : 0;
+    static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
-    static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int ACCS = kBN <= 192 ? 2 : 1;
     static constexpr int SCALE_COLS = 8 * (1 + B_TILES);  // per set: 2 x 4 for A, 2 x 4 per scale tile for B
     static constexpr int SCALE_AT = ACCS * kBN;
+    static constexpr int MOST = (512 - SCALE_AT) / SCALE_COLS < 8 ? (512 - SCALE_AT) / SCALE_COLS : 8;  // a set of scales per stage
+    static constexpr int STAGES = BUDGET / STAGE_BYTES > MOST ? MOST : BUDGET / STAGE_BYTES;
     static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
@@ -74,7 +75,7 @@ struct MxCfg {
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
-    static_assert(kBN == 32 || kBN == 128 || kBN == 256, "a tile of columns begins on a multiple of 32 inside its scale tile");
+    static_assert(kBN == 32 || kBN == 128 || kBN == 192 || kBN == 256, "a tile of columns begins on a multiple of 32 inside its scale tile");
 };
 
 template <int kBN, int kCtas, bool kSplit>
@@ -124,7 +125,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             mbar_init(tmem_full_bar(a), 1);
             mbar_init(tmem_empty_bar(a), 8 * kCtas);
         }
-        for (int i = 0; i < 2; ++i) mbar_init(split_bar(i), 4);
+        mbar_init(split_bar(0), 1);  // the receiver's arrive; it expects the sender's bytes
+        mbar_init(split_bar(1), 4);  // the receiver's four warps
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
@@ -243,6 +245,8 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             bool ok = true, ready = false;
             for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
                 const Unit u = decode(unit);
+                // 192 columns begin at row 0 or 64 of their scale tile: two columns of 32 rows further
+                const uint32_t shift = kBN == 192 ? __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0) : 0u;
                 const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
                 for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                     const uint32_t acc = ucount % ACCS;
@@ -256,7 +260,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     const int s1 = s + 1 == STAGES ? 0 : s + 1;
                     const bool next = mbar_test(full_bar(s1), ph ^ (s1 == 0));
                     const uint64_t step = static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8;
+                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + s * Cfg::SCALE_COLS, sfb = sfa + 8 + shift;
                     const int steps = min(4, (p.K - (kb_first + kb) * Cfg::BK + 63) / 64);
                     const uint32_t d_tmem = tmem_base + acc * kBN;
 #pragma unroll

@@ -221,9 +221,12 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
     }
 }
 
-// Store to the shared memory of a CTA of this cluster (an address from mapa_shared).
-__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+// Store 16 bytes to the shared memory of a CTA of this cluster and count them on a barrier there (both
+// addresses from mapa_shared): the barrier's phase says that the bytes have landed, no fence is needed.
+__device__ __forceinline__ void st_async_cluster(uint32_t addr, const uint32_t* v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar)
+                 : "memory");
 }
 
 // Bounded wait for a 32-bit word in global memory to become non-zero.  The word is written by a
