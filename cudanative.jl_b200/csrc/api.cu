@@ -212,6 +212,9 @@ int poll_previous_launch(b200_handle* h) {
     int word[4] = {0, 0, 0, 0};
     int rc = read_status(h, word);
     if (rc) return rc;
+    if (word[0] == kBadOffsets)
+        return fail(B200_INVALID_ARG, "an earlier launch of this handle found group offsets that decrease or leave the matrix; it wrote "
+                                      "nothing.  This call enqueued nothing.");
     if (word[0] != 0)
         return fail(B200_DEVICE_TIMEOUT, "a bounded wait ran out on the device in an earlier launch of this handle (wait id " +
                                              std::to_string(word[0]) + ", block " + std::to_string(word[1]) +

@@ -245,16 +245,16 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     const CUtensorMapDataType dt = map_type(g.ab_type);
     CUtensorMap tm[3];
     if (g.ragged_k) {
-        if ((rc = make_map_2d(&tm[0], dt, 2, g.A, g.M, g.K, g.lda, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "A"))) return rc;
-        if ((rc = make_map_2d(&tm[1], dt, 2, g.B, g.N, g.K, g.ldb, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
+        if ((rc = encode_map_2d(&tm[0], dt, 2, g.A, g.M, g.K, g.lda, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "A"))) return rc;
+        if ((rc = encode_map_2d(&tm[1], dt, 2, g.B, g.N, g.K, g.ldb, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
     } else {
         BatchDim b;
         b.count = g.stride_a != 0 ? g.groups : 1;
         b.stride = b.count > 1 ? g.stride_a : g.lda * (g.transA ? g.M : g.K);
-        if (g.transA) rc = make_map_2d(&tm[0], dt, 2, g.A, g.K, g.M, g.lda, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A (row-major)", b);
-        else rc = make_map_2d(&tm[0], dt, 2, g.A, g.M, g.K, g.lda, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "A (column-major)", b);
+        if (g.transA) rc = encode_map_2d(&tm[0], dt, 2, g.A, g.K, g.M, g.lda, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A (row-major)", b);
+        else rc = encode_map_2d(&tm[0], dt, 2, g.A, g.M, g.K, g.lda, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "A (column-major)", b);
         if (rc) return rc;
-        if ((rc = make_map_2d(&tm[1], dt, 2, g.B, g.K, g.N, g.ldb, 64, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
+        if ((rc = encode_map_2d(&tm[1], dt, 2, g.B, g.K, g.N, g.ldb, 64, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
     }
     // C of a ragged-K product by bulk copies: whole 16-byte chunks of rows, matrices that do not overlap
     const int cq = 16 / elem_bytes(g.c_type);
@@ -266,7 +266,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
         BatchDim b;
         b.count = g.groups;
         b.stride = g.groups > 1 ? g.stride_c : g.ldc * g.N;
-        if ((rc = make_map_2d(&tm[2], map_type(g.c_type), elem_bytes(g.c_type), g.C, g.M, g.N, g.ldc, 128, 16, CU_TENSOR_MAP_SWIZZLE_NONE, "C", b)))
+        if ((rc = encode_map_2d(&tm[2], map_type(g.c_type), elem_bytes(g.c_type), g.C, g.M, g.N, g.ldc, 128, 16, CU_TENSOR_MAP_SWIZZLE_NONE, "C", b)))
             return rc;
     }
 

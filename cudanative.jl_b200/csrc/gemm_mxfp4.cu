@@ -100,8 +100,8 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     BatchDim b;
     b.count = g.stride_a != 0 ? g.groups : 1;
     b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
-    if ((rc = make_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
-    if ((rc = make_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
+    if ((rc = encode_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
+    if ((rc = encode_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
     // scales: tiles of 128 words, K tiles, rows of tiles; a copy takes 2 along K
     const int64_t kt = (g.K + 127) / 128, sa_rows = p.a_tile_rows * b.count;
     const int64_t sb_rows = b200_mxfp4_scale_bytes(g.K, g.N, g.offsets ? g.groups : 0) / 512 / kt;
@@ -111,7 +111,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
         d.count = rows;
         d.stride = kt * 128;
         d.box = box_rows;
-        return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
+        return encode_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
     };
     if ((rc = scale_map(&tm[2], g.SA, sa_rows, 1, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, (tile_n + 127) / 128, "scales of B"))) return rc;
     const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * p.tiles_m;

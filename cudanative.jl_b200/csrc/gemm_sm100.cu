@@ -35,11 +35,11 @@ EncodeFn get_encode_fn() {
 struct MapKey {
     const void* base;
     int64_t inner, outer, ld, batch_count, batch_stride;
-    uint32_t box_inner, box_outer, box_batch;
+    uint32_t box_inner, box_outer;
     int dt, sw;
     bool operator==(const MapKey& o) const {
         return base == o.base && inner == o.inner && outer == o.outer && ld == o.ld && batch_count == o.batch_count &&
-               batch_stride == o.batch_stride && box_inner == o.box_inner && box_outer == o.box_outer && box_batch == o.box_batch && dt == o.dt && sw == o.sw;
+               batch_stride == o.batch_stride && box_inner == o.box_inner && box_outer == o.box_outer && dt == o.dt && sw == o.sw;
     }
 };
 struct MapCache {
@@ -78,14 +78,9 @@ thread_local MapCache g_map_cache;
 
 }  // namespace
 
-int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
-                int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
-                const char* what, BatchDim batch) {
-    const MapKey mk{base, inner, outer, ld, batch.count, batch.stride, box_inner, box_outer, batch.box, static_cast<int>(dt), static_cast<int>(sw)};
-    if (const CUtensorMap* hit = g_map_cache.find(mk)) {
-        *tm = *hit;
-        return B200_OK;
-    }
+int encode_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
+                  int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
+                  const char* what, BatchDim batch) {
     EncodeFn enc = get_encode_fn();
     if (!enc) return fail(B200_CUDA_ERROR, "cuTensorMapEncodeTiled entry point not found");
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer),
@@ -99,11 +94,23 @@ int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const v
     if (r != CUDA_SUCCESS)
         return fail(B200_CUDA_ERROR, std::string("cuTensorMapEncodeTiled failed for ") + what + " (CUresult " +
                                          std::to_string(static_cast<int>(r)) + ")");
-    g_map_cache.insert(mk, *tm);
     return B200_OK;
 }
 
 namespace {
+
+int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
+                int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
+                const char* what, BatchDim batch = BatchDim()) {
+    const MapKey mk{base, inner, outer, ld, batch.count, batch.stride, box_inner, box_outer, static_cast<int>(dt), static_cast<int>(sw)};
+    if (const CUtensorMap* hit = g_map_cache.find(mk)) {
+        *tm = *hit;
+        return B200_OK;
+    }
+    if (int rc = encode_map_2d(tm, dt, elem_bytes, base, inner, outer, ld, box_inner, box_outer, sw, what, batch)) return rc;
+    g_map_cache.insert(mk, *tm);
+    return B200_OK;
+}
 
 // The opt-in to more than 48 KiB of dynamic shared memory is per device and per kernel: made once
 // (this also makes the driver load the kernel, which a caller may want to have happen at start-up).

@@ -15,9 +15,9 @@ struct BatchDim {
 
 // Tensor map over a column-major matrix: dim0 (contiguous) has `inner` elements, dim1 has `outer`
 // elements `ld` elements apart; batched problems add dim2 = matrix of the batch (box extent 1 unless asked for).
-int make_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
-                int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
-                const char* what, BatchDim batch = BatchDim());
+int encode_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
+                  int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
+                  const char* what, BatchDim batch = BatchDim());
 
 inline CUtensorMapDataType map_type(int type) {  // B200_F16 / B200_F32 / B200_BF16
     return type == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : (type == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);

@@ -298,3 +298,153 @@ def test_a_layer_forward_and_backward(handle):
     close(value(Array(dX), BFloat16), *grouped_ref(w, g, None, off, 1.0, 0.0, False, np.zeros((K, T))), M, BFloat16, "input gradient")
     exact, S = grouped_k_ref(x, g, [acc[:, e * M:(e + 1) * M].astype(np.float64) for e in range(4)], off, 1.0, 1.0)
     close(value(Array(dW), F32), np.hstack(exact), np.hstack(S), max(sizes), F32, "weight gradient")
+
+
+@pytest.mark.parametrize("max_ctas", [1, 2, 3, 10])
+@pytest.mark.parametrize("tile_n,cta_pair", [(0, 0), (64, 1), (128, 1), (128, 2), (256, 2)])
+def test_few_ctas_walk_many_tiles(handle, max_ctas, tile_n, cta_pair):
+    """Every barrier goes through many phases, the ring wraps, accumulators change hands."""
+    handle.set_option(_lib.OPT_MAX_CTAS, max_ctas)
+    for d_type in (BFloat16, F32):
+        run_grouped(handle, [3, 0, 70, 300, 1, 31], 648, 264, d_type=d_type, tile_n=tile_n, cta_pair=cta_pair)
+        run_grouped_k(handle, [3, 0, 70, 300, 1, 31, 129], 392, 328, d_type=d_type, beta=1.0, tile_n=tile_n, cta_pair=cta_pair)
+    handle.set_option(_lib.OPT_PDL, 0)
+    run_grouped(handle, [1, 0, 2, 7], 648, 1032, tile_n=tile_n, cta_pair=cta_pair)
+    run_grouped_k(handle, [5, 77], 264, 72, tile_n=tile_n, cta_pair=cta_pair)
+
+
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+@pytest.mark.parametrize("transA", [True, False])
+def test_few_columns_share_the_inner_dimension(handle, d_type, transA):
+    """32-column tiles: two CTAs take half of K each when that evens out the work, one or several tiles a pair."""
+    for sizes, M, K in (([1], 130, 2048), ([1, 0, 2], 264, 1304), ([32, 5], 128, 264), ([1] * 20, 1024, 520), ([3] * 40, 512, 1032), ([1], 8, 192)):
+        run_grouped(handle, sizes, M, K, transA=transA, d_type=d_type, beta=0.5, c_type=F32)
+
+
+def test_long_sums_of_one_sign_keep_binary32(handle):
+    """A binary32 D sums several accumulators of 512 products, so that the tensor core's truncation does not grow
+    with K.  One instruction adds 16 products to the accumulator; what it drops is less than two units in the
+    last place of the sum so far: 32 instructions, 2 * 32 * 2^-23 of the sum of magnitudes, and 2^-24 for each of the
+    K / 512 additions.  One accumulator for K = 16384 is 1e-4 off on these values."""
+    r = np.random.default_rng(3)
+    K, M, N = 16384, 136, 136
+    A, B = store(np.abs(normal(r, (M, K), 2.0 ** -7)), F16), store(np.abs(normal(r, (N, K))), F16)
+    d = CuArray(np.zeros((M, N), F32, order="F"))
+    handle.gemm_grouped_k(M, N, K, 1.0, CuArray(A), M, CuArray(B), N, F16, 0.0, None, M, M * N, F32, d, M, M * N, F32, CuArray(offsets_of([K])), 1)
+    sync(handle)
+    exact = value(A, F16) @ value(B, F16).T
+    assert np.all(np.abs(Array(d) - exact) <= (2 * 32 * 2.0 ** -23 + K / 512 * 2.0 ** -24) * exact)
+    At, d2 = CuArray(np.asfortranarray(A.T)), CuArray(np.zeros((M, N), F32, order="F"))
+    handle.gemm_grouped(True, M, N, K, 1.0, At, K, M * K, CuArray(np.asfortranarray(B.T)), K, F16, 0.0, None, M, F32, d2, M, F32,
+                        CuArray(offsets_of([N])), 1)
+    sync(handle)
+    assert np.all(np.abs(Array(d2) - exact) <= (2 * 32 * 2.0 ** -23 + K / 512 * 2.0 ** -24) * exact)
+
+
+def test_same_call_twice_is_bitwise_the_same(handle):
+    r = np.random.default_rng(4)
+    off = CuArray(offsets_of([1, 0, 2, 7, 30]))
+    W, X = CuArray(store(normal(r, (1032, 5 * 264)), BFloat16)), CuArray(store(normal(r, (1032, 40)), BFloat16))
+    got = []
+    for _ in range(4):
+        d = CuArray(np.zeros((264, 40), F32, order="F"))
+        handle.gemm_grouped(True, 264, 40, 1032, 1.0, W, 1032, 1032 * 264, X, 1032, BFloat16, 0.0, None, 264, F32, d, 264, F32, off, 5)
+        sync(handle)
+        got.append(Array(d))
+    assert all(np.array_equal(g, got[0]) for g in got)
+
+
+def test_check_on_call_names_the_offsets(handle):
+    from cudanative_jl_b200 import B200Error
+
+    handle.set_option(_lib.OPT_CHECK_ON_CALL, 1)
+    a, d = CuArray(np.ones((64, 64), F16, order="F")), CuArray(np.zeros((64, 9), F32, order="F"))
+
+    def call(off):
+        handle.gemm_grouped(True, 64, 9, 64, 1.0, a, 64, 0, a, 64, F16, 0.0, None, 64, F32, d, 64, F32, CuArray(np.array(off, np.int32)), 2)
+        _lib.check(_lib.lib().b200_stream_sync(None), "sync")
+
+    call([0, 7, 3])
+    with pytest.raises(B200Error, match="group offsets") as e:
+        call([0, 3, 9])
+    assert e.value.status == _lib.INVALID_ARG
+    call([0, 3, 9])
+    assert np.all(Array(d) == 64.0)
+
+
+def test_streams_and_replayed_graphs():
+    """Sizes are read when the kernel runs: a captured layer follows new offsets and inputs.  Two captured layers on
+    one handle, replayed at once on two streams, share nothing."""
+    torch = pytest.importorskip("torch")
+    from cudanative_jl_b200.gemm import Handle, mxfp4_scale_bytes
+
+    torch.cuda.set_device(0)
+    E, M, K, T = 4, 264, 256, 300
+    with Handle(0) as h:
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        rand = lambda *s: torch.randn(s, generator=gen, device="cuda").bfloat16()  # noqa: E731
+
+        class Layer:
+            def __init__(self):
+                self.w, self.x, self.g = rand(E, M, K), rand(T, K), rand(T, M)
+                self.off = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+                self.y, self.dx = torch.zeros(T, M, device="cuda"), torch.zeros(T, K, device="cuda")
+                self.dw, self.y4 = torch.zeros(E, M, K, device="cuda"), torch.zeros(T, M, device="cuda")
+                u8 = lambda n: torch.zeros(n, dtype=torch.uint8, device="cuda")  # noqa: E731
+                self.qw, self.sw = u8(E * M * K // 2), u8(E * mxfp4_scale_bytes(K, M))
+                self.qx, self.sx = u8(T * K // 2), u8(mxfp4_scale_bytes(K, T, E))
+                self.woff = (torch.arange(E + 1, device="cuda") * M).int()
+
+            def run(self):
+                s = torch.cuda.current_stream().cuda_stream
+                p = lambda t: t.data_ptr()  # noqa: E731
+                h.gemm_grouped(True, M, T, K, 1.0, p(self.w), K, M * K, p(self.x), K, BFloat16, 0.0, None, M, F32, p(self.y), M, F32, p(self.off), E, stream=s)
+                h.gemm_grouped(False, K, T, M, 1.0, p(self.w), K, M * K, p(self.g), M, BFloat16, 0.0, None, K, F32, p(self.dx), K, F32, p(self.off), E,
+                               stream=s)
+                h.gemm_grouped_k(K, M, T, 1.0, p(self.x), K, p(self.g), M, BFloat16, 0.0, None, K, K * M, F32, p(self.dw), K, K * M, F32, p(self.off),
+                                 E, stream=s)
+                h.mxfp4_quantize(False, K, E * M, p(self.w), K, BFloat16, p(self.qw), K, p(self.sw), offsets=p(self.woff), groups=E, stream=s)
+                h.mxfp4_quantize(False, K, T, p(self.x), K, BFloat16, p(self.qx), K, p(self.sx), offsets=p(self.off), groups=E, stream=s)
+                h.gemm_mxfp4_grouped(M, T, K, 1.0, p(self.qw), K, M * K, p(self.sw), p(self.qx), K, p(self.sx), 0.0, None, M, F32, p(self.y4), M, F32,
+                                     p(self.off), E, stream=s)
+
+            def check(self):
+                from mxfp4_cases import quantize, values
+
+                o = self.off.tolist()
+                w, x, g = (t.double().cpu().numpy() for t in (self.w, self.x, self.g))
+                for e in range(E):
+                    s = slice(o[e], o[e + 1])
+                    for got, a, b, k in ((self.y, x[s], w[e].T, K), (self.dx, g[s], w[e], M)):
+                        close(got[s].double().cpu().numpy(), a @ b, np.abs(a) @ np.abs(b), k, F32)
+                    close(self.dw[e].double().cpu().numpy(), g[s].T @ x[s], np.abs(g[s]).T @ np.abs(x[s]), max(1, o[e + 1] - o[e]), F32)
+                    a, b = values(*quantize(x[s].T)).T if o[e + 1] > o[e] else np.zeros((0, K)), values(*quantize(w[e].T))
+                    close(self.y4[s].double().cpu().numpy(), a @ b, np.abs(a) @ np.abs(b), K, F32)
+
+        layers = [Layer(), Layer()]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        graphs = []
+        for layer, stream in zip(layers, streams):
+            layer.off.copy_(torch.tensor([0, 10, 10, 200, 300], dtype=torch.int32))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                layer.run()  # eagerly, on a stream of its own
+            torch.cuda.synchronize()
+            layer.check()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                layer.run()
+            graphs.append(graph)
+        for sizes in ([0, 0, 1, 2, 3], [0, 300, 300, 300, 300], [0, 75, 150, 225, 299]):
+            for layer, shift in zip(layers, (0, 1)):
+                layer.off.copy_(torch.tensor([min(v + shift, T) if v else 0 for v in sizes], dtype=torch.int32))
+                layer.x.copy_(rand(T, K))
+            torch.cuda.synchronize()
+            for _ in range(3):
+                for graph, stream in zip(graphs, streams):
+                    with torch.cuda.stream(stream):
+                        graph.replay()
+            torch.cuda.synchronize()
+            for layer in layers:
+                layer.check()
+        assert h.device_status()[0] == 0

@@ -237,3 +237,41 @@ def test_a_layer_of_experts_from_16_bit_tokens(handle):
     w, x = values(*quantize(value(W, BFloat16)))[:K], values(*quantize(value(X, BFloat16)))[:K]
     exact, S = grouped_ref([w[:, e * M:(e + 1) * M] for e in range(E)], x, None, off, 1.0, 0.0, True, np.zeros((M, T)))
     close(value(Array(d), BFloat16), exact, S, K, BFloat16)
+
+
+@pytest.mark.parametrize("max_ctas", [1, 2, 3, 10])
+@pytest.mark.parametrize("tile_n", [0, 128, 256])
+def test_few_ctas_walk_many_tiles(handle, max_ctas, tile_n):
+    """Every barrier goes through many phases, the ring wraps, accumulators change hands; 192-column tiles with a
+    short inner dimension or a C, 256 otherwise, 32 and split sums for few columns."""
+    handle.set_option(_lib.OPT_MAX_CTAS, max_ctas)
+    for K in (96, 544, 1056):
+        run_product(handle, 648, K, [3, 0, 70, 300, 1, 700], tile_n=tile_n)
+        run_product(handle, 392, K, [700], grouped=False, tile_n=tile_n, d_type=F32, beta=1.0)
+    handle.set_option(_lib.OPT_PDL, 0)
+    run_product(handle, 264, 1056, [1, 0, 2, 33], tile_n=tile_n)
+
+
+@pytest.mark.parametrize("d_type", [BFloat16, F32])
+def test_few_columns_share_the_inner_dimension(handle, d_type):
+    for sizes, M, K in (([1], 130, 8192), ([1, 0, 2], 264, 1312), ([32, 5, 40], 128, 1056), ([1] * 20, 1024, 1024), ([3] * 40, 512, 1056), ([1], 8, 768)):
+        run_product(handle, M, K, sizes, d_type=d_type, beta=0.5, c_type=F32)
+    for N in (1, 4, 5, 31, 32):
+        run_product(handle, 264, 2080, [N], grouped=False, d_type=d_type)
+
+
+def test_the_exponent_range_of_the_scales(handle):
+    """Products of the smallest and the largest scales: 2^-127 * 2^127 and beyond binary32 on either side."""
+    K, M, N = 64, 8, 4
+    qa, qb = np.full((K, M), 2, np.uint8), np.full((K, N), 2, np.uint8)  # elements 1.0
+    sa, sb = np.full((2, M), 127, np.uint8), np.full((2, N), 127, np.uint8)
+    sa[:, 0], sa[:, 1], sa[:, 2] = 0, 254, 100
+    sb[:, 0], sb[:, 1] = 254, 0
+    d = CuArray(np.zeros((M, N), F32, order="F"))
+    handle.gemm_mxfp4(M, N, K, 1.0, CuArray(pack(qa, K)), K, CuArray(tile(sa)), CuArray(pack(qb, K)), K, CuArray(tile(sb)), 0.0, None, M, F32, d, M, F32)
+    sync(handle)
+    got, exact = Array(d).astype(np.float64), K * np.ldexp(1.0, sa[0].astype(int) - 127)[:, None] * np.ldexp(1.0, sb[0].astype(int) - 127)[None]
+    normal = (exact >= 2.0 ** -126) & (exact < 2.0 ** 128)
+    assert np.array_equal(got[normal], exact[normal])
+    assert np.all(np.isinf(got[exact >= 2.0 ** 128]))
+    assert np.all(got[exact < 2.0 ** -126] <= 2.0 ** -120)
