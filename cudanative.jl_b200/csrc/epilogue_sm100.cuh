@@ -222,13 +222,19 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                     if (!ok) return;
                     const float* c = reinterpret_cast<const float*>(ring + b * E::BUF_BYTES) + et;
                     const unsigned short* ch = reinterpret_cast<const unsigned short*>(ring + b * E::BUF_BYTES) + et;
+                    float v[CW];
+                    if (p.c_fmt == 0) {
 #pragma unroll
-                    for (int i = 0; i < CW; ++i) {
-                        const float v = p.c_fmt == 0   ? c[i * 128]
-                                        : p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(ch[i * 128]) << 16)
-                                                       : __half2float(__ushort_as_half(ch[i * 128]));
-                        r[half * CW + i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[half * CW + i]), beta * v));
+                        for (int i = 0; i < CW; ++i) v[i] = c[i * 128];
+                    } else if (p.c_fmt == 2) {
+#pragma unroll
+                        for (int i = 0; i < CW; ++i) v[i] = __uint_as_float(static_cast<uint32_t>(ch[i * 128]) << 16);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < CW; ++i) v[i] = __half2float(__ushort_as_half(ch[i * 128]));
                     }
+#pragma unroll
+                    for (int i = 0; i < CW; ++i) r[half * CW + i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[half * CW + i]), beta * v[i]));
                     __syncwarp();
                     if (lane == 0) mbar_arrive(cempty + 8 * b);
                     ++c_count;
