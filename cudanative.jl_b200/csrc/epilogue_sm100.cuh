@@ -11,9 +11,10 @@
 // where the stores themselves take about 100; it also cost 48 KiB of the ring.  Any M, leading dimension and
 // alignment take the same path.
 //
-// C of a ragged-K product is as large as D and read once.  It comes by bulk copies into a ring of its own,
-// several chunks ahead, issued by a thread that does nothing else (c_producer); where its rows allow no
-// bulk copies, and for ragged N, it is read directly.
+// C is read the same way.  Where the registers allow it (kAhead) a step's C is asked for one step ahead, else the
+// warp brings the tile's lines of C into L2 before it waits for the accumulator.  (A ring of bulk copies for C took 48 KiB
+// of the stages' and was no faster: 2048 x 1408 x 32 groups, 16384 columns, C and D Float32 182 against 184 us, and
+// 138 against 132 us without a C.)
 //
 // kPromoteKb: the tensor core adds into its accumulator without rounding to nearest; every step drops what
 // lies below the last place, which pulls sums towards zero in proportion to the number of steps (measured
@@ -34,7 +35,6 @@ struct EpilogueParams {
     void* D;
     long long ldc, ldd, stride_c, stride_d;  // strides: one C and D per group (kPerGroup)
     int c_fmt, d_fmt;                        // 0 = binary32, 1 = binary16, 2 = bfloat16
-    int c_tma;                               // C comes by bulk copies (ragged K)
     int d_pairs;                             // two rows of a 16-bit D can be stored as one word
 };
 
@@ -54,69 +54,45 @@ struct SplitParams {
     uint32_t full_bar, empty_bar;
 };
 
-// kRing: chunks of C in flight per warp group; 0 where C is read directly.
-template <int kBN, int kRing, int kW = 32>
+template <int kBN>
 struct EpilogueCfg {
     static constexpr int COLS = kBN >= 64 ? kBN / 2 : kBN;  // per warp group; the second is idle below 64
-    static constexpr int W = kW;                            // columns per step
-    static constexpr int CW = 16;                           // columns per copy of C
-    static constexpr int RING = kRing;
-    static constexpr int BUF_BYTES = 128 * CW * 4;
-    static constexpr int BYTES = 2 * kRing * BUF_BYTES;
+    static constexpr int W = 32;                            // columns per step
     static_assert(COLS % W == 0, "steps");
 };
 
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(taddr, r); }
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(taddr, r); }
-
 __device__ __forceinline__ int columns_of(int tile_cols, int wg, int cols) { return min(cols, max(0, tile_cols - wg * cols)); }
 
-// ONE thread: asks for C's chunks in the order in which the two warp groups need them.
-template <class E, class Decode>
-__device__ __forceinline__ void c_producer(const EpilogueParams& p, const CUtensorMap* tmC, uint32_t ring, uint32_t cfull, uint32_t cempty,
-                                           const WaitCtx& wc, int unit_first, int unit_stride, int num_units, Decode decode) {
-    const uint32_t bytes = 128 * E::CW * (p.c_fmt ? 2 : 4);
-    const uint64_t once = l2_policy_evict_first();
-    uint32_t count[2] = {0, 0};
-    for (int unit = unit_first; unit < num_units; unit += unit_stride) {
-        const Unit u = decode(unit);
-        for (int j = 0; j * E::CW < min(u.cols, E::COLS); ++j) {
-#pragma unroll
-            for (int wg = 0; wg < 2; ++wg) {
-                if (j * E::CW >= columns_of(u.cols, wg, E::COLS)) continue;
-                const uint32_t b = wg * E::RING + count[wg] % E::RING;
-                if (!mbar_wait(cempty + 8 * b, ((count[wg] / E::RING) & 1u) ^ 1u, wc, kWaitCTile)) return;
-                mbar_arrive_expect_tx(cfull + 8 * b, bytes);
-                tma_load_3d_hint(ring + b * E::BUF_BYTES, tmC, u.m0, u.n0 + wg * E::COLS + j * E::CW, u.group, cfull + 8 * b, once);
-                ++count[wg];
-            }
-        }
-    }
-}
-
-// Warps 4 .. 11 (`wg` 0 or 1).  Barriers are 8 bytes apart: tmem_full / tmem_empty [kAccs]; cfull / cempty
-// [RING] of this warp group.
+// Warps 4 .. 11 (`wg` 0 or 1).  Barriers tmem_full / tmem_empty [kAccs] are 8 bytes apart.
 template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, bool kSplit, class Decode>
-__device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, uint32_t tmem_base, const uint8_t* ring, uint32_t tmem_full,
-                                             uint32_t tmem_empty, uint32_t cfull, uint32_t cempty, const WaitCtx& wc, int unit_first,
-                                             int unit_stride, int num_units, const SplitParams& split, Decode decode) {
-    constexpr int W = E::W, CW = E::CW, RING = E::RING > 0 ? E::RING : 1;
+__device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, uint32_t tmem_base, uint32_t tmem_full, uint32_t tmem_empty,
+                                             const WaitCtx& wc, int unit_first, int unit_stride, int num_units, const SplitParams& split,
+                                             Decode decode) {
+    constexpr int W = E::W;
     constexpr bool kDrain = kPromoteKb < 0;  // one accumulator: read it out at once so that the next tile may begin
-    constexpr bool kAhead = kPromoteKb == 0 && E::RING == 0;
+    constexpr bool kAhead = kPromoteKb == 0;
     const int et = static_cast<int>(threadIdx.x & 127);
     const int lane = static_cast<int>(threadIdx.x & 31);
     const uint32_t lane_base = static_cast<uint32_t>(((threadIdx.x >> 5) & 3) * 32) << 16;
     const bool has_c = p.beta != 0.0f;
-    const bool c_bulk = E::RING > 0 && has_c && p.c_tma;
     const float alpha = p.alpha, beta = p.beta;
     const int d_fmt = kF32 ? 0 : p.d_fmt;
     const int col0 = wg * E::COLS;
-    uint32_t acc_count = 0, split_count = 0, c_count = 0;
+    uint32_t acc_count = 0, split_count = 0;
     bool ok = true;
     const bool sends = kSplit && split.role == 1, receives = kSplit && split.role == 0;
     const uint32_t remote = kSplit ? mapa_shared(split.recv_addr + et * kSplitRow * 4, 0) : 0u;
     const uint32_t remote_bar = kSplit ? mapa_shared(split.full_bar, 0) : 0u;
     static_assert(!kSplit || (E::COLS == W && W == 32), "partial sums are one step of columns");
+
+    // this warp's lines of C of a tile into L2, a lane to a column
+    auto prefetch_c = [&](const Unit& u) {
+        const int bytes = p.c_fmt == 0 ? 4 : 2, row = u.m0 + (et & ~31), cols = columns_of(u.cols, wg, E::COLS);
+        for (int j = lane; j < cols; j += 32) {
+            const long long at = (kPerGroup ? u.group * p.stride_c : 0) + row + (u.n0 + col0 + j) * p.ldc;
+            if (row < p.M) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.C) + at * bytes));
+        }
+    };
 
     for (int unit = unit_first; unit < num_units; unit += unit_stride) {
         const Unit u = decode(unit);
@@ -196,15 +172,8 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                     c_next[i] = p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(raw[i]) << 16) : __half2float(__ushort_as_half(raw[i]));
             }
         };
-        if (kAhead && has_c && !c_bulk && !sends && cols > 0) load_c(0);
-        if (!kAhead && has_c && !c_bulk) {
-            // no registers to hold them: bring the warp's lines of C into L2 meanwhile, a lane to a column
-            const int bytes = p.c_fmt == 0 ? 4 : 2, row = u.m0 + (et & ~31);
-            for (int j = lane; j < cols; j += 32) {
-                const long long at = (kPerGroup ? u.group * p.stride_c : 0) + row + (u.n0 + col0 + j) * p.ldc;
-                if (row < p.M) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(p.C) + at * bytes));
-            }
-        }
+        if (kAhead && has_c && !sends && cols > 0) load_c(0);
+        if (!kAhead && has_c) prefetch_c(u);
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
             if constexpr (kSplit) {
@@ -212,34 +181,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 if (sends || !ok) return;
             }
             const int n = u.n0 + col0 + j * W, left = cols - j * W;
-            if (c_bulk) {
-#pragma unroll
-                for (int half = 0; half < W / CW; ++half) {
-                    if (half * CW >= left) break;
-                    const uint32_t b = c_count % RING;
-                    ok = mbar_wait(cfull + 8 * b, (c_count / RING) & 1u, wc, kWaitCTile);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return;
-                    const float* c = reinterpret_cast<const float*>(ring + b * E::BUF_BYTES) + et;
-                    const unsigned short* ch = reinterpret_cast<const unsigned short*>(ring + b * E::BUF_BYTES) + et;
-                    float v[CW];
-                    if (p.c_fmt == 0) {
-#pragma unroll
-                        for (int i = 0; i < CW; ++i) v[i] = c[i * 128];
-                    } else if (p.c_fmt == 2) {
-#pragma unroll
-                        for (int i = 0; i < CW; ++i) v[i] = __uint_as_float(static_cast<uint32_t>(ch[i * 128]) << 16);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < CW; ++i) v[i] = __half2float(__ushort_as_half(ch[i * 128]));
-                    }
-#pragma unroll
-                    for (int i = 0; i < CW; ++i) r[half * CW + i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[half * CW + i]), beta * v[i]));
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(cempty + 8 * b);
-                    ++c_count;
-                }
-            } else if (has_c) {
+            if (has_c) {
                 if (!kAhead) load_c(j);
 #pragma unroll
                 for (int i = 0; i < W; ++i) r[i] = __float_as_uint(fmaf(alpha, __uint_as_float(r[i]), beta * c_next[i]));
@@ -304,7 +246,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 for (int q = 0; q < E::COLS / W; ++q) {
                     if (q * W < cols) {
                         uint32_t r[W];
-                        tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + q * W, r);
+                        tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r);
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < W; ++i) sum[q * W + i] += __uint_as_float(r[i]);
@@ -328,7 +270,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             if (!ok) break;
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q)
-                if (q * W < cols) tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
+                if (q * W < cols) tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + q * W, r[q]);
             tmem_wait_ld();
             release(acc);
             ++acc_count;
@@ -343,7 +285,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             for (int j = 0; ok && j * W < cols; ++j) {
                 uint32_t r[W];
                 if (!empty) {
-                    tmem_ld_cols(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
+                    tmem_ld_32x32b_x32(tmem_base + lane_base + acc * kBN + col0 + j * W, r);
                     tmem_wait_ld();
                 } else {
 #pragma unroll

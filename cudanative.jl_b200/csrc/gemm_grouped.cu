@@ -135,7 +135,7 @@ struct Grouped {
 };
 
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
-int launch_promote(const CUtensorMap (&tm)[3], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
     constexpr bool kSplit = kBN == 32;  // few columns per group: pairs of CTAs that may share a tile's inner dimension
     using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
     auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote, kSplit>;
@@ -164,19 +164,19 @@ int launch_promote(const CUtensorMap (&tm)[3], const GroupedParams& p, int grid,
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], p));
+    B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], p));
     return B200_OK;
 }
 
 // binary32 results add several accumulators with rounding to nearest (epilogue_sm100.cuh)
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
-int launch_grouped(const CUtensorMap (&tm)[3], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch_grouped(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
     if (p.e.d_fmt == 0) return launch_promote<kBN, kAMn, kRaggedK, kCtas, true>(tm, p, grid, stream, pdl);
     return launch_promote<kBN, kAMn, kRaggedK, kCtas, false>(tm, p, grid, stream, pdl);
 }
 
 template <int kBN, int kCtas>
-int launch_kind(const Grouped& g, const CUtensorMap (&tm)[3], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+int launch_kind(const Grouped& g, const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
     if (g.ragged_k) {
         if constexpr ((kBN / kCtas) % 64 == 0) return launch_grouped<kBN, true, true, kCtas>(tm, p, grid, stream, pdl);
         else return fail(B200_UNSUPPORTED, "grouped_k: 64 tile columns per CTA at least");
@@ -243,7 +243,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
 
     const int bn_local = tile_n / pair, bbox = std::min(bn_local, 64);
     const CUtensorMapDataType dt = map_type(g.ab_type);
-    CUtensorMap tm[3];
+    CUtensorMap tm[2];
     if (g.ragged_k) {
         if ((rc = encode_map_2d(&tm[0], dt, 2, g.A, g.M, g.K, g.lda, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "A"))) return rc;
         if ((rc = encode_map_2d(&tm[1], dt, 2, g.B, g.N, g.K, g.ldb, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
@@ -256,19 +256,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
         if (rc) return rc;
         if ((rc = encode_map_2d(&tm[1], dt, 2, g.B, g.K, g.N, g.ldb, 64, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
     }
-    // C of a ragged-K product by bulk copies: whole 16-byte chunks of rows, matrices that do not overlap
-    const int cq = 16 / elem_bytes(g.c_type);
-    p.e.c_tma = g.ragged_k && g.beta != 0.0f && !(reinterpret_cast<uintptr_t>(g.C) & 15u) && g.ldc % cq == 0 &&
-                (g.groups == 1 || (g.stride_c % cq == 0 && g.stride_c >= g.ldc * g.N));
     p.e.d_pairs = !(reinterpret_cast<uintptr_t>(g.D) & 3u) && g.ldd % 2 == 0 && g.stride_d % 2 == 0;
-    tm[2] = tm[0];  // not used unless replaced
-    if (p.e.c_tma) {
-        BatchDim b;
-        b.count = g.groups;
-        b.stride = g.groups > 1 ? g.stride_c : g.ldc * g.N;
-        if ((rc = encode_map_2d(&tm[2], map_type(g.c_type), elem_bytes(g.c_type), g.C, g.M, g.N, g.ldc, 128, 16, CU_TENSOR_MAP_SWIZZLE_NONE, "C", b)))
-            return rc;
-    }
 
     // ragged N: at most one partial tile column per group that has columns
     const int64_t cols = g.ragged_k ? g.groups * p.tiles_n : g.N / tile_n + std::min<int64_t>(g.groups, g.N);

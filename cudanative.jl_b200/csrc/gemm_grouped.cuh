@@ -57,15 +57,15 @@ struct GroupedCfg {
     static constexpr int BBOX_BYTES = BBOX * BK * 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;        // of the instruction's N
     static constexpr int PROMOTE_KB = 8;                        // k-blocks per accumulator of a binary32 D
-    using Epi = EpilogueCfg<kBN, kRaggedK ? 3 : 0>;
+    using Epi = EpilogueCfg<kBN>;
     static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
     static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int TMEM_COLS = 2 * kBN < 32 ? 32 : 2 * kBN;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
-    static constexpr int NBARS = 4 * STAGES + 6 + 4 * Epi::RING;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int NBARS = 4 * STAGES + 6;
     static_assert(!kSplit || (kCtas == 1 && !kRaggedK && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
@@ -147,7 +147,7 @@ __device__ __forceinline__ int find_group(const int* first, int groups, int q) {
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, bool kSplit>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const __grid_constant__ CUtensorMap tmC, const GroupedParams p) {
+                     const GroupedParams p) {
     using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
     constexpr int STAGES = Cfg::STAGES;
     using Epi = typename Cfg::Epi;
@@ -158,10 +158,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES + Epi::BYTES;
+    constexpr int kRecvAt = STAGES * Cfg::STAGE_BYTES;
     constexpr int kTableAt = kRecvAt + Cfg::RECV_BYTES;
     const uint32_t bar_base = smem_base + kTableAt + Cfg::TABLE_BYTES;
-    uint8_t* ring_gen = smem_gen + STAGES * Cfg::STAGE_BYTES;
     int* off = reinterpret_cast<int*>(smem_gen + kTableAt);
     int* first = off + kMaxGroups + 4;
     uint8_t* bar_gen = smem_gen + kTableAt + Cfg::TABLE_BYTES;
@@ -173,7 +172,6 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     auto tmem_full_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
     auto tmem_empty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + 2 + a); };
     auto split_bar = [&](int i) { return bar_base + 8u * (4 * STAGES + 4 + i); };  // partial sums: full, empty
-    auto cfull_bar = [&](int b) { return bar_base + 8u * (4 * STAGES + 6 + b); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * Cfg::NBARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 8 * Cfg::NBARS + 4);
 
@@ -198,14 +196,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         mbar_init(split_bar(0), 1);  // the receiver's arrive; it expects the sender's bytes
         mbar_init(split_bar(1), 4);  // the receiver's four warps
-        for (int b = 0; b < 2 * Epi::RING; ++b) {
-            mbar_init(cfull_bar(b), 1);
-            mbar_init(cfull_bar(2 * Epi::RING + b), 4);  // free again: the warp group's four warps
-        }
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
-        tma_prefetch_desc(&tmC);
     }
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     tc_fence_before_sync();
@@ -452,20 +445,12 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             s = (s + kb1) % STAGES;
         }
         __syncwarp();
-    } else if (kRaggedK && warp == 2) {
-        if constexpr (kRaggedK) {
-            if (lane == 0 && p.e.beta != 0.0f && p.e.c_tma)
-                c_producer<Epi>(p.e, &tmC, smem_base + STAGES * Cfg::STAGE_BYTES, cfull_bar(0), cfull_bar(2 * Epi::RING), wc, unit_first,
-                                unit_stride, num_units, decode);
-        }
-        __syncwarp();
     }
     } else {
         regs_inc<224>();
         const int wg = (warp - 4) >> 2;
         run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
-            p.e, wg, tmem_base, ring_gen + wg * Epi::RING * Epi::BUF_BYTES, tmem_full_bar(0), tmem_empty_bar(0), cfull_bar(wg * Epi::RING),
-            cfull_bar((2 + wg) * Epi::RING), wc, unit_first, unit_stride, num_units, split, decode);
+            p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit

@@ -57,11 +57,11 @@ struct MxCfg {
     static constexpr int BBOX = BN_LOCAL < 128 ? BN_LOCAL : 128;
     static constexpr int BBOX_BYTES = BBOX * BK / 2;
     static constexpr int GRANULE = kCtas == 2 ? 32 : 16;
-    using Epi = EpilogueCfg<kBN, 0>;
+    using Epi = EpilogueCfg<kBN>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
     static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
-    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - Epi::BYTES - RECV_BYTES;
+    static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - RECV_BYTES;
     static constexpr int ACCS = kBN <= 192 ? 2 : 1;
     static constexpr int SCALE_COLS = 8 * (1 + B_TILES);  // per set: 2 x 4 for A, 2 x 4 per scale tile for B
     static constexpr int SCALE_AT = ACCS * kBN;
@@ -69,7 +69,7 @@ struct MxCfg {
     static constexpr int STAGES = BUDGET / STAGE_BYTES > MOST ? MOST : BUDGET / STAGE_BYTES;
     static constexpr int USED_COLS = SCALE_AT + STAGES * SCALE_COLS;
     static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + Epi::BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
     static constexpr int NBARS = 3 * STAGES + 2 + 2 * ACCS;
     static_assert(!kSplit || (kCtas == 1 && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(USED_COLS <= 512, "tensor memory");
@@ -356,7 +356,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         regs_inc<200>();
         const int wg = (warp - 4) >> 2;
         run_epilogue<Epi, kBN, ACCS, kCtas, false, ACCS == 1 ? -1 : 0, false, kSplit>(
-            p.e, wg, tmem_base, nullptr, tmem_full_bar(0), tmem_empty_bar(0), 0, 0, wc, unit_first, unit_stride, num_units, split, decode);
+            p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 
     // ---------------------------------------------------------------------- common exit
