@@ -48,7 +48,9 @@ class DevicePtr:
                 raise TypeError("expected a CUDA tensor")
             import torch
 
-            table = {torch.float16: np.float16, torch.float32: np.float32}
+            # bfloat16 as bit patterns (bfloat16.py); bytes and offsets of the 4-bit and grouped products
+            table = {torch.float16: np.float16, torch.float32: np.float32, torch.bfloat16: np.uint16, torch.uint8: np.uint8,
+                     torch.int32: np.int32}
             if obj.dtype not in table:
                 raise TypeError(f"unsupported tensor dtype {obj.dtype}")
             return DevicePtr(table[obj.dtype], obj.data_ptr(), obj)

@@ -206,6 +206,83 @@ function gemm_strided_batched!(h::Handle, D, A, B, C = nothing; batch = 1, ab_ty
                 C === nothing ? 0 : C.stride, c_type, D.ptr, D.ld, D.stride, d_type, batch))
 end
 
+"""
+    gemm_grouped!(h, D, A, B, C; offsets, ab_type, c_type, d_type, alpha, beta, transA, stream)
+
+`D[:, s_e] = alpha * op(A_e) * B[:, s_e] + beta * C[:, s_e]` for groups of columns whose borders `offsets` (Int32, one
+more than there are groups, 0-based) live on the device (b200_gemm_grouped): a layer with one weight matrix per
+group, or the gradient of its input.  `A` is (ptr, rows, cols, ld, stride), `offsets` (ptr, groups); `stride = 0`
+is one matrix for all groups.
+"""
+function gemm_grouped!(h::Handle, D, A, B, C = nothing; offsets, ab_type = ELEM_BF16, c_type = ELEM_F32, d_type = ELEM_BF16,
+                       alpha = 1f0, beta = 0f0, transA = true, stream::CuStream = CuDefaultStream())
+    M, K = transA ? (A.cols, A.rows) : (A.rows, A.cols)
+    check(ccall((:b200_gemm_grouped, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Cint, Int64, Int64, Int64, Cfloat, CuPtr{Cvoid}, Int64, Int64, CuPtr{Cvoid}, Int64, Cint, Cfloat,
+                 CuPtr{Cvoid}, Int64, Cint, CuPtr{Cvoid}, Int64, Cint, CuPtr{Int32}, Int64),
+                h.ptr, stream.handle, transA, M, B.cols, K, alpha, A.ptr, A.ld, A.stride, B.ptr, B.ld, ab_type, beta,
+                C === nothing ? CuPtr{Cvoid}(0) : C.ptr, C === nothing ? M : C.ld, c_type, D.ptr, D.ld, d_type, offsets.ptr,
+                offsets.groups))
+end
+
+"""
+    gemm_grouped_k!(h, D, A, B, C; offsets, ab_type, c_type, d_type, alpha, beta, stream)
+
+`D_e = alpha * A[:, s_e] * B[:, s_e]' + beta * C_e` (b200_gemm_grouped_k), the gradient of the groups' matrices.  `D` and
+`C` are (ptr, ld, stride).
+"""
+function gemm_grouped_k!(h::Handle, D, A, B, C = nothing; offsets, ab_type = ELEM_BF16, c_type = ELEM_F32, d_type = ELEM_F32,
+                         alpha = 1f0, beta = 0f0, stream::CuStream = CuDefaultStream())
+    check(ccall((:b200_gemm_grouped_k, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Cfloat, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Int64, Cint, Cfloat, CuPtr{Cvoid},
+                 Int64, Int64, Cint, CuPtr{Cvoid}, Int64, Int64, Cint, CuPtr{Int32}, Int64),
+                h.ptr, stream.handle, A.rows, B.rows, A.cols, alpha, A.ptr, A.ld, B.ptr, B.ld, ab_type, beta,
+                C === nothing ? CuPtr{Cvoid}(0) : C.ptr, C === nothing ? A.rows : C.ld, C === nothing ? 0 : C.stride, c_type,
+                D.ptr, D.ld, D.stride, d_type, offsets.ptr, offsets.groups))
+end
+
+# ---- microscaled 4-bit operands: elements (two to a byte) and scales, laid out as include/b200wmma.h says ----------
+"Bytes that the scales of a K x cols 4-bit matrix take (b200_mxfp4_scale_bytes)."
+mxfp4_scale_bytes(K, cols, groups = 0) = ccall((:b200_mxfp4_scale_bytes, lib), Int64, (Int64, Int64, Int64), K, cols, groups)
+
+const NO_GROUPS = (ptr = CuPtr{Int32}(0), groups = 0)
+
+"Quantise the K x cols matrix X, or the transpose of a cols x K one (b200_mxfp4_quantize); Q is (ptr, ld, scales)."
+function mxfp4_quantize!(h::Handle, Q, X; trans = false, x_type = ELEM_BF16, offsets = NO_GROUPS, stream::CuStream = CuDefaultStream())
+    K, cols = trans ? (X.cols, X.rows) : (X.rows, X.cols)
+    check(ccall((:b200_mxfp4_quantize, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Cint, Int64, Int64, CuPtr{Cvoid}, Int64, Cint, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, CuPtr{Int32}, Int64),
+                h.ptr, stream.handle, trans, K, cols, X.ptr, X.ld, x_type, Q.ptr, Q.ld, Q.scales, offsets.ptr, offsets.groups))
+end
+
+"The values that a 4-bit matrix stands for (b200_mxfp4_dequantize)."
+function mxfp4_dequantize!(h::Handle, Y, Q; y_type = ELEM_BF16, offsets = NO_GROUPS, stream::CuStream = CuDefaultStream())
+    check(ccall((:b200_mxfp4_dequantize, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, CuPtr{Cvoid}, Int64, Cint, CuPtr{Int32}, Int64),
+                h.ptr, stream.handle, Y.rows, Y.cols, Q.ptr, Q.ld, Q.scales, Y.ptr, Y.ld, y_type, offsets.ptr, offsets.groups))
+end
+
+"`D = alpha * A' * B + beta * C` with 4-bit A (K x M) and B (K x N), given as (ptr, ld, scales) (b200_gemm_mxfp4)."
+function gemm_mxfp4!(h::Handle, D, A, B, C = nothing; M, N, K, c_type = ELEM_F32, d_type = ELEM_BF16, alpha = 1f0, beta = 0f0,
+                     stream::CuStream = CuDefaultStream())
+    check(ccall((:b200_gemm_mxfp4, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Cfloat, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, CuPtr{Cvoid}, Int64, CuPtr{Cvoid}, Cfloat,
+                 CuPtr{Cvoid}, Int64, Cint, CuPtr{Cvoid}, Int64, Cint),
+                h.ptr, stream.handle, M, N, K, alpha, A.ptr, A.ld, A.scales, B.ptr, B.ld, B.scales, beta,
+                C === nothing ? CuPtr{Cvoid}(0) : C.ptr, C === nothing ? M : C.ld, c_type, D.ptr, D.ld, d_type))
+end
+
+"`gemm_grouped!` with 4-bit operands (b200_gemm_mxfp4_grouped); A is (ptr, ld, stride, scales)."
+function gemm_mxfp4_grouped!(h::Handle, D, A, B, C = nothing; M, N, K, offsets, c_type = ELEM_F32, d_type = ELEM_BF16, alpha = 1f0,
+                             beta = 0f0, stream::CuStream = CuDefaultStream())
+    check(ccall((:b200_gemm_mxfp4_grouped, lib), Cint,
+                (Ptr{Cvoid}, Ptr{Cvoid}, Int64, Int64, Int64, Cfloat, CuPtr{Cvoid}, Int64, Int64, CuPtr{Cvoid}, CuPtr{Cvoid}, Int64,
+                 CuPtr{Cvoid}, Cfloat, CuPtr{Cvoid}, Int64, Cint, CuPtr{Cvoid}, Int64, Cint, CuPtr{Int32}, Int64),
+                h.ptr, stream.handle, M, N, K, alpha, A.ptr, A.ld, A.stride, A.scales, B.ptr, B.ld, B.scales, beta,
+                C === nothing ? CuPtr{Cvoid}(0) : C.ptr, C === nothing ? M : C.ld, c_type, D.ptr, D.ld, d_type, offsets.ptr,
+                offsets.groups))
+end
+
 "Host-buffer form: `Array`s in, `Array` out, copies inside (b200_gemm_f16f32_host)."
 function gemm_host!(h::Handle, D::Matrix{Float32}, A::Matrix{Float16}, B::Matrix{Float16},
                     C::Union{Matrix{Float32}, Nothing} = nothing; alpha = 1f0, beta = 0f0, transA = false, transB = false)

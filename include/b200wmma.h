@@ -38,8 +38,8 @@ enum {
 enum { B200_COL_MAJOR = 0, B200_ROW_MAJOR = 1 };
 
 /* Element tags: Float16 / Float32, the two WMMA element types (src/device/cuda/wmma.jl:11-37).
- * B200_BF16 (bfloat16) has no counterpart in the reference; only b200_gemm_ex and
- * b200_gemm_strided_batched accept it. */
+ * B200_BF16 (bfloat16) has no counterpart in the reference; b200_gemm_ex, b200_gemm_strided_batched and
+ * the grouped and 4-bit entry points accept it. */
 enum { B200_F16 = 0, B200_F32 = 1, B200_BF16 = 2 };
 
 /* Fragment use: WMMA.MatrixA / MatrixB / Accumulator (src/device/cuda/wmma.jl:343-346). */
@@ -203,12 +203,14 @@ int b200_gemm_strided_batched(b200_handle* h, b200_stream stream, int transA, in
  *   offsets: groups + 1 ascending 32-bit integers in DEVICE memory with 0 <= offsets[0] and
  *   offsets[groups] <= N; equal neighbours are an empty group.  Read by the kernel, never by the host.
  *   Columns that belong to no group are not written.  Offsets that decrease or leave [0, N] write
- *   nothing and put id 110 into the device status word (b200_device_status).
+ *   nothing and put id 110 into the device status word (b200_device_status; with
+ *   B200_OPT_CHECK_ON_CALL the next call returns B200_INVALID_ARG).
  *   groups <= 1024.  Types as in b200_gemm_ex; a column's result does not depend on its neighbours'
  *   values.  D may alias C exactly (same pointer, ld and type).
  * The tcgen05 kernel needs 16-byte aligned A and B, lda, ldb and stride_a multiples of 8 elements and
  * stride_a at least one matrix (or 0); anything else runs on the simple kernel.  C and D may have any
- * alignment.  The split-K option is ignored. */
+ * alignment.  A binary32 D on the tcgen05 kernel sums several accumulators, each of 512 products, with
+ * rounding to nearest.  The split-K option is ignored. */
 int b200_gemm_grouped(b200_handle* h, b200_stream stream, int transA, int64_t M, int64_t N, int64_t K,
                       float alpha, const void* A, int64_t lda, int64_t stride_a, const void* B,
                       int64_t ldb, int ab_type, float beta, const void* C, int64_t ldc, int c_type,
@@ -259,9 +261,10 @@ int b200_mxfp4_dequantize(b200_handle* h, b200_stream stream, int64_t K, int64_t
 /* D = alpha * A^T * B + beta * C with 4-bit A (K x M) and B (K x N), both laid out as above; C and D are
  * M x N column-major in any of the three types and at any alignment.  One weight matrix [out, in] and
  * tokens [tokens, in], stored row by row and quantised with trans = 0, give [tokens, out].  lda and ldb
- * count elements.  Products and sums of a block are exact in the tensor core's wider adder; accumulation
- * is binary32.  A block with scale 255 makes its row or column of D NaN.  K > 0 unless M or N is 0.  There
- * is no simple kernel for 4-bit operands: alignment that the layout above rules out is refused. */
+ * count elements.  Products are exact, accumulation is binary32.  A block with scale 255 makes its row or
+ * column of D NaN.  K > 0 unless M or N is 0.  D may alias C exactly (same pointer, ld and type).  There is
+ * no simple kernel for 4-bit operands: alignment that the layout above rules out is refused.  The tile
+ * options accept 128 and 256 columns (64 counts as 128); the split-K option is ignored. */
 int b200_gemm_mxfp4(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha,
                     const void* A, int64_t lda, const void* a_scales, const void* B, int64_t ldb,
                     const void* b_scales, float beta, const void* C, int64_t ldc, int c_type, void* D,

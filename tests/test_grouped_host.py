@@ -90,3 +90,12 @@ def test_gradients_of_the_statement():
             up[i] += h
             down[i] -= h
             assert abs((f(up) - f(down)) / (2 * h) - g[i]) < 1e-6
+
+
+def test_every_new_entry_point_has_a_julia_wrapper():
+    from test_binding_signatures import julia_ccalls
+
+    seen = {name for name, *_ in julia_ccalls()}
+    for name in ("b200_gemm_grouped", "b200_gemm_grouped_k", "b200_mxfp4_scale_bytes", "b200_mxfp4_quantize", "b200_mxfp4_dequantize",
+                 "b200_gemm_mxfp4", "b200_gemm_mxfp4_grouped"):
+        assert name in seen
