@@ -375,39 +375,58 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 // 16-row steps of the last k-block; whether it has to be padded with zeros first
                 const int last_steps = min(Cfg::BK / 16, (u.k_len - (u.kb0 + kb_total - 1) * Cfg::BK + 15) / 16);
                 const bool tail = needs_tail(u);
-                for (int kb = 0; kb < kb_total; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    const uint32_t acc = ucount & 1u;
-                    const bool last = kb + 1 == kb_total;
-                    const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
-                    const bool end = last || (kPromote && (kb + 1) % Cfg::PROMOTE_KB == 0);
-                    if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
-                    if (ok && !ready) ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage));
-                    if (ok && last && tail) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(s), (tail_ph >> s) & 1u, wc, kWaitTail));
-                        tail_ph ^= 1u << s;
-                    }
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    // look at the next stage now: the answer arrives while this one's products are issued
-                    const int s1 = s + 1 == STAGES ? 0 : s + 1;
-                    const bool next = mbar_test(full_bar(s1), ph ^ (s1 == 0));
+                auto products = [&](int st, uint32_t acc, bool first, int steps) {
                     const uint32_t d_tmem = tmem_base + acc * kBN;
-                    const uint64_t da = da0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const uint64_t db = db0 + static_cast<uint64_t>(s * (Cfg::STAGE_BYTES >> 4));
-                    const int steps = last ? last_steps : Cfg::BK / 16;
+                    const uint64_t da = da0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
+                    const uint64_t db = db0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
 #pragma unroll
                     for (int k = 0; k < Cfg::BK / 16; ++k)
-                        if (k < steps) umma_f16_warp<kCtas>(lead, d_tmem, da + k * kStepA, db + k * kStepB, idesc, (begin && k == 0) ? 0u : 1u);
+                        if (k < steps) umma_f16_warp<kCtas>(lead, d_tmem, da + k * kStepA, db + k * kStepB, idesc, (first && k == 0) ? 0u : 1u);
                     if (lead) {
-                        if constexpr (kPair) umma_commit_pair(empty_bar(s));
-                        else umma_commit<kCtas>(empty_bar(s));
-                        if (end) {
-                            if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                            else umma_commit<kCtas>(tmem_full_bar(acc));
-                        }
+                        if constexpr (kPair) umma_commit_pair(empty_bar(st));
+                        else umma_commit<kCtas>(empty_bar(st));
+                    }
+                };
+                auto wait_tail = [&](int st) {  // the last k-block's foreign rows are zero
+                    const bool done = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail));
+                    tail_ph ^= 1u << st;
+                    return done;
+                };
+                // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products.
+                static_assert(Cfg::PROMOTE_KB % 2 == 0, "an accumulator begins and ends with a turn");
+                for (int kb = 0; kb < kb_total; kb += 2) {
+                    const uint32_t acc = ucount & 1u;
+                    const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
+                    const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
+                    const bool two = kb + 1 < kb_total, last = kb + 2 >= kb_total;
+                    const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
+                    const bool end = last || (kPromote && (kb + 2) % Cfg::PROMOTE_KB == 0);
+                    if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    if (ok && !ready)
+                        ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
+                                                         (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
+                    if (ok && last && tail) ok = wait_tail(two ? s1 : s);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    if (two) {
+                        // look at the next two now: the answer arrives while these two's products are issued
+                        const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
+                        products(s, acc, begin, Cfg::BK / 16);
+                        products(s1, acc, false, last ? last_steps : Cfg::BK / 16);
+                        ready = __all_sync(0xffffffffu, next);
+                        s = s2;
+                        ph = ph2;
+                    } else {
+                        products(s, acc, begin, last_steps);
+                        ready = false;
+                        s = s1;
+                        ph = ph1;
+                    }
+                    if (lead && end) {
+                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                        else umma_commit<kCtas>(tmem_full_bar(acc));
                     }
                     ucount += end ? 1u : 0u;
-                    ready = __all_sync(0xffffffffu, next);
                 }
             }
         }
