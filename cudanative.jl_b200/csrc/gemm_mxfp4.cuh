@@ -10,8 +10,8 @@
 // and 128 values of k, brought by bulk copies of its own.  The products read scales from tensor memory, the
 // same 32 lanes repeated in each warp's quarter: four more warps (12 - 15) carry them there, one quarter each,
 // a set of columns per stage.  (tcgen05.cp does the same from the MMA issuer's thread, but holds up the
-// products behind it by about 80 cycles a tile, six tiles to 512 cycles of products: 8192^3 took 370 us
-// instead of 224 us without it; issued one stage ahead 437 us.)
+// products behind it by about 80 cycles a tile, six tiles to 512 cycles of products: 8192^3 took 370 us,
+// 437 us with the copies issued one stage ahead, and 266 us with the four warps.)
 //
 // A tile's scales always come from whole tiles of 128 columns, counted from the group's first column, as
 // they were quantised.  A tile of 32 columns may begin at row 32, 64 or 96 of one: the warps that carry its

@@ -448,3 +448,83 @@ def test_streams_and_replayed_graphs():
             for layer in layers:
                 layer.check()
         assert h.device_status()[0] == 0
+
+
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+def test_results_on_any_element_border(handle, d_type):
+    """D and C begin one element behind a 16-byte border, their leading dimension is odd: still the tcgen05 kernel."""
+    r = np.random.default_rng(8)
+    M, K, N, ldd = 264, 136, 70, 267
+    off = offsets_of([5, 0, 40, 25])
+    A, B, Cm = store(normal(r, (K, 4 * M)), BFloat16), store(normal(r, (K, N)), BFloat16), store(normal(r, (M, N)), d_type)
+    sentinel = fill_of(d_type, -7.25)
+
+    def behind(x):
+        return CuArray(np.concatenate([[sentinel], taller(x, ldd, sentinel).ravel("F")]))
+
+    c, d, da, ba = behind(Cm), behind(np.full((M, N), sentinel)), CuArray(A), CuArray(B)
+    handle.gemm_grouped(True, M, N, K, 1.0, da, K, K * M, ba, K, BFloat16, 1.0, pointer(c) + 1, ldd, d_type, pointer(d) + 1, ldd, d_type, CuArray(off), 4)
+    sync(handle)
+    assert handle.last_launch()["kernel"] == _lib.KERNEL_TCGEN05
+    raw = value(Array(d), d_type)
+    got = raw[1:].reshape(ldd, N, order="F")
+    assert raw[0] == -7.25 and np.all(got[M:] == -7.25)
+    a64 = [value(A[:, e * M:(e + 1) * M], BFloat16) for e in range(4)]
+    close(got[:M], *grouped_ref(a64, value(B, BFloat16), value(Cm, d_type), off, 1.0, 1.0, True, np.zeros((M, N))), K, d_type)
+    # the other ragged dimension: matrices an odd number of elements apart
+    X, Y = store(normal(r, (M, 70)), BFloat16), store(normal(r, (40, 70)), BFloat16)
+    d2 = CuArray(np.full(1 + 4 * (ldd * 40 + 1), sentinel))
+    handle.gemm_grouped_k(M, 40, 70, 1.0, CuArray(X), M, CuArray(Y), 40, BFloat16, 0.0, None, M, 0, F32, pointer(d2) + 1, ldd, ldd * 40 + 1, d_type,
+                          CuArray(off), 4)
+    sync(handle)
+    assert handle.last_launch()["kernel"] == _lib.KERNEL_TCGEN05
+    raw = value(Array(d2), d_type)
+    exact, S = grouped_k_ref(value(X, BFloat16), value(Y, BFloat16), None, off, 1.0, 0.0)
+    for e in range(4):
+        at = 1 + e * (ldd * 40 + 1)
+        got = raw[at:at + ldd * 40].reshape(ldd, 40, order="F")
+        close(got[:M], exact[e], S[e], 40, d_type)
+        assert np.all(got[M:] == -7.25) and raw[at - 1] == -7.25
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Kernels are loaded and opted in to their shared memory by whichever call comes first, a captured one too."""
+    pytest.importorskip("torch")
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import torch, numpy as np, __graft_entry__ as e
+e.load_package()
+from cudanative_jl_b200.gemm import Handle, mxfp4_scale_bytes
+from cudanative_jl_b200.bfloat16 import BFloat16
+h = Handle(0)
+x, w = torch.randn(64, 256, device="cuda").bfloat16(), torch.randn(2, 136, 256, device="cuda").bfloat16()
+off = torch.tensor([0, 20, 64], dtype=torch.int32, device="cuda")
+y, dw = torch.zeros(64, 136, device="cuda"), torch.zeros(2, 136, 256, device="cuda")
+q, s = torch.zeros(64, 128, dtype=torch.uint8, device="cuda"), torch.zeros(mxfp4_scale_bytes(256, 64), dtype=torch.uint8, device="cuda")
+z, v = torch.zeros(64, 64, device="cuda"), torch.zeros(64, 256, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    h.gemm_grouped(True, 136, 64, 256, 1.0, w, 256, 136 * 256, x, 256, BFloat16, 0.0, None, 136, np.float32, y, 136, np.float32, off, 2, stream=st)
+    h.gemm_grouped_k(256, 136, 64, 1.0, x, 256, y.bfloat16(), 136, BFloat16, 0.0, None, 256, 0, np.float32, dw, 256, 136 * 256, np.float32, off, 2, stream=st)
+    h.mxfp4_quantize(False, 256, 64, x, 256, BFloat16, q, 256, s, stream=st)
+    h.mxfp4_dequantize(256, 64, q, 256, s, v, 256, np.float32, stream=st)
+    h.gemm_mxfp4(64, 64, 256, 1.0, q, 256, s, q, 256, s, 0.0, None, 64, np.float32, z, 64, np.float32, stream=st)
+g.replay()
+torch.cuda.synchronize()
+ref = torch.cat([x[:20].double() @ w[0].double().T, x[20:].double() @ w[1].double().T])
+assert (y.double() - ref).norm() < 1e-5 * ref.norm()
+yb = y.bfloat16().double()
+ref = torch.stack([yb[:20].T @ x[:20].double(), yb[20:].T @ x[20:].double()])
+assert (dw.double() - ref).norm() < 1e-5 * ref.norm()
+assert torch.equal(z.double(), v.double() @ v.double().T) or (z.double() - v.double() @ v.double().T).norm() < 1e-5 * z.norm()
+assert h.device_status()[0] == 0
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
