@@ -11,10 +11,11 @@
 // where the stores themselves take about 100; it also cost 48 KiB of the ring.  Any M, leading dimension and
 // alignment take the same path.
 //
-// C is read the same way.  Where the registers allow it (kAhead) a step's C is asked for one step ahead, else the
-// warp brings the tile's lines of C into L2 before it waits for the accumulator.  (A ring of bulk copies for C took 48 KiB
-// of the stages' and was no faster: 2048 x 1408 x 32 groups, 16384 columns, C and D Float32 182 against 184 us, and
-// 138 against 132 us without a C.)
+// C is read the same way: before it waits for the accumulator the warp brings the tile's lines of C into L2 and
+// asks for the first step's values, then for each next step's while one is stored (where the registers
+// allow it, kAhead).  32 groups of 2048 x 1408, 16384 columns, C and D Float32: 169 us; 184 us without the values
+// ahead, 203 us without the lines, 215 us with the lines of the next tile instead, 182 us with a ring of bulk copies of C
+// in shared memory, which took 48 KiB from the stages (132 against 138 us without a C).
 //
 // kPromoteKb: the tensor core adds into its accumulator without rounding to nearest; every step drops what
 // lies below the last place, which pulls sums towards zero in proportion to the number of steps (measured
@@ -70,7 +71,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                                              Decode decode) {
     constexpr int W = E::W;
     constexpr bool kDrain = kPromoteKb < 0;  // one accumulator: read it out at once so that the next tile may begin
-    constexpr bool kAhead = kPromoteKb == 0;
+    constexpr bool kAhead = !kDrain;
     const int et = static_cast<int>(threadIdx.x & 127);
     const int lane = static_cast<int>(threadIdx.x & 31);
     const uint32_t lane_base = static_cast<uint32_t>(((threadIdx.x >> 5) & 3) * 32) << 16;
@@ -172,8 +173,9 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                     c_next[i] = p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(raw[i]) << 16) : __half2float(__ushort_as_half(raw[i]));
             }
         };
+        if (has_c && !sends) prefetch_c(u);
         if (kAhead && has_c && !sends && cols > 0) load_c(0);
-        if (!kAhead && has_c) prefetch_c(u);
+        
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
             if constexpr (kSplit) {
