@@ -45,12 +45,14 @@ struct Unit {
     int group, m0, n0, cols, k0, k_len, kb0, kb;
 };
 
-// With few tiles the two CTAs of a cluster take half of a tile's inner dimension each: CTA 1 sends its sums
-// into CTA 0's shared memory, CTA 0 adds them to its own (always in this order) and stores.
+// With few tiles the CTAs of a cluster share a tile's inner dimension.
+// Two (kSplit = 2, few columns): CTA 1 sends its sums into CTA 0's shared memory, CTA 0 adds them to its own and
+// stores.  Four (kSplit = 4, long inner dimension): the tile's 64 columns are dealt out, 16 to a CTA; every CTA sends each
+// of the others its sums of the other's columns, adds what it gets for its own in the order of the CTAs, and stores.
 constexpr int kSplitRow = 36;  // words per row of the receiver's buffer: 32 columns, and 4 against bank conflicts
 struct SplitParams {
-    int role = -1;       // -1: whole tiles, 0: receives and stores, 1: sends
-    const float* recv;   // [128][kSplitRow]
+    int role = -1;       // -1: whole tiles, else this CTA's rank (of two: 0 receives and stores, 1 sends)
+    const float* recv;   // two: [128][kSplitRow], four: [rank][128][16]
     uint32_t recv_addr;
     uint32_t full_bar, empty_bar;
 };
@@ -65,7 +67,7 @@ struct EpilogueCfg {
 __device__ __forceinline__ int columns_of(int tile_cols, int wg, int cols) { return min(cols, max(0, tile_cols - wg * cols)); }
 
 // Warps 4 .. 11 (`wg` 0 or 1).  Barriers tmem_full / tmem_empty [kAccs] are 8 bytes apart.
-template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, bool kSplit, class Decode>
+template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, int kSplit, class Decode>
 __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, uint32_t tmem_base, uint32_t tmem_full, uint32_t tmem_empty,
                                              const WaitCtx& wc, int unit_first, int unit_stride, int num_units, const SplitParams& split,
                                              Decode decode) {
@@ -81,10 +83,10 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
     const int col0 = wg * E::COLS;
     uint32_t acc_count = 0, split_count = 0;
     bool ok = true;
-    const bool sends = kSplit && split.role == 1, receives = kSplit && split.role == 0;
-    const uint32_t remote = kSplit ? mapa_shared(split.recv_addr + et * kSplitRow * 4, 0) : 0u;
-    const uint32_t remote_bar = kSplit ? mapa_shared(split.full_bar, 0) : 0u;
-    static_assert(!kSplit || (E::COLS == W && W == 32), "partial sums are one step of columns");
+    const bool sends = kSplit == 2 && split.role == 1, receives = kSplit == 2 && split.role == 0;
+    const uint32_t remote = kSplit == 2 ? mapa_shared(split.recv_addr + et * kSplitRow * 4, 0) : 0u;
+    const uint32_t remote_bar = kSplit == 2 ? mapa_shared(split.full_bar, 0) : 0u;
+    static_assert(kSplit == 1 || (E::COLS == W && W == 32), "partial sums are one step of columns");
 
     // this warp's lines of C of a tile into L2, a lane to a column
     auto prefetch_c = [&](const Unit& u) {
@@ -173,12 +175,12 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                     c_next[i] = p.c_fmt == 2 ? __uint_as_float(static_cast<uint32_t>(raw[i]) << 16) : __half2float(__ushort_as_half(raw[i]));
             }
         };
-        if (has_c && !sends) prefetch_c(u);
-        if (kAhead && has_c && !sends && cols > 0) load_c(0);
+        if (has_c && !sends && kSplit != 4) prefetch_c(u);
+        if (kAhead && has_c && !sends && cols > 0 && kSplit != 4) load_c(0);
         
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
-            if constexpr (kSplit) {
+            if constexpr (kSplit == 2) {
                 if (sends || receives) exchange(r);
                 if (sends || !ok) return;
             }
@@ -236,6 +238,68 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             }
         };
 
+        // four CTAs: this thread's row of the warp group's 32 columns goes to two of them; the first warp group adds
+        // and stores this CTA's own columns
+        auto deal = [&](const float (&sum)[E::COLS]) {
+            constexpr int kShare = 2 * E::COLS / kSplit;  // columns of one CTA
+            ok = ok && mbar_wait_cluster(split.empty_bar, (split_count & 1u) ^ 1u, wc, kWaitPartial);  // room everywhere
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            const uint32_t at = split.recv_addr + (split.role * 128 + et) * kShare * 4;
+#pragma unroll
+            for (int q = 0; q < E::COLS / kShare; ++q) {
+                const uint32_t rank = wg * (E::COLS / kShare) + q, to = mapa_shared(at, rank), bar = mapa_shared(split.full_bar, rank);
+#pragma unroll
+                for (int i = 0; i < kShare; i += 4) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = __float_as_uint(sum[q * kShare + i + x]);
+                    st_async_cluster(to + i * 4, v, bar);
+                }
+            }
+            if (wg == 0) {
+                if (et == 0) mbar_arrive_expect_tx(split.full_bar, kSplit * 128 * kShare * 4);
+                ok = mbar_wait_cluster(split.full_bar, split_count & 1u, wc, kWaitPartial);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                float v[kShare] = {};
+#pragma unroll
+                for (int src = 0; src < kSplit; ++src) {
+                    const float4* in = reinterpret_cast<const float4*>(split.recv + (src * 128 + et) * kShare);
+#pragma unroll
+                    for (int i = 0; i < kShare / 4; ++i) {
+                        const float4 x = in[i];
+                        v[4 * i] += x.x;
+                        v[4 * i + 1] += x.y;
+                        v[4 * i + 2] += x.z;
+                        v[4 * i + 3] += x.w;
+                    }
+                }
+                __syncwarp();
+                if (lane < kSplit) mbar_arrive_cluster(split.empty_bar, lane);
+                const int n = u.n0 + split.role * kShare, left = u.cols - split.role * kShare;
+                const long long c_at = (kPerGroup ? u.group * p.stride_c : 0) + m + n * p.ldc;
+                const long long d_at = (kPerGroup ? u.group * p.stride_d : 0) + m + n * p.ldd;
+#pragma unroll
+                for (int i = 0; i < kShare; ++i) {
+                    if (m >= p.M || i >= left) continue;
+                    float x = alpha * v[i];
+                    if (has_c) {
+                        const long long e = c_at + i * p.ldc;
+                        const float c = p.c_fmt == 2   ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.C)[e])
+                                        : p.c_fmt == 1 ? __half2float(static_cast<const __half*>(p.C)[e])
+                                                       : static_cast<const float*>(p.C)[e];
+                        x = fmaf(beta, c, x);
+                    }
+                    const long long e = d_at + i * p.ldd;
+                    if (d_fmt == 2) static_cast<__nv_bfloat16*>(p.D)[e] = __float2bfloat16_rn(x);
+                    else if (d_fmt == 1) static_cast<__half*>(p.D)[e] = __float2half_rn(x);
+                    else static_cast<float*>(p.D)[e] = x;
+                }
+            }
+            ++split_count;
+        };
+
         if constexpr (kPromoteKb > 0) {
             float sum[E::COLS];
 #pragma unroll
@@ -256,8 +320,9 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 }
                 release(acc);
             }
+            if constexpr (kSplit == 4) deal(sum);
 #pragma unroll
-            for (int q = 0; q < E::COLS / W; ++q) {
+            for (int q = 0; q < (kSplit == 4 ? 0 : E::COLS / W); ++q) {
                 if (ok && q * W < cols) {
                     uint32_t r[W];
 #pragma unroll

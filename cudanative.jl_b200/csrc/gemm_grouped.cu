@@ -134,9 +134,8 @@ struct Grouped {
     const int32_t* offsets;
 };
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote>
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
 int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
-    constexpr bool kSplit = kBN == 32;  // few columns per group: pairs of CTAs that may share a tile's inner dimension
     using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
     auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote, kSplit>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
@@ -157,7 +156,7 @@ int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid,
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kSplit ? 2 : kCtas;
+    attr[0].val.clusterDim.x = kSplit > 1 ? kSplit : kCtas;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -171,8 +170,9 @@ int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid,
 // binary32 results add several accumulators with rounding to nearest (epilogue_sm100.cuh)
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
 int launch_grouped(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
-    if (p.e.d_fmt == 0) return launch_promote<kBN, kAMn, kRaggedK, kCtas, true>(tm, p, grid, stream, pdl);
-    return launch_promote<kBN, kAMn, kRaggedK, kCtas, false>(tm, p, grid, stream, pdl);
+    constexpr int kSplit = kBN == 32 ? 2 : 1;  // few columns per group: pairs of CTAs that may share a tile's inner dimension
+    if (p.e.d_fmt == 0) return launch_promote<kBN, kAMn, kRaggedK, kCtas, true, kSplit>(tm, p, grid, stream, pdl);
+    return launch_promote<kBN, kAMn, kRaggedK, kCtas, false, kSplit>(tm, p, grid, stream, pdl);
 }
 
 template <int kBN, int kCtas>
@@ -200,6 +200,18 @@ bool eligible(const Grouped& g, std::string* why) {
     return true;
 }
 
+// Few tiles and a long inner dimension: clusters of four CTAs share each tile's K (64-column tiles).  Measured, whole tiles
+// against shared ones: one round of clusters (at most SMs / 4 tiles) with K = 2048 12-17 / 11-13 us, K = 1024 8-12 /
+// 10-12 us; two rounds with K = 4096 28 / 28 us, K = 16384 88 / 52 us.
+bool shares_k(const b200_handle* h, const Grouped& g) {
+    if (h->tile_n != 0 || h->cta_pair != 0 || h->max_ctas != 0) return false;
+    const int64_t cols = g.ragged_k ? g.groups * ((g.N + 63) / 64) : g.N / 64 + std::min(g.groups, g.N);
+    const int64_t units = cols * ((g.M + 127) / 128), clusters = h->sm_count / 4;
+    const int64_t k = g.ragged_k ? g.K / g.groups : g.K;
+    if (!g.ragged_k && g.N <= 32 * g.groups) return false;  // 32-column tiles, in pairs
+    return (units <= clusters && k >= 2048) || (units <= 2 * clusters && k >= 8192);
+}
+
 // Tile columns.  Ragged N: the sizes of the groups are not known here, their mean is.  Wide tiles read
 // each A_e less often; the instruction's N follows the columns that a group really has.
 void pick_tile(const b200_handle* h, const Grouped& g, int* tile_n, int* pair) {
@@ -217,6 +229,11 @@ void pick_tile(const b200_handle* h, const Grouped& g, int* tile_n, int* pair) {
 int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     int tile_n, pair, rc;
     pick_tile(h, g, &tile_n, &pair);
+    const bool share = shares_k(h, g);
+    if (share) {
+        tile_n = 64;
+        pair = 1;
+    }
     GroupedParams p = {};
     p.e.M = static_cast<int>(g.M);
     p.N = static_cast<int>(g.N);
@@ -266,12 +283,17 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
     if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
-    if (pair == 2) rc = tile_n == 256 ? launch_kind<256, 2>(g, tm, p, grid, stream, pdl) : launch_kind<128, 2>(g, tm, p, grid, stream, pdl);
+    if (share) {
+        grid = static_cast<int>(std::min<int64_t>(std::max(cap / 4, 1), units)) * 4;
+        if (g.ragged_k) rc = launch_promote<64, true, true, 1, true, 4>(tm, p, grid, stream, pdl);
+        else if (g.transA) rc = launch_promote<64, false, false, 1, true, 4>(tm, p, grid, stream, pdl);
+        else rc = launch_promote<64, true, false, 1, true, 4>(tm, p, grid, stream, pdl);
+    } else if (pair == 2) rc = tile_n == 256 ? launch_kind<256, 2>(g, tm, p, grid, stream, pdl) : launch_kind<128, 2>(g, tm, p, grid, stream, pdl);
     else if (tile_n == 128) rc = launch_kind<128, 1>(g, tm, p, grid, stream, pdl);
     else if (tile_n == 64) rc = launch_kind<64, 1>(g, tm, p, grid, stream, pdl);
     else rc = launch_kind<32, 1>(g, tm, p, grid, stream, pdl);
     if (rc) return rc;
-    h->last = {B200_KERNEL_TCGEN05, tile_n, 1, grid, pair};
+    h->last = {B200_KERNEL_TCGEN05, tile_n, share ? 4 : 1, grid, pair};
     return B200_OK;
 }
 

@@ -44,7 +44,7 @@ struct GroupedParams {
     unsigned long long wait_budget_ns;
 };
 
-template <int kBN, bool kRaggedK, int kCtas, bool kPromote, bool kSplit>
+template <int kBN, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
 struct GroupedCfg {
     static constexpr int THREADS = 384;
     static constexpr int BM = 128;
@@ -60,13 +60,14 @@ struct GroupedCfg {
     using Epi = EpilogueCfg<kBN>;
     static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
-    static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
+    static constexpr int RECV_BYTES = kSplit == 2 ? 128 * kSplitRow * 4 : kSplit == 4 ? 128 * kBN * 4 : 0;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
     static constexpr int TMEM_COLS = 2 * kBN < 32 ? 32 : 2 * kBN;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
     static constexpr int NBARS = 4 * STAGES + 6;
-    static_assert(!kSplit || (kCtas == 1 && !kRaggedK && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
+    static_assert(kSplit != 2 || (kCtas == 1 && !kRaggedK && kBN == 32), "two share K: one-CTA tiles, one warp group");
+    static_assert(kSplit != 4 || (kCtas == 1 && kBN == 64 && kPromote), "four share K: one-CTA tiles, 16 columns each");
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
@@ -144,7 +145,7 @@ __device__ __forceinline__ int find_group(const int* first, int groups, int q) {
     return lo;
 }
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, bool kSplit>
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const GroupedParams p) {
@@ -195,7 +196,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             mbar_init(tmem_empty_bar(a), 8 * kCtas);
         }
         mbar_init(split_bar(0), 1);  // the receiver's arrive; it expects the sender's bytes
-        mbar_init(split_bar(1), 4);  // the receiver's four warps
+        mbar_init(split_bar(1), kSplit == 4 ? 16 : 4);  // four warps of the receiver, or of each of the four CTAs
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
@@ -203,7 +204,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     if (warp == 2) tmem_alloc<kCtas>(smem_u32(const_cast<uint32_t*>(tmem_slot)), Cfg::TMEM_COLS);
     tc_fence_before_sync();
     __syncthreads();
-    if constexpr (kPair || kSplit) cluster_sync_all();
+    if constexpr (kPair || kSplit > 1) cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     griddep_launch_dependents();
@@ -222,7 +223,12 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
     // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).
     SplitParams split;
-    if constexpr (kSplit) {
+    if constexpr (kSplit == 4) {
+        split.role = static_cast<int>(cluster_cta_rank());
+        unit_first = blockIdx.x >> 2;
+        unit_stride = gridDim.x >> 2;
+    }
+    if constexpr (kSplit == 2) {
         const int ctas = gridDim.x, kb_all = (p.K + Cfg::BK - 1) / Cfg::BK;
         const int whole = (num_units + ctas - 1) / ctas, halves = (num_units + ctas / 2 - 1) / (ctas / 2);
         if (kb_all >= 4 && halves < 2 * whole) {
@@ -230,6 +236,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
             unit_first = blockIdx.x >> 1;
             unit_stride = ctas >> 1;
         }
+    }
+    if constexpr (kSplit > 1) {
         split.recv = reinterpret_cast<const float*>(smem_gen + kRecvAt);
         split.recv_addr = smem_base + kRecvAt;
         split.full_bar = split_bar(0);
@@ -269,16 +277,16 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         u.kb0 = 0;
         u.kb = (u.k_len + Cfg::BK - 1) / Cfg::BK;
-        if (kSplit && split.role >= 0) {
-            const int half = (u.kb + 1) / 2;
-            u.kb0 = split.role * half;
-            u.kb = split.role ? u.kb - half : half;
+        if (kSplit > 1 && split.role >= 0) {  // this CTA's share, the last ones' may be short or empty
+            const int share = (u.kb + kSplit - 1) / kSplit;
+            u.kb0 = min(u.kb, split.role * share);
+            u.kb = min(share, u.kb - u.kb0);
         }
         return u;
     };
     auto inst_n = [&](const Unit& u) { return (u.cols + Cfg::GRANULE - 1) / Cfg::GRANULE * Cfg::GRANULE; };
-    // rows of a group's last k-block; a ragged 16-row step has to be padded with zeros
-    auto needs_tail = [&](const Unit& u) { return kRaggedK && (u.k_len % 16) != 0; };
+    // this CTA has the group's last k-block and its last 16-row step is ragged: it has to be padded with zeros
+    auto needs_tail = [&](const Unit& u) { return kRaggedK && (u.k_len % 16) != 0 && u.kb > 0 && (u.kb0 + u.kb) * Cfg::BK >= u.k_len; };
 
     // registers: 3 x 168 a thread at launch = 56 + 2 x 224; a binary32 result's sums stay in them
     if (warp < 4) {
@@ -447,7 +455,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 tail_ph ^= 1u << st;
                 // a tile is boxes of 64 (m or n) x 64 k, each k one line of 128 bytes: the swizzle moves
                 // 16-byte pieces inside a line only, so whole lines can be cleared
-                const int rem = u.k_len - (kb1 - 1) * Cfg::BK, end = (rem + 15) / 16 * 16;
+                const int rem = u.k_len - (u.kb0 + kb1 - 1) * Cfg::BK, end = (rem + 15) / 16 * 16;
                 const int boxes = 2 + (inst_n(u) / kCtas + 63) / 64;  // A's two come first, B's follow
                 uint8_t* tile = smem_gen + st * Cfg::STAGE_BYTES;
                 for (int i = lane; i < boxes * (end - rem) * 8; i += 32) {
@@ -468,7 +476,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     } else {
         regs_inc<224>();
         const int wg = (warp - 4) >> 2;
-        run_epilogue<Epi, kBN, 2, kCtas, kPromote, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote && kSplit != 4, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
             p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 
@@ -479,7 +487,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const unsigned long long t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
     }
-    if constexpr (kPair || kSplit) cluster_sync_all();
+    if constexpr (kPair || kSplit > 1) cluster_sync_all();
     if (warp == 2) {
         tc_fence_after_sync();
         tmem_dealloc<kCtas>(tmem_base, Cfg::TMEM_COLS);

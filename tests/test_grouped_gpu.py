@@ -528,3 +528,25 @@ print("captured first")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+@pytest.mark.parametrize("beta", [0.0, 1.0])
+def test_k_long_groups_share_the_inner_dimension(handle, d_type, beta):
+    """Few tiles and long groups: four CTAs take a share of a tile's columns of A and B each; shares that are ragged,
+    short or empty, edges in M and N, two rounds of tiles."""
+    for sizes, M, N, shared in (([4099], 72, 40, True), ([2048], 136, 72, True), ([9000, 0, 15, 7000], 64, 136, True), ([4096, 4100], 256, 512, True),
+                                ([5000, 1, 64, 448], 136, 200, False), ([8000, 1, 64, 448], 136, 200, True), ([3001] * 18, 64, 64, True),
+                                ([8200] * 4, 264, 264, True), ([9000, 0, 15, 7000], 64, 130, False), ([5000, 1, 64, 448], 130, 200, False)):
+        run_grouped_k(handle, sizes, M, N, d_type=d_type, c_type=d_type if d_type is not F16 else F32, beta=beta, start=2, tail=3)
+        assert (handle.last_launch()["split_k"] == 4) == shared
+    run_grouped_k(handle, [4099], 71, 33, d_type=d_type, pad=1, beta=beta, expect=_lib.KERNEL_SIMPLE)
+
+
+@pytest.mark.parametrize("d_type", [F16, BFloat16, F32])
+@pytest.mark.parametrize("transA", [True, False])
+def test_few_tiles_share_the_inner_dimension(handle, d_type, transA):
+    for sizes, M, K in (([70], 72, 2048), ([64, 0, 65, 3, 190], 136, 2056), ([33], 264, 4104), ([400], 520, 8200), ([100, 100], 8, 2311 * 8)):
+        run_grouped(handle, sizes, M, K, transA=transA, d_type=d_type, beta=0.5, c_type=F32, start=1, tail=2)
+        assert handle.last_launch()["split_k"] == 4
+    run_grouped(handle, [70], 71, 2056, d_type=d_type, expect=_lib.KERNEL_TCGEN05)
