@@ -177,7 +177,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
         };
         if (has_c && !sends && kSplit != 4) prefetch_c(u);
         if (kAhead && has_c && !sends && cols > 0 && kSplit != 4) load_c(0);
-        
+
         // W columns from column j * W of this warp group on: the whole warp, `ok` in every lane
         auto finish = [&](int j, uint32_t (&r)[W]) {
             if constexpr (kSplit == 2) {

@@ -290,189 +290,189 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
     // registers: 3 x 168 a thread at launch = 56 + 2 x 224; a binary32 result's sums stay in them
     if (warp < 4) {
-    regs_dec<56>();
-    if (warp == 0) {
-        // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            const uint64_t once = l2_policy_evict_first();
-            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const Unit u = decode(unit);
-                const int ninst = inst_n(u);
-                const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
-                const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
-                const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
-                const int kb1 = u.kb;
-                const int z = u.group * p.a_per_group;
-                // one tile column in this group: A is read once, B again and again
-                const bool a_once = !kRaggedK && first[u.group + 1] - first[u.group] == 1;
-                for (int kb = 0; kb < kb1; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
-                    if (!ok) break;
-                    const uint32_t sa = smem_base + s * Cfg::STAGE_BYTES;
-                    const uint32_t sb = sa + Cfg::A_BYTES;
-                    const int k0 = u.k0 + (u.kb0 + kb) * Cfg::BK;
-                    if constexpr (kRaggedK) {
-                        const bool tail = needs_tail(u) && kb + 1 == kb1;
-                        if (tail) {
-                            // lands on this CTA's own barrier; warp 3 passes it on to the MMA issuer
-                            const uint32_t tb = tail_full_bar(s);
-                            mbar_arrive_expect_tx(tb, bytes);
-                            tma_load_2d(sa, &tmA, u.m0, k0, tb);
-                            tma_load_2d(sa + 8192, &tmA, u.m0 + 64, k0, tb);
-                            for (int i = 0; i < boxes; ++i) tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, tb);
-                            if (cta_rank == 0) mbar_arrive(full_bar(s));  // keeps the stage's phase in step
-                        } else if constexpr (kPair) {
-                            const uint32_t fb = mapa_shared(full_bar(s), 0);
-                            if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * bytes);
-                            tma_load_2d_pair(sa, &tmA, u.m0, k0, fb);
-                            tma_load_2d_pair(sa + 8192, &tmA, u.m0 + 64, k0, fb);
-                            for (int i = 0; i < boxes; ++i) tma_load_2d_pair(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, fb);
+        regs_dec<56>();
+        if (warp == 0) {
+            // ------------------------------------------------------------------ TMA producer
+            if (lane == 0) {
+                int s = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                const uint64_t once = l2_policy_evict_first();
+                for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                    const Unit u = decode(unit);
+                    const int ninst = inst_n(u);
+                    const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
+                    const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
+                    const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
+                    const int kb1 = u.kb;
+                    const int z = u.group * p.a_per_group;
+                    // one tile column in this group: A is read once, B again and again
+                    const bool a_once = !kRaggedK && first[u.group + 1] - first[u.group] == 1;
+                    for (int kb = 0; kb < kb1; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                        ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
+                        if (!ok) break;
+                        const uint32_t sa = smem_base + s * Cfg::STAGE_BYTES;
+                        const uint32_t sb = sa + Cfg::A_BYTES;
+                        const int k0 = u.k0 + (u.kb0 + kb) * Cfg::BK;
+                        if constexpr (kRaggedK) {
+                            const bool tail = needs_tail(u) && kb + 1 == kb1;
+                            if (tail) {
+                                // lands on this CTA's own barrier; warp 3 passes it on to the MMA issuer
+                                const uint32_t tb = tail_full_bar(s);
+                                mbar_arrive_expect_tx(tb, bytes);
+                                tma_load_2d(sa, &tmA, u.m0, k0, tb);
+                                tma_load_2d(sa + 8192, &tmA, u.m0 + 64, k0, tb);
+                                for (int i = 0; i < boxes; ++i) tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, tb);
+                                if (cta_rank == 0) mbar_arrive(full_bar(s));  // keeps the stage's phase in step
+                            } else if constexpr (kPair) {
+                                const uint32_t fb = mapa_shared(full_bar(s), 0);
+                                if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * bytes);
+                                tma_load_2d_pair(sa, &tmA, u.m0, k0, fb);
+                                tma_load_2d_pair(sa + 8192, &tmA, u.m0 + 64, k0, fb);
+                                for (int i = 0; i < boxes; ++i) tma_load_2d_pair(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, fb);
+                            } else {
+                                const uint32_t fb = full_bar(s);
+                                mbar_arrive_expect_tx(fb, bytes);
+                                tma_load_2d(sa, &tmA, u.m0, k0, fb);
+                                tma_load_2d(sa + 8192, &tmA, u.m0 + 64, k0, fb);
+                                for (int i = 0; i < boxes; ++i) tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, fb);
+                            }
                         } else {
-                            const uint32_t fb = full_bar(s);
-                            mbar_arrive_expect_tx(fb, bytes);
-                            tma_load_2d(sa, &tmA, u.m0, k0, fb);
-                            tma_load_2d(sa + 8192, &tmA, u.m0 + 64, k0, fb);
-                            for (int i = 0; i < boxes; ++i) tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, nb0 + i * 64, k0, fb);
-                        }
-                    } else {
-                        uint32_t fb = full_bar(s);
-                        if constexpr (kPair) fb = mapa_shared(fb, 0);
-                        if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
-                        auto load_a = [&](uint32_t dst, int x, int y) {
-                            if constexpr (kPair) tma_load_3d_pair(dst, &tmA, x, y, z, fb);
-                            else if (a_once) tma_load_3d_hint(dst, &tmA, x, y, z, fb, once);
-                            else tma_load_3d(dst, &tmA, x, y, z, fb);
-                        };
-                        if constexpr (kAMn) {
-                            load_a(sa, u.m0, k0);
-                            load_a(sa + 8192, u.m0 + 64, k0);
-                        } else {
-                            load_a(sa, k0, u.m0);
-                        }
-                        for (int i = 0; i < boxes; ++i) {
-                            if constexpr (kPair) tma_load_2d_pair(sb + i * Cfg::BBOX_BYTES, &tmB, k0, nb0 + i * Cfg::BBOX, fb);
-                            else tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, k0, nb0 + i * Cfg::BBOX, fb);
+                            uint32_t fb = full_bar(s);
+                            if constexpr (kPair) fb = mapa_shared(fb, 0);
+                            if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
+                            auto load_a = [&](uint32_t dst, int x, int y) {
+                                if constexpr (kPair) tma_load_3d_pair(dst, &tmA, x, y, z, fb);
+                                else if (a_once) tma_load_3d_hint(dst, &tmA, x, y, z, fb, once);
+                                else tma_load_3d(dst, &tmA, x, y, z, fb);
+                            };
+                            if constexpr (kAMn) {
+                                load_a(sa, u.m0, k0);
+                                load_a(sa + 8192, u.m0 + 64, k0);
+                            } else {
+                                load_a(sa, k0, u.m0);
+                            }
+                            for (int i = 0; i < boxes; ++i) {
+                                if constexpr (kPair) tma_load_2d_pair(sb + i * Cfg::BBOX_BYTES, &tmB, k0, nb0 + i * Cfg::BBOX, fb);
+                                else tma_load_2d(sb + i * Cfg::BBOX_BYTES, &tmB, k0, nb0 + i * Cfg::BBOX, fb);
+                            }
                         }
                     }
                 }
             }
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
-        // The whole warp walks the loop and one lane issues: see umma_mxf4 in ptx_sm100.cuh.
-        if (cta_rank == 0) {
-            const uint32_t lead = elect_lane();
-            const uint32_t idesc0 = make_idesc_f16_f32(Cfg::BM * kCtas, 0, kAMn ? 1 : 0, kBMn ? 1 : 0, p.ab_bf16 ? 1 : 0);
-            const uint64_t da0 = kAMn ? make_smem_desc(smem_base, 8192, 1024, kSwizzle128B)
-                                      : make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
-            const uint64_t db0 = kBMn ? make_smem_desc(smem_base + Cfg::A_BYTES, 8192, 1024, kSwizzle128B)
-                                      : make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
-            constexpr uint32_t kStepA = (kAMn ? 2048 : 32) >> 4, kStepB = (kBMn ? 2048 : 32) >> 4;
-            int s = 0;
-            uint32_t ph = 0, tail_ph = 0, ucount = 0;
-            bool ok = true, ready = false;
-            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const Unit u = decode(unit);
-                // an empty group has no accumulator
-                const int kb_total = __shfl_sync(0xffffffffu, u.kb, 0);
-                const uint32_t idesc = idesc0 | (static_cast<uint32_t>(__shfl_sync(0xffffffffu, inst_n(u), 0) >> 3) << 17);
-                // 16-row steps of the last k-block; whether it has to be padded with zeros first
-                const int last_steps = min(Cfg::BK / 16, (u.k_len - (u.kb0 + kb_total - 1) * Cfg::BK + 15) / 16);
-                const bool tail = needs_tail(u);
-                auto products = [&](int st, uint32_t acc, bool first, int steps) {
-                    const uint32_t d_tmem = tmem_base + acc * kBN;
-                    const uint64_t da = da0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
-                    const uint64_t db = db0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
+            __syncwarp();
+        } else if (warp == 1) {
+            // ------------------------------------------------------------------ MMA issuer
+            // The whole warp walks the loop and one lane issues: see umma_mxf4 in ptx_sm100.cuh.
+            if (cta_rank == 0) {
+                const uint32_t lead = elect_lane();
+                const uint32_t idesc0 = make_idesc_f16_f32(Cfg::BM * kCtas, 0, kAMn ? 1 : 0, kBMn ? 1 : 0, p.ab_bf16 ? 1 : 0);
+                const uint64_t da0 = kAMn ? make_smem_desc(smem_base, 8192, 1024, kSwizzle128B)
+                                          : make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
+                const uint64_t db0 = kBMn ? make_smem_desc(smem_base + Cfg::A_BYTES, 8192, 1024, kSwizzle128B)
+                                          : make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
+                constexpr uint32_t kStepA = (kAMn ? 2048 : 32) >> 4, kStepB = (kBMn ? 2048 : 32) >> 4;
+                int s = 0;
+                uint32_t ph = 0, tail_ph = 0, ucount = 0;
+                bool ok = true, ready = false;
+                for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                    const Unit u = decode(unit);
+                    // an empty group has no accumulator
+                    const int kb_total = __shfl_sync(0xffffffffu, u.kb, 0);
+                    const uint32_t idesc = idesc0 | (static_cast<uint32_t>(__shfl_sync(0xffffffffu, inst_n(u), 0) >> 3) << 17);
+                    // 16-row steps of the last k-block; whether it has to be padded with zeros first
+                    const int last_steps = min(Cfg::BK / 16, (u.k_len - (u.kb0 + kb_total - 1) * Cfg::BK + 15) / 16);
+                    const bool tail = needs_tail(u);
+                    auto products = [&](int st, uint32_t acc, bool first, int steps) {
+                        const uint32_t d_tmem = tmem_base + acc * kBN;
+                        const uint64_t da = da0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
+                        const uint64_t db = db0 + static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < Cfg::BK / 16; ++k)
-                        if (k < steps) umma_f16_warp<kCtas>(lead, d_tmem, da + k * kStepA, db + k * kStepB, idesc, (first && k == 0) ? 0u : 1u);
-                    if (lead) {
-                        if constexpr (kPair) umma_commit_pair(empty_bar(st));
-                        else umma_commit<kCtas>(empty_bar(st));
+                        for (int k = 0; k < Cfg::BK / 16; ++k)
+                            if (k < steps) umma_f16_warp<kCtas>(lead, d_tmem, da + k * kStepA, db + k * kStepB, idesc, (first && k == 0) ? 0u : 1u);
+                        if (lead) {
+                            if constexpr (kPair) umma_commit_pair(empty_bar(st));
+                            else umma_commit<kCtas>(empty_bar(st));
+                        }
+                    };
+                    auto wait_tail = [&](int st) {  // the last k-block's foreign rows are zero
+                        const bool done = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail));
+                        tail_ph ^= 1u << st;
+                        return done;
+                    };
+                    // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products.
+                    static_assert(Cfg::PROMOTE_KB % 2 == 0, "an accumulator begins and ends with a turn");
+                    for (int kb = 0; kb < kb_total; kb += 2) {
+                        const uint32_t acc = ucount & 1u;
+                        const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
+                        const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
+                        const bool two = kb + 1 < kb_total, last = kb + 2 >= kb_total;
+                        const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
+                        const bool end = last || (kPromote && (kb + 2) % Cfg::PROMOTE_KB == 0);
+                        if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                        if (ok && !ready)
+                            ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
+                                                             (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
+                        if (ok && last && tail) ok = wait_tail(two ? s1 : s);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        if (two) {
+                            // look at the next two now: the answer arrives while these two's products are issued
+                            const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
+                            products(s, acc, begin, Cfg::BK / 16);
+                            products(s1, acc, false, last ? last_steps : Cfg::BK / 16);
+                            ready = __all_sync(0xffffffffu, next);
+                            s = s2;
+                            ph = ph2;
+                        } else {
+                            products(s, acc, begin, last_steps);
+                            ready = false;
+                            s = s1;
+                            ph = ph1;
+                        }
+                        if (lead && end) {
+                            if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                            else umma_commit<kCtas>(tmem_full_bar(acc));
+                        }
+                        ucount += end ? 1u : 0u;
                     }
-                };
-                auto wait_tail = [&](int st) {  // the last k-block's foreign rows are zero
-                    const bool done = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail));
-                    tail_ph ^= 1u << st;
-                    return done;
-                };
-                // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products.
-                static_assert(Cfg::PROMOTE_KB % 2 == 0, "an accumulator begins and ends with a turn");
-                for (int kb = 0; kb < kb_total; kb += 2) {
-                    const uint32_t acc = ucount & 1u;
-                    const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
-                    const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
-                    const bool two = kb + 1 < kb_total, last = kb + 2 >= kb_total;
-                    const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
-                    const bool end = last || (kPromote && (kb + 2) % Cfg::PROMOTE_KB == 0);
-                    if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
-                    if (ok && !ready)
-                        ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
-                                                         (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
-                    if (ok && last && tail) ok = wait_tail(two ? s1 : s);
+                }
+            }
+            __syncwarp();
+        } else if (kRaggedK && warp == 3) {
+            // ------------------------------------------------------------------ zeros behind a group's last row
+            int s = 0;
+            uint32_t tail_ph = 0;
+            bool ok = true;
+            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                const Unit u = decode(unit);
+                const int kb1 = u.kb;
+                if (needs_tail(u)) {
+                    const int st = (s + kb1 - 1) % STAGES;
+                    ok = mbar_wait(tail_full_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    tc_fence_after_sync();
-                    if (two) {
-                        // look at the next two now: the answer arrives while these two's products are issued
-                        const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
-                        products(s, acc, begin, Cfg::BK / 16);
-                        products(s1, acc, false, last ? last_steps : Cfg::BK / 16);
-                        ready = __all_sync(0xffffffffu, next);
-                        s = s2;
-                        ph = ph2;
-                    } else {
-                        products(s, acc, begin, last_steps);
-                        ready = false;
-                        s = s1;
-                        ph = ph1;
+                    tail_ph ^= 1u << st;
+                    // a tile is boxes of 64 (m or n) x 64 k, each k one line of 128 bytes: the swizzle moves
+                    // 16-byte pieces inside a line only, so whole lines can be cleared
+                    const int rem = u.k_len - (u.kb0 + kb1 - 1) * Cfg::BK, end = (rem + 15) / 16 * 16;
+                    const int boxes = 2 + (inst_n(u) / kCtas + 63) / 64;  // A's two come first, B's follow
+                    uint8_t* tile = smem_gen + st * Cfg::STAGE_BYTES;
+                    for (int i = lane; i < boxes * (end - rem) * 8; i += 32) {
+                        const int box = i / ((end - rem) * 8), in = i - box * ((end - rem) * 8);
+                        *reinterpret_cast<uint4*>(tile + box * 8192 + (rem + in / 8) * 128 + (in & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
-                    if (lead && end) {
-                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                        else umma_commit<kCtas>(tmem_full_bar(acc));
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if constexpr (kPair) mbar_arrive_cluster(tail_ready_bar(st), 0);
+                        else mbar_arrive(tail_ready_bar(st));
                     }
-                    ucount += end ? 1u : 0u;
                 }
+                s = (s + kb1) % STAGES;
             }
+            __syncwarp();
         }
-        __syncwarp();
-    } else if (kRaggedK && warp == 3) {
-        // ------------------------------------------------------------------ zeros behind a group's last row
-        int s = 0;
-        uint32_t tail_ph = 0;
-        bool ok = true;
-        for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-            const Unit u = decode(unit);
-            const int kb1 = u.kb;
-            if (needs_tail(u)) {
-                const int st = (s + kb1 - 1) % STAGES;
-                ok = mbar_wait(tail_full_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tail_ph ^= 1u << st;
-                // a tile is boxes of 64 (m or n) x 64 k, each k one line of 128 bytes: the swizzle moves
-                // 16-byte pieces inside a line only, so whole lines can be cleared
-                const int rem = u.k_len - (u.kb0 + kb1 - 1) * Cfg::BK, end = (rem + 15) / 16 * 16;
-                const int boxes = 2 + (inst_n(u) / kCtas + 63) / 64;  // A's two come first, B's follow
-                uint8_t* tile = smem_gen + st * Cfg::STAGE_BYTES;
-                for (int i = lane; i < boxes * (end - rem) * 8; i += 32) {
-                    const int box = i / ((end - rem) * 8), in = i - box * ((end - rem) * 8);
-                    *reinterpret_cast<uint4*>(tile + box * 8192 + (rem + in / 8) * 128 + (in & 7) * 16) = make_uint4(0, 0, 0, 0);
-                }
-                asm volatile("fence.proxy.async;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (kPair) mbar_arrive_cluster(tail_ready_bar(st), 0);
-                    else mbar_arrive(tail_ready_bar(st));
-                }
-            }
-            s = (s + kb1) % STAGES;
-        }
-        __syncwarp();
-    }
     } else {
         regs_inc<224>();
         const int wg = (warp - 4) >> 2;

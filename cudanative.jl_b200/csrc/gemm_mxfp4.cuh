@@ -198,138 +198,138 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
     // registers: 4 x 128 a thread at launch = 2 x 56 + 2 x 200; the epilogue holds half a tile row in them
     if (warp < 4) {
-    regs_dec<56>();
-    if (warp == 0) {
-        // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            const uint64_t once = l2_policy_evict_first();
-            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const Unit u = decode(unit);
-                const int ninst = inst_n(u);
-                const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
-                const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
-                const bool a_once = first[u.group + 1] - first[u.group] == 1;
-                const int z = u.group * p.a_per_group;
-                const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
-                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
-                    if (!ok) break;
-                    const uint32_t at_a = smem_base + s * Cfg::STAGE_BYTES;
-                    const uint32_t at_b = at_a + Cfg::A_BYTES;
-                    uint32_t fb = full_bar(s);
-                    if constexpr (kPair) fb = mapa_shared(fb, 0);
-                    if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
-                    if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
-                    else if (a_once) tma_load_3d_hint(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb, once);
-                    else tma_load_3d(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
-                    auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
-                        if constexpr (kPair) tma_load_2d_pair(dst, tm, x, y, fb);
-                        else tma_load_2d(dst, tm, x, y, fb);
-                    };
-                    for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, (kb_first + kb) * 128, nb0 + i * Cfg::BBOX);
+        regs_dec<56>();
+        if (warp == 0) {
+            // ------------------------------------------------------------------ TMA producer
+            if (lane == 0) {
+                int s = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                const uint64_t once = l2_policy_evict_first();
+                for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                    const Unit u = decode(unit);
+                    const int ninst = inst_n(u);
+                    const int nb0 = u.n0 + static_cast<int>(cta_rank) * (ninst / kCtas);
+                    const int boxes = (ninst / kCtas + Cfg::BBOX - 1) / Cfg::BBOX;
+                    const bool a_once = first[u.group + 1] - first[u.group] == 1;
+                    const int z = u.group * p.a_per_group;
+                    const uint32_t bytes = Cfg::A_BYTES + boxes * Cfg::BBOX_BYTES;
+                    for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                        ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
+                        if (!ok) break;
+                        const uint32_t at_a = smem_base + s * Cfg::STAGE_BYTES;
+                        const uint32_t at_b = at_a + Cfg::A_BYTES;
+                        uint32_t fb = full_bar(s);
+                        if constexpr (kPair) fb = mapa_shared(fb, 0);
+                        if (cta_rank == 0) mbar_arrive_expect_tx(full_bar(s), kCtas * bytes);
+                        if constexpr (kPair) tma_load_3d_pair(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
+                        else if (a_once) tma_load_3d_hint(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb, once);
+                        else tma_load_3d(at_a, &tmA, (kb_first + kb) * 128, u.m0, z, fb);
+                        auto load = [&](uint32_t dst, const CUtensorMap* tm, int x, int y) {
+                            if constexpr (kPair) tma_load_2d_pair(dst, tm, x, y, fb);
+                            else tma_load_2d(dst, tm, x, y, fb);
+                        };
+                        for (int i = 0; i < boxes; ++i) load(at_b + i * Cfg::BBOX_BYTES, &tmB, (kb_first + kb) * 128, nb0 + i * Cfg::BBOX);
+                    }
                 }
             }
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
-        if (cta_rank == 0) {
-            const uint32_t lead = elect_lane();
-            const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
-            const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
-            int s = 0;
-            uint32_t ph = 0, ucount = 0;
-            bool ok = true, ready = false;
-            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const Unit u = decode(unit);
-                // 192 columns begin at row 0 or 64 of their scale tile: two columns of 32 rows further
-                const uint32_t shift = kBN == 192 ? __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0) : 0u;
-                const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
-                const uint32_t acc = ucount % ACCS;
-                const uint32_t d_tmem = tmem_base + acc * kBN;
-                ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty));
-                if (!ok) break;
-                const int last_steps = min(4, (p.K - (kb_first + kb_total - 1) * Cfg::BK + 63) / 64);
-                auto products = [&](int st, bool first, int steps) {
-                    const uint64_t step = static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
-                    const uint32_t sfa = tmem_base + Cfg::SCALE_AT + st * Cfg::SCALE_COLS, sfb = sfa + 8 + shift;
+            __syncwarp();
+        } else if (warp == 1) {
+            // ------------------------------------------------------------------ MMA issuer
+            if (cta_rank == 0) {
+                const uint32_t lead = elect_lane();
+                const uint64_t da0 = make_smem_desc(smem_base, 16, 1024, kSwizzle128B);
+                const uint64_t db0 = make_smem_desc(smem_base + Cfg::A_BYTES, 16, 1024, kSwizzle128B);
+                int s = 0;
+                uint32_t ph = 0, ucount = 0;
+                bool ok = true, ready = false;
+                for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                    const Unit u = decode(unit);
+                    // 192 columns begin at row 0 or 64 of their scale tile: two columns of 32 rows further
+                    const uint32_t shift = kBN == 192 ? __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0) : 0u;
+                    const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
+                    const uint32_t acc = ucount % ACCS;
+                    const uint32_t d_tmem = tmem_base + acc * kBN;
+                    ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    if (!ok) break;
+                    const int last_steps = min(4, (p.K - (kb_first + kb_total - 1) * Cfg::BK + 63) / 64);
+                    auto products = [&](int st, bool first, int steps) {
+                        const uint64_t step = static_cast<uint64_t>(st * (Cfg::STAGE_BYTES >> 4));
+                        const uint32_t sfa = tmem_base + Cfg::SCALE_AT + st * Cfg::SCALE_COLS, sfb = sfa + 8 + shift;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k < steps) {
-                            const uint32_t id = idesc0 | (k & 1 ? (2u << 4) | (2u << 29) : 0u);
-                            umma_mxf4<kCtas>(lead, d_tmem, da0 + step + 2 * k, db0 + step + 2 * k, id, sfa + 4 * (k >> 1),
-                                             sfb + (k >> 1) * Cfg::B_TILES * 4, (first && k == 0) ? 0u : 1u);
+                        for (int k = 0; k < 4; ++k) {
+                            if (k < steps) {
+                                const uint32_t id = idesc0 | (k & 1 ? (2u << 4) | (2u << 29) : 0u);
+                                umma_mxf4<kCtas>(lead, d_tmem, da0 + step + 2 * k, db0 + step + 2 * k, id, sfa + 4 * (k >> 1),
+                                                 sfb + (k >> 1) * Cfg::B_TILES * 4, (first && k == 0) ? 0u : 1u);
+                            }
+                        }
+                        if (lead) {
+                            if constexpr (kPair) umma_commit_pair(empty_bar(st));
+                            else umma_commit<kCtas>(empty_bar(st));
+                        }
+                    };
+                    // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products
+                    // (8192^3: 204 us one by one, 187 us).
+                    for (int kb = 0; kb < kb_total; kb += 2) {
+                        const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
+                        const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
+                        const bool two = kb + 1 < kb_total;
+                        if (!ready)
+                            ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
+                                                             (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        if (two) {
+                            // look at the next two now: the answer arrives while these two's products are issued
+                            const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
+                            products(s, kb == 0, 4);
+                            products(s1, false, kb + 2 == kb_total ? last_steps : 4);
+                            ready = __all_sync(0xffffffffu, next);
+                            s = s2;
+                            ph = ph2;
+                        } else {
+                            products(s, kb == 0, last_steps);
+                            ready = false;
+                            s = s1;
+                            ph = ph1;
                         }
                     }
+                    if (!ok) break;
                     if (lead) {
-                        if constexpr (kPair) umma_commit_pair(empty_bar(st));
-                        else umma_commit<kCtas>(empty_bar(st));
+                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                        else umma_commit<kCtas>(tmem_full_bar(acc));
                     }
-                };
-                // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products
-                // (8192^3: 204 us one by one, 187 us).
-                for (int kb = 0; kb < kb_total; kb += 2) {
-                    const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
-                    const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
-                    const bool two = kb + 1 < kb_total;
-                    if (!ready)
-                        ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
-                                                         (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    if (two) {
-                        // look at the next two now: the answer arrives while these two's products are issued
-                        const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
-                        products(s, kb == 0, 4);
-                        products(s1, false, kb + 2 == kb_total ? last_steps : 4);
-                        ready = __all_sync(0xffffffffu, next);
-                        s = s2;
-                        ph = ph2;
-                    } else {
-                        products(s, kb == 0, last_steps);
-                        ready = false;
-                        s = s1;
-                        ph = ph1;
-                    }
-                }
-                if (!ok) break;
-                if (lead) {
-                    if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                    else umma_commit<kCtas>(tmem_full_bar(acc));
-                }
-                ++ucount;
-            }
-        }
-        __syncwarp();
-    } else if (warp == 3) {
-        // ------------------------------------------------------------------ TMA producer of the scales
-        // A thread of its own: with the scales' copies in warp 0 its issue rate bounds the pipeline.
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
-                const Unit u = decode(unit);
-                // a CTA of a pair may own no rows of A: its scales are then those of the last rows
-                const int a_row = u.group * p.a_per_group * p.a_tile_rows + min(u.m0 / 128, p.a_tile_rows - 1);
-                const int b_row = first128[u.group] + (u.n0 - off[u.group]) / 128;
-                for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
-                    if (!ok) break;
-                    const uint32_t at = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES;
-                    // two tiles along K (behind an odd last one: zeros), B_TILES along the columns; tiles that
-                    // this tile's columns do not touch are loaded and not used
-                    mbar_arrive_expect_tx(scales_full_bar(s), Cfg::SF_BYTES);
-                    tma_load_3d(at, &tmSA, 0, 2 * (kb_first + kb), a_row, scales_full_bar(s));
-                    tma_load_3d(at + 1024, &tmSB, 0, 2 * (kb_first + kb), b_row, scales_full_bar(s));
+                    ++ucount;
                 }
             }
+            __syncwarp();
+        } else if (warp == 3) {
+            // ------------------------------------------------------------------ TMA producer of the scales
+            // A thread of its own: with the scales' copies in warp 0 its issue rate bounds the pipeline.
+            if (lane == 0) {
+                int s = 0;
+                uint32_t ph = 0;
+                bool ok = true;
+                for (int unit = unit_first; ok && unit < num_units; unit += unit_stride) {
+                    const Unit u = decode(unit);
+                    // a CTA of a pair may own no rows of A: its scales are then those of the last rows
+                    const int a_row = u.group * p.a_per_group * p.a_tile_rows + min(u.m0 / 128, p.a_tile_rows - 1);
+                    const int b_row = first128[u.group] + (u.n0 - off[u.group]) / 128;
+                    for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                        ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
+                        if (!ok) break;
+                        const uint32_t at = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES;
+                        // two tiles along K (behind an odd last one: zeros), B_TILES along the columns; tiles that
+                        // this tile's columns do not touch are loaded and not used
+                        mbar_arrive_expect_tx(scales_full_bar(s), Cfg::SF_BYTES);
+                        tma_load_3d(at, &tmSA, 0, 2 * (kb_first + kb), a_row, scales_full_bar(s));
+                        tma_load_3d(at + 1024, &tmSB, 0, 2 * (kb_first + kb), b_row, scales_full_bar(s));
+                    }
+                }
+            }
+            __syncwarp();
         }
-        __syncwarp();
-    }
     } else if (warp >= 12) {
         regs_dec<56>();
         // ------------------------------------------------------------------ scales: shared -> tensor memory

@@ -122,7 +122,7 @@ __device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off
 
 // Vectors whose values are contiguous.  A tile is 128 vectors x 128 values: 16 lanes take a vector's 128, eight
 // values (16 bytes of a 16-bit type) each, so that a warp reads and writes whole lines; four lanes find a
-// block's largest magnitude with two shuffles.  A thread has eight vectors in flight.
+// block's largest magnitude with two shuffles.  A thread has four vectors in flight.
 template <typename T>
 __global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p) {
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
@@ -144,47 +144,47 @@ __global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p
         constexpr int kVec = 8 * sizeof(T) / 16;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-        const int r0 = first_row + 64 * half;
-        uint4 raw[4][kVec];
-        const T* src = X + (t.first + r0) * p.ldx + k0;
-        if (wide && k_tile * 128 + 128 <= p.K) {  // all loads before the first use
+            const int r0 = first_row + 64 * half;
+            uint4 raw[4][kVec];
+            const T* src = X + (t.first + r0) * p.ldx + k0;
+            if (wide && k_tile * 128 + 128 <= p.K) {  // all loads before the first use
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < kVec; ++j)
-                    raw[i][j] = r0 + 16 * i < t.count ? reinterpret_cast<const uint4*>(src + 16 * i * p.ldx)[j] : make_uint4(0, 0, 0, 0);
-        } else {
+                    for (int j = 0; j < kVec; ++j)
+                        raw[i][j] = r0 + 16 * i < t.count ? reinterpret_cast<const uint4*>(src + 16 * i * p.ldx)[j] : make_uint4(0, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    T* e = reinterpret_cast<T*>(raw[i]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e[j] = r0 + 16 * i < t.count && k0 + j < p.K ? src[16 * i * p.ldx + j] : from_float<T>(0.0f);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                T* e = reinterpret_cast<T*>(raw[i]);
+                const int r = r0 + 16 * i;
+                const T* e = reinterpret_cast<const T*>(raw[i]);
+                float v[8];
+                uint32_t top = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = r0 + 16 * i < t.count && k0 + j < p.K ? src[16 * i * p.ldx + j] : from_float<T>(0.0f);
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = as_float(e[j]);
+                    top = max(top, magnitude(v[j]));
+                }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                uint32_t s = scale_code(top);
+                const float inv = inverse(s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] *= inv;
+                if (r < t.count && k0 < (p.K + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(p.Q + ((t.first + r) * p.ldq + k0) / 2) = to_elements(v);
+                // a vector's four scales as one word; vectors and blocks that do not exist were read as zeros: s = 0
+                s <<= 8 * (part / 4);
+                s |= __shfl_xor_sync(0xffffffffu, s, 4);
+                s |= __shfl_xor_sync(0xffffffffu, s, 8);
+                if (part == 0) *reinterpret_cast<uint32_t*>(p.S + scale_at(q, kt, k_tile * 4, r)) = s;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = r0 + 16 * i;
-            const T* e = reinterpret_cast<const T*>(raw[i]);
-            float v[8];
-            uint32_t top = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = as_float(e[j]);
-                top = max(top, magnitude(v[j]));
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            uint32_t s = scale_code(top);
-            const float inv = inverse(s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= inv;
-            if (r < t.count && k0 < (p.K + 31) / 32 * 32) *reinterpret_cast<uint32_t*>(p.Q + ((t.first + r) * p.ldq + k0) / 2) = to_elements(v);
-            // a vector's four scales as one word; vectors and blocks that do not exist were read as zeros: s = 0
-            s <<= 8 * (part / 4);
-            s |= __shfl_xor_sync(0xffffffffu, s, 4);
-            s |= __shfl_xor_sync(0xffffffffu, s, 8);
-            if (part == 0) *reinterpret_cast<uint32_t*>(p.S + scale_at(q, kt, k_tile * 4, r)) = s;
-        }
         }
     }
 }
