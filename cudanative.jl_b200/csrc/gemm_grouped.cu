@@ -239,9 +239,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
     p.groups = static_cast<int>(g.groups);
-    p.tiles_m = static_cast<int>((g.M + 128 * pair - 1) / (128 * pair));
-    p.tiles_n = g.ragged_k ? static_cast<int>((g.N + tile_n - 1) / tile_n) : 0;
-    p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
+    const int64_t tiles_m = (g.M + 128 * pair - 1) / (128 * pair), tiles_n = (g.N + tile_n - 1) / tile_n;
     p.e.alpha = g.alpha;
     p.e.beta = g.beta;
     p.offsets = g.offsets;
@@ -276,9 +274,14 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     p.e.d_pairs = !(reinterpret_cast<uintptr_t>(g.D) & 3u) && g.ldd % 2 == 0 && g.stride_d % 2 == 0;
 
     // ragged N: at most one partial tile column per group that has columns
-    const int64_t cols = g.ragged_k ? g.groups * p.tiles_n : g.N / tile_n + std::min<int64_t>(g.groups, g.N);
-    const int64_t units = cols * p.tiles_m;
+    const int64_t cols = g.ragged_k ? g.groups * tiles_n : g.N / tile_n + std::min<int64_t>(g.groups, g.N);
+    const int64_t units = cols * tiles_m;
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "grouped gemm: too many tiles for one launch");
+    p.raster = Raster::of(h->raster_group > 0 ? h->raster_group : 8, static_cast<int>(tiles_m));
+    if (g.ragged_k) {
+        p.tiles_n = static_cast<int>(tiles_n);
+        p.tiles = Divisor::of(static_cast<int>(tiles_m * tiles_n));
+    }
     int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
     int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;
     if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here

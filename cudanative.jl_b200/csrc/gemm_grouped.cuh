@@ -31,11 +31,46 @@ namespace b200 {
 
 constexpr int kMaxGroups = 1024;
 
+// Division of 0 .. 2^31 - 1 by a number that the host knows, as a product: every role places every tile of its CTA,
+// three divisions one after the other (256 groups of 512 x 768, 1501 columns: 61 us with divisions, 57 so).
+// q = (high(n * mul) + n) >> shift with mul = floor(2^32 (2^shift - d) / d) + 1 and shift = ceil(log2 d) (Granlund
+// and Montgomery 1994); n + high(n * mul) stays below 2^32.
+struct Divisor {
+    uint32_t mul, shift;
+    int d;
+    __host__ static Divisor of(int d) {
+        uint32_t shift = 0;
+        while ((1ull << shift) < static_cast<unsigned long long>(d)) ++shift;
+        const unsigned long long mul = (((1ull << shift) - d) << 32) / d + 1;
+        return {static_cast<uint32_t>(mul), shift, d};
+    }
+};
+__device__ __forceinline__ int operator/(int n, const Divisor& v) {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), v.mul) + static_cast<uint32_t>(n)) >> v.shift);
+}
+
+// Tile rows are walked down inside bands of `band` rows: CTAs that run together share panels in L2.
+struct Raster {
+    Divisor band, rows;  // rows of all the tiles of a matrix
+    __host__ static Raster of(int band, int rows) { return {Divisor::of(band), Divisor::of(rows)}; }
+};
+// Row and column of tile `idx` of a matrix with `cols` columns of tiles.
+__device__ __forceinline__ int2 place_tile(const Raster& r, int idx, int cols) {
+    if (r.rows.d <= r.band.d) {
+        const int col = idx / r.rows;
+        return make_int2(idx - col * r.rows.d, col);
+    }
+    const int band = idx / (r.band.d * cols), row0 = band * r.band.d, in = idx - row0 * cols, rows = r.rows.d - row0;
+    const int col = rows >= r.band.d ? in / r.band : in / rows;
+    return make_int2(row0 + in - col * min(rows, r.band.d), col);
+}
+
 struct GroupedParams {
     int N, K;              // ragged N: N = columns of B, C, D; ragged K: K = columns of A and B
     int groups;
-    int tiles_m, tiles_n;  // tiles_n: ragged K only (tile columns of one D_e)
-    int raster_group;
+    int tiles_n;           // ragged K only (tile columns of one D_e)
+    Divisor tiles;         // ragged K only: tiles of one D_e
+    Raster raster;
     const int* offsets;
     int a_per_group;       // ragged N: 0 = one A for all groups
     int ab_bf16;
@@ -218,8 +253,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         p.status[2] = p.groups;
         __threadfence();
     }
-    const int tiles_per_group = p.tiles_m * p.tiles_n;  // ragged K
-    const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * tiles_per_group : first[p.groups] * p.tiles_m;
+    const int tiles_m = p.raster.rows.d;
+    const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * p.tiles.d : first[p.groups] * tiles_m;
 
     // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).
     SplitParams split;
@@ -248,21 +283,17 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
         Unit u;
         int idx, tn_count;
         if constexpr (kRaggedK) {
-            u.group = unit / tiles_per_group;
-            idx = unit - u.group * tiles_per_group;
+            u.group = unit / p.tiles;
+            idx = unit - u.group * p.tiles.d;
             tn_count = p.tiles_n;
         } else {
-            u.group = find_group(first, p.groups, unit / p.tiles_m);
-            idx = unit - first[u.group] * p.tiles_m;
+            u.group = find_group(first, p.groups, unit / p.raster.rows);
+            idx = unit - first[u.group] * tiles_m;
             tn_count = first[u.group + 1] - first[u.group];
         }
-        // walk down M inside bands of raster_group tile rows: CTAs that run together share panels in L2
-        const int band = idx / (p.raster_group * tn_count);
-        const int row0 = band * p.raster_group;
-        const int rows = min(p.raster_group, p.tiles_m - row0);
-        const int in = idx - band * p.raster_group * tn_count;
-        const int tn = in / rows;
-        u.m0 = (row0 + in - tn * rows) * (Cfg::BM * kCtas) + static_cast<int>(cta_rank) * Cfg::BM;
+        const int2 tile = place_tile(p.raster, idx, tn_count);
+        const int tn = tile.y;
+        u.m0 = tile.x * (Cfg::BM * kCtas) + static_cast<int>(cta_rank) * Cfg::BM;
         const int o0 = off[u.group], o1 = off[u.group + 1];
         if constexpr (kRaggedK) {
             u.n0 = tn * kBN;

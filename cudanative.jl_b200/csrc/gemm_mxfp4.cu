@@ -76,8 +76,8 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     p.N = static_cast<int>(g.N);
     p.K = static_cast<int>(g.K);
     p.groups = static_cast<int>(g.groups);
-    p.tiles_m = static_cast<int>((g.M + 128 * pair - 1) / (128 * pair));
-    p.raster_group = h->raster_group > 0 ? h->raster_group : 8;
+    const int64_t tiles_m = (g.M + 128 * pair - 1) / (128 * pair);
+    p.raster = Raster::of(h->raster_group > 0 ? h->raster_group : 8, static_cast<int>(tiles_m));
     p.offsets = g.offsets;
     p.a_per_group = g.stride_a != 0 ? 1 : 0;
     p.a_tile_rows = static_cast<int>((g.M + 127) / 128);
@@ -114,7 +114,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
         return encode_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
     };
     if ((rc = scale_map(&tm[2], g.SA, sa_rows, 1, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, (tile_n + 127) / 128, "scales of B"))) return rc;
-    const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * p.tiles_m;
+    const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * tiles_m;
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
     const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;
     int grid = static_cast<int>(std::min<int64_t>(std::max(cap / pair, 1), units)) * pair;

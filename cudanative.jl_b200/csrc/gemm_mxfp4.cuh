@@ -33,8 +33,7 @@ namespace b200 {
 struct MxGemmParams {
     int N, K;
     int groups;
-    int tiles_m;
-    int raster_group;
+    Raster raster;
     const int* offsets;  // nullptr: one group, all columns
     int a_per_group;
     int a_tile_rows;     // rows of scale tiles of one A_e
@@ -150,7 +149,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         p.status[2] = p.groups;
         __threadfence();
     }
-    const int num_units = offsets_ok ? first[p.groups] * p.tiles_m : 0;
+    const int num_units = offsets_ok ? first[p.groups] * p.raster.rows.d : 0;
 
     // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).
     SplitParams split;
@@ -175,16 +174,10 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 
     auto decode = [&](int unit) {
         Unit u;
-        u.group = find_group(first, p.groups, unit / p.tiles_m);
-        const int idx = unit - first[u.group] * p.tiles_m;
-        const int tn_count = first[u.group + 1] - first[u.group];
-        const int band = idx / (p.raster_group * tn_count);
-        const int row0 = band * p.raster_group;
-        const int rows = min(p.raster_group, p.tiles_m - row0);
-        const int in = idx - band * p.raster_group * tn_count;
-        const int tn = in / rows;
-        u.m0 = (row0 + in - tn * rows) * (Cfg::BM * kCtas) + static_cast<int>(cta_rank) * Cfg::BM;
-        u.n0 = off[u.group] + tn * kBN;
+        u.group = find_group(first, p.groups, unit / p.raster.rows);
+        const int2 tile = place_tile(p.raster, unit - first[u.group] * p.raster.rows.d, first[u.group + 1] - first[u.group]);
+        u.m0 = tile.x * (Cfg::BM * kCtas) + static_cast<int>(cta_rank) * Cfg::BM;
+        u.n0 = off[u.group] + tile.y * kBN;
         u.cols = min(kBN, off[u.group + 1] - u.n0);
         u.k0 = 0;
         u.k_len = p.K;
