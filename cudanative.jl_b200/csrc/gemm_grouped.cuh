@@ -489,11 +489,10 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     const int rem = u.k_len - (u.kb0 + kb1 - 1) * Cfg::BK, end = (rem + 15) / 16 * 16;
                     const int boxes = 2 + (inst_n(u) / kCtas + 63) / 64;  // A's two come first, B's follow
                     uint8_t* tile = smem_gen + st * Cfg::STAGE_BYTES;
-                    for (int i = lane; i < boxes * (end - rem) * 8; i += 32) {
-                        const int box = i / ((end - rem) * 8), in = i - box * ((end - rem) * 8);
-                        *reinterpret_cast<uint4*>(tile + box * 8192 + (rem + in / 8) * 128 + (in & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async;" ::: "memory");
+                    for (int box = 0; box < boxes; ++box)
+                    for (int row = rem + lane / 8; row < end; row += 4)
+                        *reinterpret_cast<uint4*>(tile + box * 8192 + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
                         if constexpr (kPair) mbar_arrive_cluster(tail_ready_bar(st), 0);
