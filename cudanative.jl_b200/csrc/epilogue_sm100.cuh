@@ -10,6 +10,10 @@
 // for bulk stores took two barriers, a proxy fence and a copy's issue per 16 columns, 750 cycles (1 300 with C)
 // where the stores themselves take about 100; it also cost 48 KiB of the ring.  Any M, leading dimension and
 // alignment take the same path.
+// With one k-block per tile the instructions of these warps are the bound: one uniform branch per 32 columns on the
+// format and addresses that move on by addition took 256 groups of 512 x 768, 16 columns each, from 53 to 48 us
+// (bfloat16 D; 42 us for the stores alone) and from 81 to 77 us (Float32).  All of a tile's accumulator at once, its four steps
+// unrolled, was slower (70 us).
 //
 // C is read the same way: before it waits for the accumulator the warp brings the tile's lines of C into L2 and
 // asks for the first step's values, then for each next step's while one is stored (where the registers
@@ -192,14 +196,23 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
                 if (kAhead && (j + 1) * W < cols) load_c(j + 1);
             } else {
 #pragma unroll
-                for (int i = 0; i < W; ++i) r[i] = __float_as_uint(alpha * __uint_as_float(r[i]));
+                for (int i = 0; i < W; i += 2) {
+                    if constexpr (kF32) {
+                        r[i] = __float_as_uint(alpha * __uint_as_float(r[i]));
+                        r[i + 1] = __float_as_uint(alpha * __uint_as_float(r[i + 1]));
+                    } else {
+                        const float2 x = __fmul2_rn(make_float2(alpha, alpha), make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+                        r[i] = __float_as_uint(x.x);
+                        r[i + 1] = __float_as_uint(x.y);
+                    }
+                }
             }
             const long long at = (kPerGroup ? u.group * p.stride_d : 0) + m + n * p.ldd;
             if (d_fmt == 0) {
                 float* d = static_cast<float*>(p.D) + at;
                 if (whole_rows && left >= W) {
 #pragma unroll
-                    for (int i = 0; i < W; ++i) d[i * p.ldd] = __uint_as_float(r[i]);
+                    for (int i = 0; i < W; ++i, d += p.ldd) *d = __uint_as_float(r[i]);
                 } else if (m < p.M) {
 #pragma unroll
                     for (int i = 0; i < W; ++i)
@@ -209,12 +222,15 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             }
             if constexpr (!kF32) {
                 uint32_t v[W / 2];  // columns 2 i and 2 i + 1, rounded
+                if (d_fmt == 2) {
 #pragma unroll
-                for (int i = 0; i < W; i += 2) {
-                    if (d_fmt == 2) {
+                    for (int i = 0; i < W; i += 2) {
                         const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
                         v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                    } else {
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; i += 2) {
                         const __half2 h = __floats2half2_rn(__uint_as_float(r[i]), __uint_as_float(r[i + 1]));
                         v[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
                     }
@@ -228,7 +244,8 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
 #pragma unroll
                     for (int i = 0; i < W; i += 2) {
                         const uint32_t x = __shfl_xor_sync(0xffffffffu, v[i / 2], 1);
-                        *reinterpret_cast<uint32_t*>(d + i * p.ldd) = __byte_perm(v[i / 2], x, pick);
+                        *reinterpret_cast<uint32_t*>(d) = __byte_perm(v[i / 2], x, pick);
+                        d += 2 * p.ldd;
                     }
                 } else if (m < p.M) {
 #pragma unroll
