@@ -550,3 +550,39 @@ def test_few_tiles_share_the_inner_dimension(handle, d_type, transA):
         run_grouped(handle, sizes, M, K, transA=transA, d_type=d_type, beta=0.5, c_type=F32, start=1, tail=2)
         assert handle.last_launch()["split_k"] == 4
     run_grouped(handle, [70], 71, 2056, d_type=d_type, expect=_lib.KERNEL_TCGEN05)
+
+
+@pytest.mark.parametrize("band", [1, 2, 3, 5, 64])
+@pytest.mark.parametrize("tile_n,cta_pair", [(64, 1), (128, 1), (256, 2)])
+def test_tile_rows_in_bands(handle, band, tile_n, cta_pair):
+    """Every tile is placed once, with one band, whole bands and a last band of fewer rows."""
+    handle.set_option(_lib.OPT_RASTER_GROUP, band)
+    run_grouped(handle, [70, 0, 300, 513, 1], 1416, 72, tile_n=tile_n, cta_pair=cta_pair, tail=3)
+    run_grouped_k(handle, [70, 0, 33], 1416, 328, tile_n=tile_n, cta_pair=cta_pair)
+    handle.set_option(_lib.OPT_MAX_CTAS, 6)
+    run_grouped(handle, [70, 0, 300, 513, 1], 1416, 72, tile_n=tile_n, cta_pair=cta_pair, tail=3)
+
+
+def test_shared_sums_of_poisoned_neighbours_repeat_bitwise(handle):
+    """Four CTAs to a tile: a group whose operands are NaN keeps them to itself, and the same call gives the same bits."""
+    r = np.random.default_rng(5)
+    sizes, M, N = [5003, 64, 0, 4090], 72, 136
+    off = offsets_of(sizes, 0)
+    K, E = int(off[-1]), len(sizes)
+    A, B = store(normal(r, (M, K)), BFloat16), store(normal(r, (N, K)), BFloat16)
+    for x in (A, B):
+        x[:, off[1]:off[2]] = fill_of(BFloat16, np.nan)
+    a_dev, b_dev, o_dev = CuArray(np.asfortranarray(A)), CuArray(np.asfortranarray(B)), CuArray(off)
+    got = []
+    for _ in range(3):
+        d_dev = CuArray(np.full(M * N * E, 7.0, np.float32))
+        handle.gemm_grouped_k(M, N, K, 1.0, a_dev, M, b_dev, N, BFloat16, 0.0, None, M, M * N, F32, d_dev, M, M * N, F32, o_dev, E)
+        sync(handle)
+        assert handle.last_launch()["split_k"] == 4
+        got.append(Array(d_dev).reshape(E, N, M).transpose(0, 2, 1))
+    assert got[0].tobytes() == got[1].tobytes() == got[2].tobytes()
+    assert np.isnan(got[0][1]).all() and not got[0][2].any()
+    a, b = value(A, BFloat16), value(B, BFloat16)
+    for e in (0, 3):
+        s = slice(off[e], off[e + 1])
+        close(got[0][e], a[:, s] @ b[:, s].T, np.abs(a[:, s]) @ np.abs(b[:, s]).T, sizes[e], F32, f"group {e}")

@@ -275,3 +275,12 @@ def test_the_exponent_range_of_the_scales(handle):
     assert np.array_equal(got[normal], exact[normal])
     assert np.all(np.isinf(got[exact >= 2.0 ** 128]))
     assert np.all(got[exact < 2.0 ** -126] <= 2.0 ** -120)
+
+
+@pytest.mark.parametrize("band", [1, 2, 3, 5, 64])
+@pytest.mark.parametrize("tile_n", [0, 128, 256])
+def test_tile_rows_in_bands(handle, band, tile_n):
+    """Every tile is placed once, with one band, whole bands and a last band of fewer rows."""
+    handle.set_option(_lib.OPT_RASTER_GROUP, band)
+    run_product(handle, 1416, 96, [70, 0, 300, 513, 1], tile_n=tile_n, tail=3)
+    run_product(handle, 1416, 1056, [520], grouped=False, tile_n=tile_n, d_type=F32, beta=1.0)
