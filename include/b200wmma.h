@@ -210,7 +210,9 @@ int b200_gemm_strided_batched(b200_handle* h, b200_stream stream, int transA, in
  * The tcgen05 kernel needs 16-byte aligned A and B, lda, ldb and stride_a multiples of 8 elements and
  * stride_a at least one matrix (or 0); anything else runs on the simple kernel.  C and D may have any
  * alignment.  A binary32 D on the tcgen05 kernel sums several accumulators, each of 512 products, with
- * rounding to nearest.  The split-K option is ignored. */
+ * rounding to nearest; so does any D where tiles are few and K is long: four CTAs share a tile's K then
+ * (b200_last_launch reports split_k 4) and their sums are added in a fixed order.  The split-K option is
+ * ignored. */
 int b200_gemm_grouped(b200_handle* h, b200_stream stream, int transA, int64_t M, int64_t N, int64_t K,
                       float alpha, const void* A, int64_t lda, int64_t stride_a, const void* B,
                       int64_t ldb, int ab_type, float beta, const void* C, int64_t ldc, int c_type,
