@@ -200,16 +200,44 @@ bool eligible(const Grouped& g, std::string* why) {
     return true;
 }
 
+// How many clusters of four CTAs the current device holds at once: fewer than SMs / 4, since a cluster lies within one
+// part of the chip and those have no multiple of four SMs (33 of 37 on a B200).
+int resident_clusters(int* clusters) {
+    static std::atomic<int> known[64];  // per device
+    int dev = 0;
+    B200_CUDA_TRY(cudaGetDevice(&dev));
+    *clusters = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (*clusters > 0) return B200_OK;
+    auto kern = gemm_grouped_tcgen05<64, true, true, 1, true, 4>;
+    using Cfg = GroupedCfg<64, true, 1, true, 4>;
+    B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 4;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(4, 1, 1);
+    cfg.blockDim = dim3(Cfg::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    B200_CUDA_TRY(cudaOccupancyMaxActiveClusters(clusters, kern, &cfg));
+    if (dev < 64) known[dev].store(*clusters, std::memory_order_relaxed);
+    return B200_OK;
+}
+
 // Few tiles and a long inner dimension: clusters of four CTAs share each tile's K (64-column tiles).  Measured, whole tiles
-// against shared ones: one round of clusters (at most SMs / 4 tiles) with K = 2048 12-17 / 11-13 us, K = 1024 8-12 /
-// 10-12 us; two rounds with K = 4096 28 / 28 us, K = 16384 88 / 52 us.
-bool shares_k(const b200_handle* h, const Grouped& g) {
+// against shared ones: one round of clusters (33 tiles) with K = 2048 14.2 / 12.6 us, K = 4096 23.6 / 14.6 us, K =
+// 1024 8-12 / 10-12 us; two rounds (64 tiles) with K = 4096 28 / 28 us, K = 8192 43.5 / 35.6 us; three 44 / 44 us.
+bool may_share_k(const b200_handle* h, const Grouped& g) {
     if (h->tile_n != 0 || h->cta_pair != 0 || h->max_ctas != 0) return false;
-    const int64_t cols = g.ragged_k ? g.groups * ((g.N + 63) / 64) : g.N / 64 + std::min(g.groups, g.N);
-    const int64_t units = cols * ((g.M + 127) / 128), clusters = h->sm_count / 4;
-    const int64_t k = g.ragged_k ? g.K / g.groups : g.K;
     if (!g.ragged_k && g.N <= 32 * g.groups) return false;  // 32-column tiles, in pairs
-    return (units <= clusters && k >= 2048) || (units <= 2 * clusters && k >= 8192);
+    return (g.ragged_k ? g.K / g.groups : g.K) >= 2048;
+}
+bool shares_k(const Grouped& g, int clusters) {
+    const int64_t cols = g.ragged_k ? g.groups * ((g.N + 63) / 64) : g.N / 64 + std::min(g.groups, g.N);
+    const int64_t units = cols * ((g.M + 127) / 128), k = g.ragged_k ? g.K / g.groups : g.K;
+    return units <= clusters || (units <= 2 * clusters && k >= 8192);
 }
 
 // Tile columns.  Ragged N: the sizes of the groups are not known here, their mean is.  Wide tiles read
@@ -229,7 +257,12 @@ void pick_tile(const b200_handle* h, const Grouped& g, int* tile_n, int* pair) {
 int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     int tile_n, pair, rc;
     pick_tile(h, g, &tile_n, &pair);
-    const bool share = shares_k(h, g);
+    bool share = may_share_k(h, g);
+    int clusters = 0;
+    if (share) {
+        if ((rc = resident_clusters(&clusters))) return rc;
+        share = shares_k(g, clusters);
+    }
     if (share) {
         tile_n = 64;
         pair = 1;
@@ -287,7 +320,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     if (tile_n == 32) grid = std::max(cap / 2, 1) * 2;  // pairs of CTAs; how many tiles there are is not known here
     const bool pdl = h->pdl != 0;
     if (share) {
-        grid = static_cast<int>(std::min<int64_t>(std::max(cap / 4, 1), units)) * 4;
+        grid = static_cast<int>(std::min<int64_t>(clusters, units)) * 4;
         if (g.ragged_k) rc = launch_promote<64, true, true, 1, true, 4>(tm, p, grid, stream, pdl);
         else if (g.transA) rc = launch_promote<64, false, false, 1, true, 4>(tm, p, grid, stream, pdl);
         else rc = launch_promote<64, true, false, 1, true, 4>(tm, p, grid, stream, pdl);

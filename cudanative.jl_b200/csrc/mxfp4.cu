@@ -122,7 +122,8 @@ __device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off
 
 // Vectors whose values are contiguous.  A tile is 128 vectors x 128 values: 16 lanes take a vector's 128, eight
 // values (16 bytes of a 16-bit type) each, so that a warp reads and writes whole lines; four lanes find a
-// block's largest magnitude with two shuffles.  A thread has four vectors in flight.
+// block's largest magnitude with two shuffles.  A thread has four vectors in flight, four blocks share an SM: Float16
+// 16384 x 2048 19.0 us (4.5 TB/s; three blocks 20.6, five 20.3; eight vectors and three blocks 22.7).
 template <typename T>
 __global__ void __launch_bounds__(256, 4) mxfp4_quantize_kernel(const MxParams p) {
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];

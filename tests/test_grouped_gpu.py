@@ -586,3 +586,16 @@ def test_shared_sums_of_poisoned_neighbours_repeat_bitwise(handle):
     for e in (0, 3):
         s = slice(off[e], off[e + 1])
         close(got[0][e], a[:, s] @ b[:, s].T, np.abs(a[:, s]) @ np.abs(b[:, s]).T, sizes[e], F32, f"group {e}")
+
+
+def test_shared_sums_stay_within_one_round_of_clusters(handle):
+    """A device holds fewer clusters of four than a quarter of its SMs: tiles beyond those would run a round later."""
+    run_grouped_k(handle, [2100], 128, 64 * 30)
+    assert handle.last_launch()["split_k"] == 4
+    for cols in (35, 37, 72):
+        run_grouped_k(handle, [2100], 128, 64 * cols)
+        launch = handle.last_launch()
+        assert launch["split_k"] == 1 or launch["ctas"] >= 4 * cols
+    run_grouped_k(handle, [8200], 128, 64 * 60)
+    launch = handle.last_launch()
+    assert launch["split_k"] == 1 or launch["ctas"] * 2 >= 4 * 60
