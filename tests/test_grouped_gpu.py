@@ -599,3 +599,14 @@ def test_shared_sums_stay_within_one_round_of_clusters(handle):
     run_grouped_k(handle, [8200], 128, 64 * 60)
     launch = handle.last_launch()
     assert launch["split_k"] == 1 or launch["ctas"] * 2 >= 4 * 60
+
+
+@pytest.mark.parametrize("d_type", [BFloat16, F32])
+def test_shared_sums_in_two_and_three_rounds(handle, d_type):
+    """The buffers that the four CTAs send to are used again for the next tile."""
+    for K, tiles in ((4100, 50), (8200, 90)):
+        run_grouped_k(handle, [K], 128, 64 * tiles, d_type=d_type, beta=1.0)
+        launch = handle.last_launch()
+        assert launch["split_k"] == 4 or launch["ctas"] * 3 < 4 * tiles
+        run_grouped(handle, [64 * tiles - 64], 128, K + 4, d_type=d_type)
+        run_grouped_k(handle, [K // 2, K // 2 + K % 2 + 1, K, K - 3], 128, 16 * tiles // 64 * 64, d_type=d_type)
