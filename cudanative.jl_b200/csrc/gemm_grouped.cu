@@ -228,18 +228,19 @@ int resident_clusters(int* clusters) {
 
 // Few tiles and a long inner dimension: clusters of four CTAs share each tile's K (64-column tiles), in as many rounds as
 // the clusters that the device holds need.  Measured, whole tiles against shared ones, the last number of tiles of each
-// round: one round K = 1024 9.3 / 11.5 us, K = 1536 11.8 / 12.1, K = 2048 14.2 / 12.6; two rounds K = 3000 19.0 / 19.1, K =
+// round: one round K = 1024 9.3 / 11.5 us, K = 1536 11.8 / 12.1 (16 tiles 11.8 / 10.5), K = 2048 14.2 / 12.6; two rounds K = 3000 19.0 / 19.1, K =
 // 4096 23.8 / 20.1; three K = 4096 23.9 / 26.2, K = 6000 34.2 / 33.6, K = 8192 46.3 / 42.7; four K = 16384 87.8 / 90.0.
+// Ragged K: by the mean length; a longer group than the others takes more from whole tiles than from shared ones.
 bool may_share_k(const b200_handle* h, const Grouped& g) {
     if (h->tile_n != 0 || h->cta_pair != 0 || h->max_ctas != 0) return false;
     if (!g.ragged_k && g.N <= 32 * g.groups) return false;  // 32-column tiles, in pairs
-    return (g.ragged_k ? g.K / g.groups : g.K) >= 2048;
+    return (g.ragged_k ? g.K / g.groups : g.K) >= 1536;
 }
 bool shares_k(const Grouped& g, int clusters) {
     const int64_t cols = g.ragged_k ? g.groups * ((g.N + 63) / 64) : g.N / 64 + std::min(g.groups, g.N);
     const int64_t units = cols * ((g.M + 127) / 128), k = g.ragged_k ? g.K / g.groups : g.K;
     const int64_t rounds = (units + clusters - 1) / std::max(clusters, 1);
-    return clusters > 0 && rounds <= 3 && k >= int64_t(2048) << (rounds - 1);
+    return clusters > 0 && rounds <= 3 && k >= (rounds == 1 ? 1536 : int64_t(2048) << (rounds - 1));
 }
 
 // Tile columns.  Ragged N: the sizes of the groups are not known here, their mean is.  Wide tiles read
