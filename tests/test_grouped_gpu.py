@@ -610,3 +610,47 @@ def test_shared_sums_in_two_and_three_rounds(handle, d_type):
         assert launch["split_k"] == 4 or launch["ctas"] * 3 < 4 * tiles
         run_grouped(handle, [64 * tiles - 64], 128, K + 4, d_type=d_type)
         run_grouped_k(handle, [K // 2, K // 2 + K % 2 + 1, K, K - 3], 128, 16 * tiles // 64 * 64, d_type=d_type)
+
+
+def test_shared_sums_first_called_inside_a_capture():
+    """The device is asked for its clusters by the first call that may share K, a captured one too; two captured calls
+    replayed at once on two streams share nothing."""
+    pytest.importorskip("torch")
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import torch, numpy as np, __graft_entry__ as e
+e.load_package()
+from cudanative_jl_b200.gemm import Handle
+from cudanative_jl_b200.bfloat16 import BFloat16
+h = Handle(0)
+T, M, N = 5000, 136, 264
+off = torch.tensor([0, 1703, 5000], dtype=torch.int32, device="cuda")
+xs, ys = [torch.randn(T, M, device="cuda").bfloat16() for _ in range(2)], [torch.randn(T, N, device="cuda").bfloat16() for _ in range(2)]
+ds, gs, streams = [torch.zeros(2, N, M, device="cuda") for _ in range(2)], [], [torch.cuda.Stream() for _ in range(2)]
+torch.cuda.synchronize()
+for x, y, d, s in zip(xs, ys, ds, streams):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        for _ in range(3):
+            h.gemm_grouped_k(M, N, T, 1.0, x, M, y, N, BFloat16, 0.0, None, M, 0, np.float32, d, M, M * N, np.float32, off, 2,
+                             stream=torch.cuda.current_stream().cuda_stream)
+    assert h.last_launch()["split_k"] == 4
+    gs.append(g)
+for _ in range(5):
+    for g, s in zip(gs, streams):
+        with torch.cuda.stream(s):
+            g.replay()
+torch.cuda.synchronize()
+for x, y, d in zip(xs, ys, ds):
+    x, y = x.double(), y.double()
+    ref = torch.stack([y[:1703].T @ x[:1703], y[1703:].T @ x[1703:]])
+    assert (d.double() - ref).norm() < 1e-5 * ref.norm()
+assert h.device_status()[0] == 0
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
