@@ -86,9 +86,11 @@ class Handle:
     # -- device pointers ---------------------------------------------------------------------
     def gemm(self, transA: bool, transB: bool, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int,
              beta: float, Cm, ldc: int, D, ldd: int, stream=None) -> None:
-        """Raw form: A, B, C, D are device addresses (ints), DevicePtr, CuHostArray or CUDA tensors."""
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        """Raw form: A, B, C, D are device addresses (ints), DevicePtr, CuHostArray or CUDA tensors.  What has an
+        element type must have the one that is read: Float16 A and B, Float32 C and D; an address is taken as it is,
+        and so is a C that beta = 0 leaves unread."""
+        a, b = _addr(A, np.float16, "A"), _addr(B, np.float16, "B")
+        c, d = _addr(Cm, np.float32 if beta else None, "C"), _addr(D, np.float32, "D")
         _lib.check(_lib.lib().b200_gemm_f16f32(self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K,
                                                float(alpha), a, lda, b, ldb, float(beta), c, ldc, d, ldd), "gemm")
 
@@ -96,8 +98,10 @@ class Handle:
                    beta: float, Cm, ldc: int, c_type, D, ldd: int, d_type, stream=None) -> None:
         """``gemm`` with Float16 or Float32 C and D (b200_gemm_f16_typed); types are numpy dtypes."""
         code = {np.dtype(np.float16): _lib.F16, np.dtype(np.float32): _lib.F32}
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        if np.dtype(c_type) not in code or np.dtype(d_type) not in code:
+            raise TypeError("gemm_typed: C and D must be Float16 or Float32")
+        a, b = _addr(A, np.float16, "A"), _addr(B, np.float16, "B")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_f16_typed(self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K,
                                                   float(alpha), a, lda, b, ldb, float(beta), c, ldc, code[np.dtype(c_type)],
                                                   d, ldd, code[np.dtype(d_type)]), "gemm_typed")
@@ -114,8 +118,8 @@ class Handle:
                              stride_c: int, c_type, D, ldd: int, stride_d: int, d_type, batch: int, stream=None) -> None:
         """``batch`` products of one shape, matrix i of X starting ``stride_x * i`` elements after X
         (b200_gemm_strided_batched); a stride of 0 repeats A, B or C."""
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        a, b = _addr(A, ab_type, "A"), _addr(B, ab_type, "B")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_strided_batched(
             self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K, float(alpha), a, lda, stride_a, b, ldb,
             stride_b, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type), d, ldd, stride_d,
@@ -177,11 +181,12 @@ class Handle:
                    beta: float, Cm, ldc: int, D, ldd: int, panel_flags, panel_k: int, stream=None) -> None:
         """``gemm`` whose main loop reads columns [j*panel_k, (j+1)*panel_k) of op(A) only once the
         32-bit device word ``panel_flags[j]`` is non-zero (b200_gemm_f16f32_gated)."""
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        a, b = _addr(A, np.float16, "A"), _addr(B, np.float16, "B")
+        c, d = _addr(Cm, np.float32 if beta else None, "C"), _addr(D, np.float32, "D")
         _lib.check(_lib.lib().b200_gemm_f16f32_gated(self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K,
                                                      float(alpha), a, lda, b, ldb, float(beta), c, ldc, d, ldd,
-                                                     _addr(panel_flags), panel_k), "gemm_gated")
+                                                     _addr(panel_flags, (np.uint32, np.int32), "panel_flags"), panel_k),
+                   "gemm_gated")
 
     # -- host buffers (numpy, ideally page-locked) ---------------------------------------------
     def gemm_host(self, transA: bool, transB: bool, M: int, N: int, K: int, alpha: float, A: np.ndarray, lda: int,
@@ -202,12 +207,25 @@ def mxfp4_scale_bytes(K: int, cols: int, groups: int = 0) -> int:
     return _lib.lib().b200_mxfp4_scale_bytes(K, cols, groups)
 
 
-def _addr(x):
+# numpy dtype in which the owner of an operand (CuHostArray, DevicePtr, tensor) reports an element type
+_STORED = {_lib.F16: np.dtype(np.float16), _lib.F32: np.dtype(np.float32), _lib.BF16: np.dtype(np.uint16)}
+
+
+def _addr(x, elem=None, what: str = "operand"):
+    """Device address of an operand whose elements the library reads as ``elem``: an element type (Float16, Float32 or the
+    ``BFloat16`` tag, which lies in memory as uint16 patterns) or a tuple of the numpy types that may stand there.  A typed
+    operand of another type is refused; None and plain addresses have no type to compare."""
     if x is None:
         return None
     if isinstance(x, int):
         return x
-    return DevicePtr.of(x).addr
+    p = DevicePtr.of(x)
+    if elem is not None:
+        ok = [np.dtype(t) for t in elem] if isinstance(elem, tuple) else [_STORED[_type_code(elem)]]
+        if p.dtype not in ok:
+            raise TypeError(f"{what}: expected {' or '.join(t.name for t in ok)} elements" +
+                            (" (bfloat16 bit patterns)" if elem is BFloat16 else "") + f", got {p.dtype.name}")
+    return p.addr
 
 
 def _dtype(x) -> np.dtype:
@@ -363,13 +381,14 @@ class ShardedGemm:
     def run(self, alpha: float, B_slab, beta: float, C_slab, D_slab, *, stream=None, gated: bool = False,
             no_transfer: bool = False, no_compute: bool = False, ldb: int | None = None, ldc: int | None = None, ldd: int | None = None) -> None:
         """Enqueue one product (b200_sharded_run).  B_slab: K x slab_cols, C_slab / D_slab: M x
-        slab_cols, column-major device matrices (addresses, DevicePtr, CuHostArray or CUDA tensors).
+        slab_cols, column-major device matrices (addresses, DevicePtr, CuHostArray or CUDA tensors); B
+        is Float16, C and D are Float32.
         Every rank must make the call, also one whose slab is empty."""
         flags = ((_lib.SHARDED_GATED if gated else 0) | (_lib.SHARDED_NO_TRANSFER if no_transfer else 0) |
                  (_lib.SHARDED_NO_COMPUTE if no_compute else 0))
-        _lib.check(_lib.lib().b200_sharded_run(self._s, stream, float(alpha), _addr(B_slab), ldb or self.K, float(beta),
-                                               _addr(C_slab) if C_slab is not None else None, ldc or self.M,
-                                               _addr(D_slab), ldd or self.M, flags), "sharded_run")
+        _lib.check(_lib.lib().b200_sharded_run(self._s, stream, float(alpha), _addr(B_slab, np.float16, "B_slab"), ldb or self.K,
+                                               float(beta), _addr(C_slab, np.float32 if beta else None, "C_slab"), ldc or self.M,
+                                               _addr(D_slab, np.float32, "D_slab"), ldd or self.M, flags), "sharded_run")
 
     def wait(self, timeout_ms: int = 60000) -> None:
         """Host-side wait with a deadline (b200_sharded_wait): raises B200Error with status

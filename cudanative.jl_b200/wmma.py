@@ -430,6 +430,8 @@ def wmma_16x16x16(a, b, c, d, *, a_layout=ColMajor, b_layout=ColMajor, c_layout=
     pc = DevicePtr.of(c) if c is not None else None
     if pa.dtype != np.float16 or pb.dtype != np.float16:
         raise ValueError("Invalid element type for WMMA: a and b must be Float16")
+    if pd.dtype not in _TYPE_CODE or (pc is not None and pc.dtype not in _TYPE_CODE):
+        raise ValueError("Invalid element type for WMMA: c and d must be Float16 or Float32")
     c_type = _TYPE_CODE[pc.dtype] if pc is not None else _TYPE_CODE[pd.dtype]
     _lib.check(_lib.lib().b200_wmma_16x16x16(
         stream, lowering, _layout_code(a_layout), _layout_code(b_layout), _layout_code(c_layout),

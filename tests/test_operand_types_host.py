@@ -1,0 +1,129 @@
+"""Element types of the operands that the Python entry points are given: an operand whose owner knows its type (a tensor, a
+device array) has to have the one that the library reads.  No GPU: the tensors are stand-ins, and a refused call reaches
+no entry point of the library."""
+import numpy as np
+import pytest
+
+from cudanative_jl_b200 import gemm as G
+from cudanative_jl_b200 import wmma
+from cudanative_jl_b200.array import DevicePtr
+from cudanative_jl_b200.bfloat16 import BFloat16
+
+torch = pytest.importorskip("torch")
+
+F16, F32 = np.float16, np.float32
+
+
+class Tensor:
+    """What the package asks of a tensor on the device."""
+
+    is_cuda = True
+
+    def __init__(self, dtype, rows=16, cols=16):
+        self.dtype, self.shape = dtype, (cols, rows)
+
+    def data_ptr(self):
+        return 4096
+
+    def stride(self, i):
+        return (self.shape[1], 1)[i]
+
+
+class Library:
+    """Notes the entry points that are called; all of them succeed."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture()
+def library(monkeypatch):
+    lib = Library()
+    monkeypatch.setattr(G._lib, "lib", lambda: lib)
+    return lib
+
+
+def handle():
+    h = G.Handle.__new__(G.Handle)
+    h._h, h.device = None, 0
+    return h
+
+
+def sharded():
+    s = G.ShardedGemm.__new__(G.ShardedGemm)
+    s._s, s.M, s.K = None, 16, 16
+    return s
+
+
+h16, f32, b16, u8, i32 = torch.float16, torch.float32, torch.bfloat16, torch.uint8, torch.int32
+
+# entry point -> (call with operands by name, the types it reads)
+ENTRIES = {
+    "gemm": (lambda t: handle().gemm(False, False, 16, 16, 16, 1.0, t["A"], 16, t["B"], 16, 1.0, t["C"], 16, t["D"], 16), dict(A=h16, B=h16, C=f32, D=f32)),
+    "gemm_gated": (lambda t: handle().gemm_gated(False, False, 16, 16, 16, 1.0, t["A"], 16, t["B"], 16, 1.0, t["C"], 16, t["D"], 16, t["flags"], 64),
+                   dict(A=h16, B=h16, C=f32, D=f32, flags=i32)),
+    "gemm_typed": (lambda t: handle().gemm_typed(False, False, 16, 16, 16, 1.0, t["A"], 16, t["B"], 16, 1.0, t["C"], 16, F16, t["D"], 16, F32),
+                   dict(A=h16, B=h16, C=h16, D=f32)),
+    "gemm_f16f32": (lambda t: G.gemm_f16f32(handle(), t["D"], t["A"], t["B"], t["C"], beta=1.0), dict(A=h16, B=h16, C=f32, D=f32)),
+    "gemm_ex": (lambda t: handle().gemm_ex(False, False, 16, 16, 16, 1.0, t["A"], 16, t["B"], 16, BFloat16, 1.0, t["C"], 16, F16, t["D"], 16, BFloat16),
+                dict(A=b16, B=b16, C=h16, D=b16)),
+    "gemm_strided_batched": (lambda t: handle().gemm_strided_batched(False, False, 16, 16, 16, 1.0, t["A"], 16, 256, t["B"], 16, 256, F16, 1.0, t["C"], 16, 256, F32,
+                                                                     t["D"], 16, 256, F16, 2), dict(A=h16, B=h16, C=f32, D=h16)),
+    "ShardedGemm.run": (lambda t: sharded().run(1.0, t["B"], 1.0, t["C"], t["D"]), dict(B=h16, C=f32, D=f32)),
+}
+# gemm_f16f32 takes the types of C and D from the operands
+FREE = {("gemm_f16f32", "C"): (h16, f32), ("gemm_f16f32", "D"): (h16, f32)}
+
+
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_the_right_types_reach_the_library(library, entry):
+    call, types = ENTRIES[entry]
+    call({k: Tensor(t) for k, t in types.items()})
+    assert len(library.calls) == 1
+
+
+@pytest.mark.parametrize("entry,operand", [(e, o) for e, (_, types) in ENTRIES.items() for o in types])
+@pytest.mark.parametrize("wrong", [h16, f32, b16, u8, i32, torch.int64, torch.float64], ids=str)
+def test_another_type_is_refused(library, entry, operand, wrong):
+    call, types = ENTRIES[entry]
+    if wrong in FREE.get((entry, operand), (types[operand],)):
+        pytest.skip("a type it reads")
+    with pytest.raises(TypeError):
+        call({**{k: Tensor(t) for k, t in types.items()}, operand: Tensor(wrong)})
+    assert not library.calls
+
+
+@pytest.mark.parametrize("entry", ENTRIES)
+def test_addresses_and_typed_pointers(library, entry):
+    """An address has no type; a DevicePtr has one, bfloat16 being its bit patterns."""
+    call, types = ENTRIES[entry]
+    stored = {h16: F16, f32: F32, b16: np.uint16, i32: np.int32}
+    call({k: DevicePtr(stored[t], 4096) if entry != "gemm_f16f32" else Tensor(t) for k, t in types.items()})
+    if entry != "gemm_f16f32":
+        call({k: 4096 for k in types})
+        with pytest.raises(TypeError):
+            call({k: DevicePtr(np.uint8, 4096) for k in types})
+
+
+def test_a_c_that_is_not_read_has_any_type(library):
+    handle().gemm(False, False, 16, 16, 16, 1.0, Tensor(h16), 16, Tensor(h16), 16, 0.0, Tensor(h16), 16, Tensor(f32), 16)
+    assert len(library.calls) == 1
+
+
+def test_the_16x16x16_unit_refuses_other_types(library):
+    for c, d in ((Tensor(u8), Tensor(f32)), (Tensor(f32), Tensor(i32)), (None, Tensor(b16))):
+        with pytest.raises(ValueError, match="Invalid element type"):
+            wmma.wmma_16x16x16(Tensor(h16), Tensor(h16), c, d)
+    with pytest.raises(ValueError, match="Invalid element type"):
+        wmma.wmma_16x16x16(Tensor(b16), Tensor(h16), None, Tensor(f32))
+    assert not library.calls
