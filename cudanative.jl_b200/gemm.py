@@ -21,6 +21,7 @@ from .array import CuHostArray, DevicePtr
 from .bfloat16 import BFloat16
 
 
+_BYTES, _OFFSETS = (np.uint8,), (np.int32,)  # 4-bit elements and scales; group borders
 _TYPE_CODES = {BFloat16: _lib.BF16, np.float16: _lib.F16, np.float32: _lib.F32}
 
 
@@ -130,52 +131,58 @@ class Handle:
         """``D[:, s_e] = alpha*op(A_e)*B[:, s_e] + beta*C[:, s_e]`` for the columns ``s_e`` of every group, whose
         borders are ``groups + 1`` int32 on the device (b200_gemm_grouped): a layer with one weight matrix per
         group (transA) or the gradient of its input."""
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        a, b = _addr(A, ab_type, "A"), _addr(B, ab_type, "B")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_grouped(
             self._h, stream, int(bool(transA)), M, N, K, float(alpha), a, lda, stride_a, b, ldb, _type_code(ab_type), float(beta), c,
-            ldc, _type_code(c_type), d, ldd, _type_code(d_type), _addr(offsets), groups), "gemm_grouped")
+            ldc, _type_code(c_type), d, ldd, _type_code(d_type), _addr(offsets, _OFFSETS, "offsets"), groups), "gemm_grouped")
 
     def gemm_grouped_k(self, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int, ab_type, beta: float, Cm, ldc: int,
                        stride_c: int, c_type, D, ldd: int, stride_d: int, d_type, offsets, groups: int, stream=None) -> None:
         """``D_e = alpha*A[:, s_e]*B[:, s_e]^T + beta*C_e`` (b200_gemm_grouped_k): the gradient of the groups'
         matrices; an empty group gives ``beta*C_e``."""
-        a, b, d = _addr(A), _addr(B), _addr(D)
-        c = _addr(Cm) if Cm is not None else None
+        a, b = _addr(A, ab_type, "A"), _addr(B, ab_type, "B")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_grouped_k(
             self._h, stream, M, N, K, float(alpha), a, lda, b, ldb, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type),
-            d, ldd, stride_d, _type_code(d_type), _addr(offsets), groups), "gemm_grouped_k")
+            d, ldd, stride_d, _type_code(d_type), _addr(offsets, _OFFSETS, "offsets"), groups), "gemm_grouped_k")
 
     def mxfp4_quantize(self, trans: bool, K: int, cols: int, X, ldx: int, x_type, Q, ldq: int, scales, offsets=None, groups: int = 0,
                        stream=None) -> None:
         """The K x cols matrix X (trans: its transpose is stored) in blocks of 32 down each column as 4-bit elements
         ``Q`` with a shared 8-bit power of two each (b200_mxfp4_quantize).  ``scales`` takes
         ``mxfp4_scale_bytes(K, cols, groups)`` bytes."""
-        _lib.check(_lib.lib().b200_mxfp4_quantize(self._h, stream, int(bool(trans)), K, cols, _addr(X), ldx, _type_code(x_type), _addr(Q), ldq,
-                                                  _addr(scales), _addr(offsets), groups), "mxfp4_quantize")
+        x, q, s = _addr(X, x_type, "X"), _addr(Q, _BYTES, "Q"), _addr(scales, _BYTES, "scales")
+        _lib.check(_lib.lib().b200_mxfp4_quantize(self._h, stream, int(bool(trans)), K, cols, x, ldx, _type_code(x_type), q, ldq, s,
+                                                  _addr(offsets, _OFFSETS, "offsets"), groups), "mxfp4_quantize")
 
     def mxfp4_dequantize(self, K: int, cols: int, Q, ldq: int, scales, Y, ldy: int, y_type, offsets=None, groups: int = 0, stream=None) -> None:
         """The values a 4-bit matrix stands for (b200_mxfp4_dequantize)."""
-        _lib.check(_lib.lib().b200_mxfp4_dequantize(self._h, stream, K, cols, _addr(Q), ldq, _addr(scales), _addr(Y), ldy, _type_code(y_type),
-                                                    _addr(offsets), groups), "mxfp4_dequantize")
+        q, s, y = _addr(Q, _BYTES, "Q"), _addr(scales, _BYTES, "scales"), _addr(Y, y_type, "Y")
+        _lib.check(_lib.lib().b200_mxfp4_dequantize(self._h, stream, K, cols, q, ldq, s, y, ldy, _type_code(y_type),
+                                                    _addr(offsets, _OFFSETS, "offsets"), groups), "mxfp4_dequantize")
 
     def gemm_mxfp4(self, M: int, N: int, K: int, alpha: float, A, lda: int, a_scales, B, ldb: int, b_scales, beta: float, Cm, ldc: int, c_type,
                    D, ldd: int, d_type, stream=None) -> None:
         """``D = alpha*A^T*B + beta*C`` with 4-bit A (K x M) and B (K x N) as ``mxfp4_quantize`` writes them
         (b200_gemm_mxfp4)."""
-        c = _addr(Cm) if Cm is not None else None
+        a, sa = _addr(A, _BYTES, "A"), _addr(a_scales, _BYTES, "a_scales")
+        b, sb = _addr(B, _BYTES, "B"), _addr(b_scales, _BYTES, "b_scales")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_mxfp4(
-            self._h, stream, M, N, K, float(alpha), _addr(A), lda, _addr(a_scales), _addr(B), ldb, _addr(b_scales), float(beta), c, ldc,
-            _type_code(c_type), _addr(D), ldd, _type_code(d_type)), "gemm_mxfp4")
+            self._h, stream, M, N, K, float(alpha), a, lda, sa, b, ldb, sb, float(beta), c, ldc, _type_code(c_type), d, ldd,
+            _type_code(d_type)), "gemm_mxfp4")
 
     def gemm_mxfp4_grouped(self, M: int, N: int, K: int, alpha: float, A, lda: int, stride_a: int, a_scales, B, ldb: int, b_scales, beta: float,
                            Cm, ldc: int, c_type, D, ldd: int, d_type, offsets, groups: int, stream=None) -> None:
         """``gemm_grouped`` with 4-bit matrices per group and 4-bit columns, quantised with the same offsets
         (b200_gemm_mxfp4_grouped)."""
-        c = _addr(Cm) if Cm is not None else None
+        a, sa = _addr(A, _BYTES, "A"), _addr(a_scales, _BYTES, "a_scales")
+        b, sb = _addr(B, _BYTES, "B"), _addr(b_scales, _BYTES, "b_scales")
+        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
         _lib.check(_lib.lib().b200_gemm_mxfp4_grouped(
-            self._h, stream, M, N, K, float(alpha), _addr(A), lda, stride_a, _addr(a_scales), _addr(B), ldb, _addr(b_scales), float(beta), c,
-            ldc, _type_code(c_type), _addr(D), ldd, _type_code(d_type), _addr(offsets), groups), "gemm_mxfp4_grouped")
+            self._h, stream, M, N, K, float(alpha), a, lda, stride_a, sa, b, ldb, sb, float(beta), c, ldc, _type_code(c_type), d, ldd,
+            _type_code(d_type), _addr(offsets, _OFFSETS, "offsets"), groups), "gemm_mxfp4_grouped")
 
     def gemm_gated(self, transA: bool, transB: bool, M: int, N: int, K: int, alpha: float, A, lda: int, B, ldb: int,
                    beta: float, Cm, ldc: int, D, ldd: int, panel_flags, panel_k: int, stream=None) -> None:

@@ -79,6 +79,18 @@ ENTRIES = {
                 dict(A=b16, B=b16, C=h16, D=b16)),
     "gemm_strided_batched": (lambda t: handle().gemm_strided_batched(False, False, 16, 16, 16, 1.0, t["A"], 16, 256, t["B"], 16, 256, F16, 1.0, t["C"], 16, 256, F32,
                                                                      t["D"], 16, 256, F16, 2), dict(A=h16, B=h16, C=f32, D=h16)),
+    "gemm_grouped": (lambda t: handle().gemm_grouped(True, 16, 16, 16, 1.0, t["A"], 16, 256, t["B"], 16, BFloat16, 1.0, t["C"], 16, F32, t["D"], 16, F16,
+                                                     t["offsets"], 2), dict(A=b16, B=b16, C=f32, D=h16, offsets=i32)),
+    "gemm_grouped_k": (lambda t: handle().gemm_grouped_k(16, 16, 16, 1.0, t["A"], 16, t["B"], 16, F16, 1.0, t["C"], 16, 256, BFloat16, t["D"], 16, 256,
+                                                         F32, t["offsets"], 2), dict(A=h16, B=h16, C=b16, D=f32, offsets=i32)),
+    "mxfp4_quantize": (lambda t: handle().mxfp4_quantize(False, 32, 16, t["X"], 32, BFloat16, t["Q"], 32, t["scales"], t["offsets"], 2),
+                       dict(X=b16, Q=u8, scales=u8, offsets=i32)),
+    "mxfp4_dequantize": (lambda t: handle().mxfp4_dequantize(32, 16, t["Q"], 32, t["scales"], t["Y"], 32, F32, t["offsets"], 2),
+                         dict(Q=u8, scales=u8, Y=f32, offsets=i32)),
+    "gemm_mxfp4": (lambda t: handle().gemm_mxfp4(16, 16, 32, 1.0, t["A"], 32, t["SA"], t["B"], 32, t["SB"], 1.0, t["C"], 16, F32, t["D"], 16, BFloat16),
+                   dict(A=u8, SA=u8, B=u8, SB=u8, C=f32, D=b16)),
+    "gemm_mxfp4_grouped": (lambda t: handle().gemm_mxfp4_grouped(16, 16, 32, 1.0, t["A"], 32, 512, t["SA"], t["B"], 32, t["SB"], 1.0, t["C"], 16, F16, t["D"],
+                                                                 16, F32, t["offsets"], 2), dict(A=u8, SA=u8, B=u8, SB=u8, C=h16, D=f32, offsets=i32)),
     "ShardedGemm.run": (lambda t: sharded().run(1.0, t["B"], 1.0, t["C"], t["D"]), dict(B=h16, C=f32, D=f32)),
 }
 # gemm_f16f32 takes the types of C and D from the operands
@@ -107,12 +119,21 @@ def test_another_type_is_refused(library, entry, operand, wrong):
 def test_addresses_and_typed_pointers(library, entry):
     """An address has no type; a DevicePtr has one, bfloat16 being its bit patterns."""
     call, types = ENTRIES[entry]
-    stored = {h16: F16, f32: F32, b16: np.uint16, i32: np.int32}
+    stored = {h16: F16, f32: F32, b16: np.uint16, u8: np.uint8, i32: np.int32}
     call({k: DevicePtr(stored[t], 4096) if entry != "gemm_f16f32" else Tensor(t) for k, t in types.items()})
     if entry != "gemm_f16f32":
         call({k: 4096 for k in types})
         with pytest.raises(TypeError):
-            call({k: DevicePtr(np.uint8, 4096) for k in types})
+            call({k: DevicePtr(np.int8, 4096) for k in types})
+
+
+def test_offsets_of_64_bits_are_refused(library):
+    """Read as 32 bits, 0, 0, n, 0 would be a legal empty group: nothing written, nothing reported."""
+    for name in ("gemm_grouped", "gemm_grouped_k", "mxfp4_quantize", "mxfp4_dequantize", "gemm_mxfp4_grouped"):
+        call, types = ENTRIES[name]
+        with pytest.raises(TypeError, match="offsets: expected int32"):
+            call({**{k: Tensor(t) for k, t in types.items()}, "offsets": DevicePtr(np.int64, 4096)})
+    assert not library.calls
 
 
 def test_a_c_that_is_not_read_has_any_type(library):
