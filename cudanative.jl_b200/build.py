@@ -20,7 +20,7 @@ BUILD_DIR = PKG_DIR / "build"
 LIB_PATH = PKG_DIR / "libb200wmma.so"
 
 SOURCES = ["api.cu", "gemm_sm100.cu", "gemm_simple.cu", "wmma_unit.cu", "noalloc.cu", "sharded.cu", "gemm_grouped.cu", "mxfp4.cu", "gemm_mxfp4.cu"]
-HEADERS = ["ptx_sm100.cuh", "gemm_sm100.cuh", "gemm_grouped.cuh", "gemm_mxfp4.cuh", "epilogue_sm100.cuh", "internal.h", "tensor_map.h", "rng.cuh", "wmma_frag.cuh"]
+HEADERS = ["ptx_sm100.cuh", "gemm_sm100.cuh", "gemm_grouped.cuh", "gemm_mxfp4.cuh", "epilogue_sm100.cuh", "mx_scale_rows.h", "internal.h", "tensor_map.h", "rng.cuh", "wmma_frag.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -27,6 +27,7 @@
 #pragma once
 
 #include "gemm_grouped.cuh"
+#include "mx_scale_rows.h"
 
 namespace b200 {
 
@@ -308,16 +309,19 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     const Unit u = decode(unit);
                     // a CTA of a pair may own no rows of A: its scales are then those of the last rows
                     const int a_row = u.group * p.a_per_group * p.a_tile_rows + min(u.m0 / 128, p.a_tile_rows - 1);
-                    const int b_row = first128[u.group] + (u.n0 - off[u.group]) / 128;
+                    const ScaleRows b_rows = scale_rows(first128[u.group], u.n0 - off[u.group], u.cols);
+                    const uint32_t bytes = 1024 * (1 + b_rows.count);
                     for (int kb = 0; kb < u.kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
                         ok = mbar_wait(empty_bar(s), ph ^ 1u, wc, kWaitEmptyStage);
                         if (!ok) break;
                         const uint32_t at = smem_base + s * Cfg::STAGE_BYTES + Cfg::A_BYTES + Cfg::B_BYTES;
-                        // two tiles along K (behind an odd last one: zeros), B_TILES along the columns; tiles that
-                        // this tile's columns do not touch are loaded and not used
-                        mbar_arrive_expect_tx(scales_full_bar(s), Cfg::SF_BYTES);
+                        // two tiles along K (behind an odd last one: zeros) of every row of tiles that this tile's columns
+                        // touch; what an earlier stage left in the place of another row belongs to no column of the products
+                        mbar_arrive_expect_tx(scales_full_bar(s), bytes);
                         tma_load_3d(at, &tmSA, 0, 2 * (kb_first + kb), a_row, scales_full_bar(s));
-                        tma_load_3d(at + 1024, &tmSB, 0, 2 * (kb_first + kb), b_row, scales_full_bar(s));
+#pragma unroll
+                        for (int i = 0; i < Cfg::B_TILES; ++i)
+                            if (i < b_rows.count) tma_load_3d(at + 1024 * (1 + i), &tmSB, 0, 2 * (kb_first + kb), b_rows.first + i, scales_full_bar(s));
                     }
                 }
             }

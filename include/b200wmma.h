@@ -246,7 +246,7 @@ int b200_gemm_grouped_k(b200_handle* h, b200_stream stream, int64_t M, int64_t N
  * Columns of no group are neither read nor written.  offsets = NULL and groups = 0: one plain matrix.
  *
  * b200_mxfp4_scale_bytes: bytes that the buffer of `scales` has to have (with groups > 0 for the worst
- *   sizes; a product may read all of it).
+ *   sizes).  Only the rows of tiles that the groups' columns use are read and written, the first ones.
  * b200_mxfp4_quantize: trans = 0: X is K x cols column-major, trans = 1: X is cols x K column-major, i.e.
  *   its transpose is quantised.  Float16, bfloat16 or Float32.  A block's scale is 2^(floor(log2 max) - 2),
  *   at least 2^-127; elements are rounded to nearest, ties to even, and saturate at 6.  A block that holds
