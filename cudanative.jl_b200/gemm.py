@@ -118,9 +118,10 @@ class Handle:
                              stride_a: int, B, ldb: int, stride_b: int, ab_type, beta: float, Cm, ldc: int,
                              stride_c: int, c_type, D, ldd: int, stride_d: int, d_type, batch: int, stream=None) -> None:
         """``batch`` products of one shape, matrix i of X starting ``stride_x * i`` elements after X
-        (b200_gemm_strided_batched); a stride of 0 repeats A, B or C."""
-        a, b = _addr(A, ab_type, "A"), _addr(B, ab_type, "B")
-        c, d = _addr(Cm, c_type if beta else None, "C"), _addr(D, d_type, "D")
+        (b200_gemm_strided_batched); a stride of 0 repeats A, B or C.  Tensors must have the types that the tags
+        name; a device array is a buffer of whatever they say."""
+        a, b = _addr(A, ab_type, "A", buffers=True), _addr(B, ab_type, "B", buffers=True)
+        c, d = _addr(Cm, c_type if beta else None, "C", buffers=True), _addr(D, d_type, "D", buffers=True)
         _lib.check(_lib.lib().b200_gemm_strided_batched(
             self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K, float(alpha), a, lda, stride_a, b, ldb,
             stride_b, _type_code(ab_type), float(beta), c, ldc, stride_c, _type_code(c_type), d, ldd, stride_d,
@@ -218,16 +219,17 @@ def mxfp4_scale_bytes(K: int, cols: int, groups: int = 0) -> int:
 _STORED = {_lib.F16: np.dtype(np.float16), _lib.F32: np.dtype(np.float32), _lib.BF16: np.dtype(np.uint16)}
 
 
-def _addr(x, elem=None, what: str = "operand"):
+def _addr(x, elem=None, what: str = "operand", buffers: bool = False):
     """Device address of an operand whose elements the library reads as ``elem``: an element type (Float16, Float32 or the
     ``BFloat16`` tag, which lies in memory as uint16 patterns) or a tuple of the numpy types that may stand there.  A typed
-    operand of another type is refused; None and plain addresses have no type to compare."""
+    operand of another type is refused; None and plain addresses have no type to compare, and with ``buffers`` device arrays
+    and typed pointers are taken as plain memory too."""
     if x is None:
         return None
     if isinstance(x, int):
         return x
     p = DevicePtr.of(x)
-    if elem is not None:
+    if elem is not None and (not buffers or hasattr(x, "data_ptr")):
         ok = [np.dtype(t) for t in elem] if isinstance(elem, tuple) else [_STORED[_type_code(elem)]]
         if p.dtype not in ok:
             raise TypeError(f"{what}: expected {' or '.join(t.name for t in ok)} elements" +
