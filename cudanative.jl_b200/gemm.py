@@ -22,6 +22,7 @@ from .bfloat16 import BFloat16
 
 
 _BYTES, _OFFSETS = (np.uint8,), (np.int32,)  # 4-bit elements and scales; group borders
+_WORDS = (np.uint32, np.int32, np.float32)  # memory of 32-bit flags
 _TYPE_CODES = {BFloat16: _lib.BF16, np.float16: _lib.F16, np.float32: _lib.F32}
 
 
@@ -193,7 +194,7 @@ class Handle:
         c, d = _addr(Cm, np.float32 if beta else None, "C"), _addr(D, np.float32, "D")
         _lib.check(_lib.lib().b200_gemm_f16f32_gated(self._h, stream, int(bool(transA)), int(bool(transB)), M, N, K,
                                                      float(alpha), a, lda, b, ldb, float(beta), c, ldc, d, ldd,
-                                                     _addr(panel_flags, (np.uint32, np.int32), "panel_flags"), panel_k),
+                                                     _addr(panel_flags, _WORDS, "panel_flags"), panel_k),
                    "gemm_gated")
 
     # -- host buffers (numpy, ideally page-locked) ---------------------------------------------

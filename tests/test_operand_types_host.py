@@ -93,8 +93,8 @@ ENTRIES = {
                                                                  16, F32, t["offsets"], 2), dict(A=u8, SA=u8, B=u8, SB=u8, C=h16, D=f32, offsets=i32)),
     "ShardedGemm.run": (lambda t: sharded().run(1.0, t["B"], 1.0, t["C"], t["D"]), dict(B=h16, C=f32, D=f32)),
 }
-# gemm_f16f32 takes the types of C and D from the operands
-FREE = {("gemm_f16f32", "C"): (h16, f32), ("gemm_f16f32", "D"): (h16, f32)}
+# gemm_f16f32 takes the types of C and D from the operands; flags are any 32-bit words
+FREE = {("gemm_gated", "flags"): (i32, f32), ("gemm_f16f32", "C"): (h16, f32), ("gemm_f16f32", "D"): (h16, f32)}
 
 
 @pytest.mark.parametrize("entry", ENTRIES)
