@@ -23,10 +23,12 @@
 //
 // kPromoteKb: the tensor core adds into its accumulator without rounding to nearest; every step drops what
 // lies below the last place, which pulls sums towards zero in proportion to the number of steps (measured
-// on K = 4096: 4e-6 of the result, 2e-5 for K = 16384; on K = 256 3e-7).  For a binary32 D that is more
-// than the result's own precision, so the MMA issuer starts a new accumulator every kPromoteKb k-blocks
-// and the warps add it, rounding to nearest, to a running sum in their registers while the next one is
-// being filled.  A 16-bit D rounds at 2^-9 or 2^-12 and takes the whole sum from one accumulator (0).
+// on K = 4096: 4e-6 of the result, 2e-5 for K = 16384; on K = 256 3e-7; on sums of one sign 1.1e-4 for K = 16384 and
+// 1.7e-3 for 262144).  For a binary32 D that is more than the result's own precision, so the MMA issuer starts a new
+// accumulator every kPromoteKb k-blocks and the warps add it, rounding to nearest, to a running sum in their
+// registers while the next one is being filled.  A 16-bit D rounds by up to 2^-8 or 2^-11 of the result: it takes
+// whole_kb k-blocks from one accumulator, which nearly always is all of K (kPromoteKb = 0), and kLong puts a longer sum
+// together from several.
 #pragma once
 
 #include "ptx_sm100.cuh"
@@ -40,6 +42,7 @@ struct EpilogueParams {
     void* D;
     long long ldc, ldd, stride_c, stride_d;  // strides: one C and D per group (kPerGroup)
     int c_fmt, d_fmt;                        // 0 = binary32, 1 = binary16, 2 = bfloat16
+    int whole_kb;                            // kLong: k-blocks that one accumulator sums at most, a power of two
     int d_pairs;                             // two rows of a 16-bit D can be stored as one word
 };
 
@@ -71,7 +74,7 @@ struct EpilogueCfg {
 __device__ __forceinline__ int columns_of(int tile_cols, int wg, int cols) { return min(cols, max(0, tile_cols - wg * cols)); }
 
 // Warps 4 .. 11 (`wg` 0 or 1).  Barriers tmem_full / tmem_empty [kAccs] are 8 bytes apart.
-template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kPerGroup, int kSplit, class Decode>
+template <class E, int kBN, int kAccs, int kCtas, bool kF32, int kPromoteKb, bool kLong, bool kPerGroup, int kSplit, class Decode>
 __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, uint32_t tmem_base, uint32_t tmem_full, uint32_t tmem_empty,
                                              const WaitCtx& wc, int unit_first, int unit_stride, int num_units, const SplitParams& split,
                                              Decode decode) {
@@ -149,6 +152,42 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld is warp-collective
             tc_fence_after_sync();
         };
+        // Several accumulators to a 16-bit D: the last one takes the sum, and what follows finds it there.  The running
+        // sums are indexed at run time and so lie in local memory: in registers they made the compiler spill in all of this
+        // function, and short groups beside a long one took 22% longer (256 groups of 16 columns, 512 x 768: 51 -> 63 us).
+        const bool longer = kLong && u.kb > p.whole_kb;
+        if (longer) {
+            float sum[E::COLS];
+#pragma unroll 1
+            for (int i = 0; i < E::COLS; ++i) sum[i] = 0.0f;
+            for (int kb = 0; kb < u.kb; kb += p.whole_kb) {
+                const uint32_t acc = acc_count % kAccs;
+                const bool last = kb + p.whole_kb >= u.kb;
+                wait_acc(acc);
+                if (!ok) break;
+#pragma unroll 1
+                for (int q = 0; q < E::COLS; q += 16) {
+                    if (q < cols) {
+                        const uint32_t at = tmem_base + lane_base + acc * kBN + col0 + q;
+                        uint32_t r[16];
+                        tmem_ld_32x32b_x16(at, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) sum[q + i] += __uint_as_float(r[i]);
+                        if (last) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(sum[q + i]);
+                            tmem_st_32x32b_x16(at, r);
+                        }
+                    }
+                }
+                if (last) break;
+                release(acc);
+                ++acc_count;
+            }
+            if (!ok) break;
+            tmem_wait_st();
+        }
         // C read directly: W columns ahead, the first before the accumulator is waited for, where the registers
         // are there for it (kAhead)
         float c_next[W];
@@ -364,7 +403,7 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
         } else {
             const bool empty = u.kb == 0;
             const uint32_t acc = acc_count % kAccs;
-            if (!empty) wait_acc(acc);
+            if (!empty && !longer) wait_acc(acc);
             if (!ok) break;
             for (int j = 0; ok && j * W < cols; ++j) {
                 uint32_t r[W];

@@ -134,10 +134,10 @@ struct Grouped {
     const int32_t* offsets;
 };
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
-int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
-    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kPromote, kSplit>;
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, int kSums, int kSplit>
+int launch_sums(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kSums, kSplit>;
+    auto kern = gemm_grouped_tcgen05<kBN, kAMn, kRaggedK, kCtas, kSums, kSplit>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
@@ -167,12 +167,13 @@ int launch_promote(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid,
     return B200_OK;
 }
 
-// binary32 results add several accumulators with rounding to nearest (epilogue_sm100.cuh)
+// binary32 results, and long sums of 16-bit ones, add several accumulators with rounding to nearest (epilogue_sm100.cuh)
 template <int kBN, bool kAMn, bool kRaggedK, int kCtas>
 int launch_grouped(const CUtensorMap (&tm)[2], const GroupedParams& p, int grid, cudaStream_t stream, bool pdl) {
     constexpr int kSplit = kBN == 32 ? 2 : 1;  // few columns per group: pairs of CTAs that may share a tile's inner dimension
-    if (p.e.d_fmt == 0) return launch_promote<kBN, kAMn, kRaggedK, kCtas, true, kSplit>(tm, p, grid, stream, pdl);
-    return launch_promote<kBN, kAMn, kRaggedK, kCtas, false, kSplit>(tm, p, grid, stream, pdl);
+    if (p.e.d_fmt == 0) return launch_sums<kBN, kAMn, kRaggedK, kCtas, kBinary32, kSplit>(tm, p, grid, stream, pdl);
+    if (p.K > p.e.whole_kb * 64) return launch_sums<kBN, kAMn, kRaggedK, kCtas, kLongSums, kSplit>(tm, p, grid, stream, pdl);
+    return launch_sums<kBN, kAMn, kRaggedK, kCtas, kOneAccumulator, kSplit>(tm, p, grid, stream, pdl);
 }
 
 template <int kBN, int kCtas>
@@ -208,8 +209,8 @@ int resident_clusters(int* clusters) {
     B200_CUDA_TRY(cudaGetDevice(&dev));
     *clusters = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
     if (*clusters > 0) return B200_OK;
-    auto kern = gemm_grouped_tcgen05<64, true, true, 1, true, 4>;
-    using Cfg = GroupedCfg<64, true, 1, true, 4>;
+    auto kern = gemm_grouped_tcgen05<64, true, true, 1, kBinary32, 4>;
+    using Cfg = GroupedCfg<64, true, 1, kBinary32, 4>;
     B200_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -287,6 +288,7 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     p.e.stride_d = g.stride_d;
     p.e.c_fmt = elem_fmt(g.c_type);
     p.e.d_fmt = elem_fmt(g.d_type);
+    p.e.whole_kb = whole_kb(p.e.d_fmt);
     p.a_per_group = g.stride_a != 0 ? 1 : 0;
     p.ab_bf16 = g.ab_type == B200_BF16 ? 1 : 0;
     p.status = h->status_word;
@@ -324,9 +326,9 @@ int run_tcgen05(b200_handle* h, cudaStream_t stream, const Grouped& g) {
     const bool pdl = h->pdl != 0;
     if (share) {
         grid = static_cast<int>(std::min<int64_t>(clusters, units)) * 4;
-        if (g.ragged_k) rc = launch_promote<64, true, true, 1, true, 4>(tm, p, grid, stream, pdl);
-        else if (g.transA) rc = launch_promote<64, false, false, 1, true, 4>(tm, p, grid, stream, pdl);
-        else rc = launch_promote<64, true, false, 1, true, 4>(tm, p, grid, stream, pdl);
+        if (g.ragged_k) rc = launch_sums<64, true, true, 1, kBinary32, 4>(tm, p, grid, stream, pdl);
+        else if (g.transA) rc = launch_sums<64, false, false, 1, kBinary32, 4>(tm, p, grid, stream, pdl);
+        else rc = launch_sums<64, true, false, 1, kBinary32, 4>(tm, p, grid, stream, pdl);
     } else if (pair == 2) rc = tile_n == 256 ? launch_kind<256, 2>(g, tm, p, grid, stream, pdl) : launch_kind<128, 2>(g, tm, p, grid, stream, pdl);
     else if (tile_n == 128) rc = launch_kind<128, 1>(g, tm, p, grid, stream, pdl);
     else if (tile_n == 64) rc = launch_kind<64, 1>(g, tm, p, grid, stream, pdl);

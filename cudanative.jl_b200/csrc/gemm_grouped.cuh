@@ -79,7 +79,16 @@ struct GroupedParams {
     unsigned long long wait_budget_ns;
 };
 
-template <int kBN, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
+// How a result's sum over K is put together: from one accumulator; of a binary32 D from several (epilogue_sm100.cuh); of
+// a 16-bit D from several where K is long.  The last is a kernel of its own, for the calls whose K or, for ragged K, whose
+// longest possible group passes whole_kb(): in the first one it cost 5% on many short groups that never need it.
+enum : int { kOneAccumulator = 0, kBinary32 = 1, kLongSums = 2 };
+
+// k-blocks that one accumulator of a 16-bit D sums at most: 16384 products for binary16, 65536 for bfloat16, which leaves sums of
+// one sign 1.1e-4 or 4.3e-4 off where the rounding that follows is up to 4.9e-4 or 3.9e-3.
+__host__ __device__ constexpr int whole_kb(int d_fmt) { return d_fmt == 1 ? 256 : 1024; }
+
+template <int kBN, bool kRaggedK, int kCtas, int kSums, int kSplit>
 struct GroupedCfg {
     static constexpr int THREADS = 384;
     static constexpr int BM = 128;
@@ -102,7 +111,7 @@ struct GroupedCfg {
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + RECV_BYTES + TABLE_BYTES + BAR_BYTES + 1024;
     static constexpr int NBARS = 4 * STAGES + 6;
     static_assert(kSplit != 2 || (kCtas == 1 && !kRaggedK && kBN == 32), "two share K: one-CTA tiles, one warp group");
-    static_assert(kSplit != 4 || (kCtas == 1 && kBN == 64 && kPromote), "four share K: one-CTA tiles, 16 columns each");
+    static_assert(kSplit != 4 || (kCtas == 1 && kBN == 64 && kSums == kBinary32), "four share K: one-CTA tiles, 16 columns each");
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
@@ -180,11 +189,12 @@ __device__ __forceinline__ int find_group(const int* first, int groups, int q) {
     return lo;
 }
 
-template <int kBN, bool kAMn, bool kRaggedK, int kCtas, bool kPromote, int kSplit>
+template <int kBN, bool kAMn, bool kRaggedK, int kCtas, int kSums, int kSplit>
 __global__ void __launch_bounds__(384, 1)
 gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const GroupedParams p) {
-    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kPromote, kSplit>;
+    using Cfg = GroupedCfg<kBN, kRaggedK, kCtas, kSums, kSplit>;
+    constexpr bool kPromote = kSums == kBinary32;
     constexpr int STAGES = Cfg::STAGES;
     using Epi = typename Cfg::Epi;
     constexpr bool kPair = (kCtas == 2);
@@ -432,14 +442,15 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         return done;
                     };
                     // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products.
-                    static_assert(Cfg::PROMOTE_KB % 2 == 0, "an accumulator begins and ends with a turn");
+                    // An accumulator begins and ends with a turn: what it sums is an even power of two of k-blocks.
+                    const int acc_mask = (kPromote ? Cfg::PROMOTE_KB : p.e.whole_kb) - 1;
                     for (int kb = 0; kb < kb_total; kb += 2) {
                         const uint32_t acc = ucount & 1u;
                         const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
                         const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
                         const bool two = kb + 1 < kb_total, last = kb + 2 >= kb_total;
-                        const bool begin = kb == 0 || (kPromote && kb % Cfg::PROMOTE_KB == 0);
-                        const bool end = last || (kPromote && (kb + 2) % Cfg::PROMOTE_KB == 0);
+                        const bool begin = kb == 0 || (kSums != kOneAccumulator && (kb & acc_mask) == 0);
+                        const bool end = last || (kSums != kOneAccumulator && ((kb + 2) & acc_mask) == 0);
                         if (begin) ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount >> 1) & 1u) ^ 1u, wc, kWaitTmemEmpty));
                         if (ok && !ready)
                             ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
@@ -506,7 +517,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     } else {
         regs_inc<224>();
         const int wg = (warp - 4) >> 2;
-        run_epilogue<Epi, kBN, 2, kCtas, kPromote && kSplit != 4, kPromote ? Cfg::PROMOTE_KB : 0, kRaggedK, kSplit>(
+        run_epilogue<Epi, kBN, 2, kCtas, kPromote && kSplit != 4, kPromote ? Cfg::PROMOTE_KB : 0, kSums == kLongSums, kRaggedK, kSplit>(
             p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 

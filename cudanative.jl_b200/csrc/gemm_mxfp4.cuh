@@ -371,7 +371,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     } else {
         regs_inc<200>();
         const int wg = (warp - 4) >> 2;
-        run_epilogue<Epi, kBN, ACCS, kCtas, false, ACCS == 1 ? -1 : 0, false, kSplit ? 2 : 1>(
+        run_epilogue<Epi, kBN, ACCS, kCtas, false, ACCS == 1 ? -1 : 0, false, false, kSplit ? 2 : 1>(
             p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 

@@ -209,9 +209,11 @@ int b200_gemm_strided_batched(b200_handle* h, b200_stream stream, int transA, in
  *   values.  D may alias C exactly (same pointer, ld and type).
  * The tcgen05 kernel needs 16-byte aligned A and B, lda, ldb and stride_a multiples of 8 elements and
  * stride_a at least one matrix (or 0); anything else runs on the simple kernel.  C and D may have any
- * alignment.  A binary32 D on the tcgen05 kernel sums several accumulators, each of 512 products, with
- * rounding to nearest; so does any D where tiles are few and K is long: four CTAs share a tile's K then
- * (b200_last_launch reports split_k 4) and their sums are added in a fixed order.  The split-K option is
+ * alignment.  The tensor core truncates when it adds, so no accumulator of the tcgen05 kernel takes an
+ * unlimited sum: a binary32 D adds several, each of 512 products, with rounding to nearest; a Float16 D
+ * takes at most 16384 products from one and a bfloat16 D 65536.  Where tiles are few and K is long, four
+ * CTAs share a tile's K (b200_last_launch reports split_k 4): 512 products to an accumulator for any D, and
+ * their sums are added in a fixed order.  The split-K option is
  * ignored. */
 int b200_gemm_grouped(b200_handle* h, b200_stream stream, int transA, int64_t M, int64_t N, int64_t K,
                       float alpha, const void* A, int64_t lda, int64_t stride_a, const void* B,
