@@ -152,10 +152,10 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             ok = __all_sync(0xffffffffu, ok);  // tcgen05.ld is warp-collective
             tc_fence_after_sync();
         };
-        // Several accumulators to a 16-bit D: the last one takes the sum, and what follows finds it there.  The running
+        // Several accumulators: the last one takes the sum, and what follows finds it there.  The running
         // sums are indexed at run time and so lie in local memory: in registers they made the compiler spill in all of this
         // function, and short groups beside a long one took 22% longer (256 groups of 16 columns, 512 x 768: 51 -> 63 us).
-        const bool longer = kLong && u.kb > p.whole_kb;
+        const bool longer = kLong && !kDrain && u.kb > p.whole_kb;
         if (longer) {
             float sum[E::COLS];
 #pragma unroll 1
@@ -397,6 +397,24 @@ __device__ __forceinline__ void run_epilogue(const EpilogueParams& p, int wg, ui
             tmem_wait_ld();
             release(acc);
             ++acc_count;
+            // the issuer waits for each of the further ones to be read: its sum stays in the registers
+            for (int kb = p.whole_kb; kLong && kb < u.kb; kb += p.whole_kb, ++acc_count) {
+                const uint32_t acc = acc_count % kAccs;
+                wait_acc(acc);
+                if (!ok) break;
+#pragma unroll
+                for (int q = 0; q < E::COLS; q += 16) {
+                    if (q < cols) {
+                        uint32_t x[16];
+                        tmem_ld_32x32b_x16(tmem_base + lane_base + acc * kBN + col0 + q, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) r[q / W][q % W + i] = __float_as_uint(__uint_as_float(r[q / W][q % W + i]) + __uint_as_float(x[i]));
+                    }
+                }
+                release(acc);
+            }
+            if (!ok) break;
 #pragma unroll
             for (int q = 0; q < E::COLS / W; ++q)
                 if (ok && q * W < cols) finish(q, r[q]);

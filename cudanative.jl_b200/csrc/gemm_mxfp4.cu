@@ -20,11 +20,11 @@ struct MxProblem {
     const int32_t* offsets;
 };
 
-template <int kBN, int kCtas>
-int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+template <int kBN, int kCtas, bool kLong>
+int launch_as(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
     constexpr bool kSplit = kBN == 32;  // few columns: pairs of CTAs that may share a tile's inner dimension
     using Cfg = MxCfg<kBN, kCtas, kSplit>;
-    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kSplit>;
+    auto kern = gemm_mxfp4_tcgen05<kBN, kCtas, kSplit, kLong>;
     static std::atomic<uint64_t> done{0};  // devices that have been opted in to the kernel's shared memory
     int dev = 0;
     B200_CUDA_TRY(cudaGetDevice(&dev));
@@ -52,6 +52,12 @@ int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStre
     cfg.numAttrs = pdl ? 2 : 1;
     B200_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p));
     return B200_OK;
+}
+
+template <int kBN, int kCtas>
+int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStream_t stream, bool pdl) {
+    if (p.K > p.e.whole_kb * 256) return launch_as<kBN, kCtas, true>(tm, p, grid, stream, pdl);  // more than one accumulator sums
+    return launch_as<kBN, kCtas, false>(tm, p, grid, stream, pdl);
 }
 
 // Tile columns, by the mean length of the groups.  256 columns leave tensor memory for one accumulator: its
@@ -90,6 +96,7 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     p.e.ldd = g.ldd;
     p.e.c_fmt = elem_fmt(g.c_type);
     p.e.d_fmt = elem_fmt(g.d_type);
+    p.e.whole_kb = mx_whole_kb(p.e.d_fmt);
     p.status = h->status_word;
     p.wait_budget_ns = h->wait_budget_ns;
     p.e.d_pairs = !(reinterpret_cast<uintptr_t>(g.D) & 3u) && g.ldd % 2 == 0;

@@ -18,9 +18,10 @@
 // scales put those rows into the first column, since an odd column is no legal scale address.  A tile of 192
 // begins at row 0 or 64, which is column 0 or 2.
 //
-// One accumulator takes the whole sum in every case: the products have so few bits that the tensor core's
-// truncation hardly meets one (K = 8192: exact on normal data, 1.7e-7 of the result with values spread over
-// e^+-6; summed every 2048 values 4e-8).
+// How long a sum one accumulator may take: the tensor core truncates when it adds, and though 4-bit products have few bits, sums of
+// one sign whose scales differ lose some with every instruction (scales within 2^+-4, one accumulator: 8e-7 of the
+// result at K = 8192, 1.4e-5 at 65536, 7e-5 at 262144).  A binary32 D takes 8192 products from one accumulator, a 16-bit D
+// 65536; a longer K has a kernel of its own (kLong) that adds several with rounding to nearest.
 //
 // What bounds it: 4-bit products run at four times the rate of 16-bit ones, with the same bytes per cycle.
 // For few columns (a token, a decode step) the elements of A, 17/32 byte per value, are the floor.
@@ -78,7 +79,10 @@ struct MxCfg {
     static_assert(kBN == 32 || kBN == 128 || kBN == 192 || kBN == 256, "a tile of columns begins on a multiple of 32 inside its scale tile");
 };
 
-template <int kBN, int kCtas, bool kSplit>
+// k-blocks that one accumulator sums at most
+__host__ __device__ constexpr int mx_whole_kb(int d_fmt) { return d_fmt == 0 ? 32 : 256; }
+
+template <int kBN, int kCtas, bool kSplit, bool kLong>
 __global__ void __launch_bounds__(512, 1)
 gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB, const MxGemmParams p) {
@@ -242,9 +246,20 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                     // 192 columns begin at row 0 or 64 of their scale tile: two columns of 32 rows further
                     const uint32_t shift = kBN == 192 ? __shfl_sync(0xffffffffu, static_cast<uint32_t>(scale_shift(u)) / 32, 0) : 0u;
                     const uint32_t idesc0 = make_idesc_mxf4(Cfg::BM * kCtas, __shfl_sync(0xffffffffu, inst_n(u), 0), 0);
-                    const uint32_t acc = ucount % ACCS;
-                    const uint32_t d_tmem = tmem_base + acc * kBN;
-                    ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    uint32_t acc, d_tmem;
+                    auto begin = [&] {
+                        acc = ucount % ACCS;
+                        d_tmem = tmem_base + acc * kBN;
+                        ok = __all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((ucount / ACCS) & 1u) ^ 1u, wc, kWaitTmemEmpty));
+                    };
+                    auto end = [&] {
+                        if (lead) {
+                            if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
+                            else umma_commit<kCtas>(tmem_full_bar(acc));
+                        }
+                        ++ucount;
+                    };
+                    begin();
                     if (!ok) break;
                     const int last_steps = min(4, (p.K - (kb_first + kb_total - 1) * Cfg::BK + 63) / 64);
                     auto products = [&](int st, bool first, int steps) {
@@ -269,6 +284,13 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
                         const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);
                         const bool two = kb + 1 < kb_total;
+                        // an accumulator begins with a turn: what it sums is an even power of two of k-blocks
+                        const bool next_acc = kLong && kb != 0 && (kb & (p.e.whole_kb - 1)) == 0;
+                        if (next_acc) {
+                            end();
+                            begin();
+                            if (!ok) break;
+                        }
                         if (!ready)
                             ok = __all_sync(0xffffffffu, mbar_wait(full_bar(s), ph, wc, kWaitFullStage) &&
                                                              (!two || mbar_wait(full_bar(s1), ph1, wc, kWaitFullStage)));
@@ -277,24 +299,20 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         if (two) {
                             // look at the next two now: the answer arrives while these two's products are issued
                             const bool next = mbar_test(full_bar(s2), ph2) && mbar_test(full_bar(s3), ph3);
-                            products(s, kb == 0, 4);
+                            products(s, kb == 0 || next_acc, 4);
                             products(s1, false, kb + 2 == kb_total ? last_steps : 4);
                             ready = __all_sync(0xffffffffu, next);
                             s = s2;
                             ph = ph2;
                         } else {
-                            products(s, kb == 0, last_steps);
+                            products(s, kb == 0 || next_acc, last_steps);
                             ready = false;
                             s = s1;
                             ph = ph1;
                         }
                     }
                     if (!ok) break;
-                    if (lead) {
-                        if constexpr (kPair) umma_commit_pair(tmem_full_bar(acc));
-                        else umma_commit<kCtas>(tmem_full_bar(acc));
-                    }
-                    ++ucount;
+                    end();
                 }
             }
             __syncwarp();
@@ -371,7 +389,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     } else {
         regs_inc<200>();
         const int wg = (warp - 4) >> 2;
-        run_epilogue<Epi, kBN, ACCS, kCtas, false, ACCS == 1 ? -1 : 0, false, false, kSplit ? 2 : 1>(
+        run_epilogue<Epi, kBN, ACCS, kCtas, false, ACCS == 1 ? -1 : 0, kLong, false, kSplit ? 2 : 1>(
             p.e, wg, tmem_base, tmem_full_bar(0), tmem_empty_bar(0), wc, unit_first, unit_stride, num_units, split, decode);
     }
 

@@ -78,3 +78,53 @@ def test_ragged_n(handle, positive, d_type, tile_n, cta_pair, N):
                         d, M, d_type, CuArray(offsets_of([N // 2, 0, N - N // 2])), 3)
     sync(handle)
     near16(Array(d), alpha * (value(A, F16) @ value(B[:N], F16).T) + 2.0, d_type, K, f"tiles of {tile_n}")
+
+
+# ---- 4-bit operands: 64 products to an instruction; a binary32 result takes 8192 from one accumulator, a 16-bit one 65536
+def operand(r, K, cols, spread=4):
+    """Elements of one sign, scales that differ; zeros behind K."""
+    codes = r.integers(1, 8, ((K + 31) // 32 * 32, cols)).astype(np.uint8)
+    codes[K:] = 0
+    return codes, (127 + r.integers(-spread, spread + 1, (codes.shape[0] // 32, cols))).astype(np.uint8)
+
+
+def run_mx(handle, M, N, K, d_type, beta=0.0, sizes=None, alpha=2.0 ** -12):
+    r = np.random.default_rng(K + N)
+    (qa, sa), (qb, sb) = operand(r, K, M), operand(r, K, N)
+    off = None if sizes is None else offsets_of(sizes)
+    ld = qa.shape[0]
+    d, c = CuArray(np.zeros((M, N), np.uint16 if d_type is BFloat16 else d_type, order="F")), CuArray(np.full((M, N), 2.0, F32, order="F"))
+    args = (CuArray(pack(qa, ld)), ld) + (() if off is None else (0,)) + (CuArray(tile(sa)), CuArray(pack(qb, ld)), ld, CuArray(tile(sb, off)), beta, c, M, F32, d, M, d_type)
+    if off is None:
+        handle.gemm_mxfp4(M, N, K, alpha, *args)
+    else:
+        handle.gemm_mxfp4_grouped(M, N, K, alpha, *args, CuArray(off), len(sizes))
+    sync(handle)
+    exact = alpha * (values(qa, sa)[:K].T @ values(qb, sb)[:K]) + beta * 2.0
+    products = 8192 if d_type is F32 else 65536
+    near(value(Array(d), d_type), exact, d_type, K, products, products // 64, f"{M} x {N} x {K}")
+    return handle.last_launch()["tile_n"]
+
+
+@pytest.mark.parametrize("N,tile_n,beta,expect", [(8, 0, 0.0, 32), (72, 0, 0.0, 128), (136, 0, 0.0, 256), (136, 0, 1.0, 192), (136, 256, 0.0, 256), (8, 128, 1.0, 128)])
+def test_mx_binary32(handle, N, tile_n, beta, expect):
+    handle.set_option(_lib.OPT_TILE_N, tile_n)
+    assert run_mx(handle, 136, N, 262144 + 40, F32, beta=beta) == expect
+    for K in (8192, 8193, 16384, 24576 + 31):  # one accumulator, a second one of one value, whole ones
+        assert run_mx(handle, 136, N, K, F32, beta=beta) == expect
+
+
+def test_mx_binary32_groups(handle):
+    for sizes in ([5, 0, 3], [70, 0, 1], [300, 0, 129, 64]):
+        run_mx(handle, 264, sum(sizes), 40000, F32, sizes=sizes)
+    handle.set_option(_lib.OPT_MAX_CTAS, 2)  # many tiles to a CTA: the accumulators go around
+    run_mx(handle, 264, 429, 25000, F32, beta=1.0, sizes=[300, 0, 129])
+    run_mx(handle, 520, 300, 25000, F32)
+
+
+@pytest.mark.parametrize("d_type", [F16, BFloat16])
+@pytest.mark.parametrize("tile_n", [0, 128, 256])
+def test_mx_16_bits(handle, d_type, tile_n):
+    handle.set_option(_lib.OPT_TILE_N, tile_n)
+    for K in (65536, 65536 + 40, 2 ** 21):
+        run_mx(handle, 136 if tile_n == 256 else 8, 8, K, d_type, alpha=2.0 ** -15)
