@@ -109,17 +109,19 @@ int run(b200_handle* h, cudaStream_t stream, const MxProblem& g) {
     b.stride = b.count > 1 ? g.stride_a / 2 : g.lda / 2 * g.M;
     if ((rc = encode_map_2d(&tm[0], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.A, k_bytes, g.M, g.lda / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B, "A", b))) return rc;
     if ((rc = encode_map_2d(&tm[1], CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.B, k_bytes, g.N, g.ldb / 2, 128, bbox, CU_TENSOR_MAP_SWIZZLE_128B, "B"))) return rc;
-    // scales: tiles of 128 words, K tiles, rows of tiles; a copy takes 2 along K of one row
+    // scales: tiles of 128 words, K tiles, rows of tiles; a copy takes 2 along K.  How many rows the groups of B use is not
+    // known here, only the most they can: those copies take one row each
     const int64_t kt = (g.K + 127) / 128, sa_rows = p.a_tile_rows * b.count;
     const int64_t sb_rows = b200_mxfp4_scale_bytes(g.K, g.N, g.offsets ? g.groups : 0) / 512 / kt;
     if (sa_rows > 0x7fffff00ll || sb_rows > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many scale tiles");
-    auto scale_map = [&](CUtensorMap* m, const void* ptr, int64_t rows, const char* what) {
+    auto scale_map = [&](CUtensorMap* m, const void* ptr, int64_t rows, int box_rows, const char* what) {
         BatchDim d;
         d.count = rows;
         d.stride = kt * 128;
+        d.box = box_rows;
         return encode_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, ptr, 128, kt, 128, 128, 2, CU_TENSOR_MAP_SWIZZLE_NONE, what, d);
     };
-    if ((rc = scale_map(&tm[2], g.SA, sa_rows, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, "scales of B"))) return rc;
+    if ((rc = scale_map(&tm[2], g.SA, sa_rows, 1, "scales of A")) || (rc = scale_map(&tm[3], g.SB, sb_rows, g.offsets ? 1 : (tile_n + 127) / 128, "scales of B"))) return rc;
     const int64_t units = (g.N / tile_n + std::min(g.groups, g.N)) * tiles_m;
     if (units > 0x7fffff00ll) return fail(B200_UNSUPPORTED, "mxfp4 gemm: too many tiles for one launch");
     const int cap = h->max_ctas > 0 ? std::min(h->max_ctas, h->sm_count) : h->sm_count;

@@ -86,7 +86,7 @@ int encode_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer),
                           static_cast<cuuint64_t>(batch.count)};
     cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * elem_bytes, static_cast<cuuint64_t>(batch.stride) * elem_bytes};
-    cuuint32_t box[3] = {box_inner, box_outer, 1};
+    cuuint32_t box[3] = {box_inner, box_outer, batch.box};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(tm, dt, batch.count > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE,

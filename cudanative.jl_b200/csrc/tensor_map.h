@@ -10,10 +10,11 @@ namespace b200 {
 struct BatchDim {
     int64_t count = 0;
     int64_t stride = 0;
+    uint32_t box = 1;  // matrices per copy
 };
 
 // Tensor map over a column-major matrix: dim0 (contiguous) has `inner` elements, dim1 has `outer`
-// elements `ld` elements apart; batched problems add dim2 = matrix of the batch (box extent 1).
+// elements `ld` elements apart; batched problems add dim2 = matrix of the batch (box extent 1 unless asked for).
 int encode_map_2d(CUtensorMap* tm, CUtensorMapDataType dt, int elem_bytes, const void* base, int64_t inner,
                   int64_t outer, int64_t ld, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw,
                   const char* what, BatchDim batch = BatchDim());
