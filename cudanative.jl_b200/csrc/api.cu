@@ -186,17 +186,24 @@ int gemm_dispatch(b200_handle* h, cudaStream_t stream, const GemmProblem& g) {
     return fail(B200_INVALID_ARG, "unknown kernel selector");
 }
 
-int read_status(b200_handle* h, int* word) {
+int read_status(b200_handle* h, int* wait, int* offsets) {
     if (!h->poll_stream) B200_CUDA_TRY(cudaStreamCreateWithFlags(&h->poll_stream, cudaStreamNonBlocking));
-    if (!h->host_word) B200_CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&h->host_word), 4 * sizeof(int), cudaHostAllocDefault));
-    B200_CUDA_TRY(cudaMemcpyAsync(h->host_word, h->status_word, 4 * sizeof(int), cudaMemcpyDeviceToHost, h->poll_stream));
+    if (!h->host_word) B200_CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&h->host_word), 8 * sizeof(int), cudaHostAllocDefault));
+    B200_CUDA_TRY(cudaMemcpyAsync(h->host_word, h->status_word, 8 * sizeof(int), cudaMemcpyDeviceToHost, h->poll_stream));
     B200_CUDA_TRY(cudaStreamSynchronize(h->poll_stream));
-    for (int i = 0; i < 4; ++i) word[i] = h->host_word[i];
-    if (word[0] != 0) {
-        B200_CUDA_TRY(cudaMemsetAsync(h->status_word, 0, 4 * sizeof(int), h->poll_stream));
+    for (int i = 0; i < 4; ++i) wait[i] = h->host_word[i];
+    const bool take_offsets = offsets && wait[0] == 0;
+    for (int i = 0; offsets && i < 4; ++i) offsets[i] = take_offsets ? h->host_word[4 + i] : 0;
+    if (wait[0] != 0 || (take_offsets && offsets[0] != 0)) {
+        B200_CUDA_TRY(cudaMemsetAsync(h->status_word + (wait[0] != 0 ? 0 : 4), 0, 4 * sizeof(int), h->poll_stream));
         B200_CUDA_TRY(cudaStreamSynchronize(h->poll_stream));
     }
     return B200_OK;
+}
+
+int wait_error(const int* wait, const std::string& before, const std::string& after) {
+    if (wait[0] == 0) return B200_OK;
+    return fail(B200_DEVICE_TIMEOUT, before + " (wait id " + std::to_string(wait[0]) + ", block " + std::to_string(wait[1]) + ")" + after);
 }
 
 // B200_OPT_CHECK_ON_CALL: what the reference does in prepare_cuda_call (src/init.jl:37 ->
@@ -209,17 +216,14 @@ int poll_previous_launch(b200_handle* h) {
     if (e == cudaErrorNotReady) return B200_OK;
     if (e != cudaSuccess) return cuda_fail(e, "cudaEventQuery(previous launch)");
     h->last_pending = false;
-    int word[4] = {0, 0, 0, 0};
-    int rc = read_status(h, word);
+    int wait[4], offsets[4];
+    int rc = read_status(h, wait, offsets);
     if (rc) return rc;
-    if (word[0] == kBadOffsets)
+    if (offsets[0] != 0)
         return fail(B200_INVALID_ARG, "an earlier launch of this handle found group offsets that decrease or leave the matrix; it wrote "
                                       "nothing.  This call enqueued nothing.");
-    if (word[0] != 0)
-        return fail(B200_DEVICE_TIMEOUT, "a bounded wait ran out on the device in an earlier launch of this handle (wait id " +
-                                             std::to_string(word[0]) + ", block " + std::to_string(word[1]) +
-                                             "); its result is not valid.  This call enqueued nothing.");
-    return B200_OK;
+    return wait_error(wait, "a bounded wait ran out on the device in an earlier launch of this handle",
+                      "; its result is not valid.  This call enqueued nothing.");
 }
 
 int note_launch(b200_handle* h, cudaStream_t stream) {
@@ -296,7 +300,7 @@ int b200_create(b200_handle** out, int device) {
     b200_handle* h = new b200_handle();
     h->device = device;
     h->sm_count = sms;
-    if (cudaMalloc(&h->status_word, 4 * sizeof(int)) != cudaSuccess || cudaMemset(h->status_word, 0, 4 * sizeof(int)) != cudaSuccess) {
+    if (cudaMalloc(&h->status_word, 8 * sizeof(int)) != cudaSuccess || cudaMemset(h->status_word, 0, 8 * sizeof(int)) != cudaSuccess) {
         int rc = cuda_fail(cudaGetLastError(), "b200_create: status word");
         delete h;
         return rc;
@@ -389,9 +393,10 @@ int b200_get_option(b200_handle* h, int option, int64_t* value) {
 
 int b200_device_status(b200_handle* h, int* code, int* block, int* detail) {
     if (!h) return fail(B200_INVALID_ARG, "null handle");
-    int word[4] = {0, 0, 0, 0};
-    int rc = read_status(h, word);
+    int wait[4], offsets[4];
+    int rc = read_status(h, wait, offsets);
     if (rc) return rc;
+    const int* word = wait[0] != 0 ? wait : offsets;
     if (code) *code = word[0];
     if (block) *block = word[1];
     if (detail) *detail = word[2];
@@ -628,12 +633,9 @@ int b200_gemm_f16f32_host(b200_handle* h, int transA, int transB, int64_t M, int
     B200_CUDA_TRY(cudaStreamSynchronize(s_dn));
     B200_CUDA_TRY(cudaStreamSynchronize(s_mm));
     B200_CUDA_TRY(cudaStreamSynchronize(s_up));
-    int word[4] = {0, 0, 0, 0};
-    if ((rc = read_status(h, word))) return rc;
-    if (word[0] != 0)
-        return fail(B200_DEVICE_TIMEOUT, "gemm: a bounded wait ran out on the device (wait id " + std::to_string(word[0]) +
-                                             ", block " + std::to_string(word[1]) + ")");
-    return B200_OK;
+    int wait[4];
+    if ((rc = read_status(h, wait))) return rc;
+    return wait_error(wait, "gemm: a bounded wait ran out on the device");
 }
 
 int b200_malloc(void** dptr, size_t bytes) {

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256) grouped_plain_kernel(const PlainParams p)
     __shared__ int off[kMaxGroups + 1], first[kMaxGroups + 1];
     __shared__ unsigned long long sums[8];
     if (!load_groups<true>(p.offsets, p.groups, static_cast<int>(p.N), kTile, off, first, sums)) {
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
+        if (threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
         return;
     }
     for (int q = blockIdx.y; q < first[p.groups]; q += gridDim.y) {
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) grouped_k_plain_kernel(const PlainParams 
     __shared__ float sA[kTileK][kTile + 1], sB[kTileK][kTile + 1];
     __shared__ int off[kMaxGroups + 1];
     if (!load_groups<false>(p.offsets, p.groups, static_cast<int>(p.K), kTile, off, nullptr, nullptr)) {
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
+        if (threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
         return;
     }
     const long long m0 = static_cast<long long>(blockIdx.x) * kTile, n0 = static_cast<long long>(blockIdx.y) * kTile;

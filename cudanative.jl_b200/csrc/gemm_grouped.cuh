@@ -258,11 +258,7 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     // the scan's scratch may lie in the first stage: nothing uses it yet
     const bool offsets_ok = load_groups<!kRaggedK, Cfg::THREADS>(p.offsets, p.groups, kRaggedK ? p.K : p.N, kBN, off, first,
                                                    reinterpret_cast<unsigned long long*>(smem_gen));
-    if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
-        p.status[1] = static_cast<int>(blockIdx.x);
-        p.status[2] = p.groups;
-        __threadfence();
-    }
+    if (!offsets_ok && threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
     const int tiles_m = p.raster.rows.d;
     const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * p.tiles.d : first[p.groups] * tiles_m;
 

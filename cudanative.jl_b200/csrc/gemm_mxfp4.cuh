@@ -151,11 +151,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     // the scan's scratch may lie in the first stage: nothing uses it yet
     const bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<unsigned long long*>(smem_gen),
                                                             kBN == 128 ? nullptr : first128);
-    if (!offsets_ok && threadIdx.x == 0 && atomicCAS(p.status, 0, static_cast<int>(kBadOffsets)) == 0) {
-        p.status[1] = static_cast<int>(blockIdx.x);
-        p.status[2] = p.groups;
-        __threadfence();
-    }
+    if (!offsets_ok && threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
     const int num_units = offsets_ok ? first[p.groups] * p.raster.rows.d : 0;
 
     // Split the inner dimension when that shortens the longest CTA's work (counted in whole tiles).

@@ -76,7 +76,7 @@ struct LaunchInfo {
 struct b200_handle {
     int device = 0;
     int sm_count = 0;
-    int* status_word = nullptr;  // 4 ints on the device
+    int* status_word = nullptr;  // on the device: 4 ints for a wait that ran out, 4 for group offsets that are none
     // options
     int force_kernel = B200_KERNEL_AUTO;
     int max_ctas = 0;
@@ -114,8 +114,12 @@ int check_current_device(const b200_handle* h);
 // B200_OPT_CHECK_ON_CALL around a launch: look at the failure word of the previous one, note this one.
 int poll_previous_launch(b200_handle* h);
 int note_launch(b200_handle* h, cudaStream_t stream);
-// Copies the handle's 4-int device status word to `word` (synchronous) and clears it when non-zero.
-int read_status(b200_handle* h, int* word);
+// Takes the record of a wait that ran out (4 ints, the first 0 when there is none) and, where it is asked for and no wait ran
+// out, that of bad group offsets; synchronous, a record that was taken is cleared.  Bad offsets are the fault of the
+// grouped call alone: what looks for its own waits leaves them for b200_device_status.
+int read_status(b200_handle* h, int* wait, int* offsets = nullptr);
+// The error of a wait record, B200_OK for none.
+int wait_error(const int* wait, const std::string& before, const std::string& after = "");
 
 // Scratch needed for the plan's split-K partials, in bytes (0 when split_k == 1).
 size_t gemm_tcgen05_scratch_bytes(const GemmProblem& g, const GemmPlan& plan);

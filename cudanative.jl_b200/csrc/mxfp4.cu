@@ -114,7 +114,7 @@ __device__ __forceinline__ TileRow tile_row(const MxParams& p, const int* off, c
 __device__ __forceinline__ long long scale_tile_rows(const MxParams& p, int* off, int* first, unsigned long long* sums) {
     if (!p.offsets) return (p.cols + 127) / 128;
     if (!load_groups<true>(p.offsets, p.groups, p.cols, 128, off, first, sums)) {
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, static_cast<int>(kBadOffsets));
+        if (threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
         return 0;
     }
     return first[p.groups];

@@ -171,6 +171,15 @@ static __device__ __noinline__ void report_timeout(const WaitCtx& w, int where, 
     }
 }
 
+// Group offsets that decrease or leave the matrix have a record of their own behind that of the waits: neither hides the other.
+static __device__ __forceinline__ void report_bad_offsets(int* status, int groups) {
+    if (atomicCAS(status + 4, 0, static_cast<int>(kBadOffsets)) == 0) {
+        status[5] = static_cast<int>(blockIdx.x);
+        status[6] = groups;
+        __threadfence();
+    }
+}
+
 // Bounded wait for phase `parity` of an mbarrier.  Returns false when the budget ran out or
 // another role of this CTA already gave up; the caller must then fall through to the kernel's
 // common exit (which frees TMEM).  Never spins unboundedly.

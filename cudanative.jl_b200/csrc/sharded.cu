@@ -662,19 +662,16 @@ int b200_sharded_wait(b200_sharded* s, int64_t timeout_ms) {
         B200_CUDA_TRY(cudaStreamSynchronize(s->rescue));
         // the released work is finite (copies and GEMM launches with bounded waits): let it drain
         for (const auto& sk : streams) B200_CUDA_TRY(cudaStreamSynchronize(sk.first));
-        int word[4];
-        read_status(s->h, word);
+        int wait[4];
+        read_status(s->h, wait);
         s->in_flight = false;
         return fail(B200_PEER_TIMEOUT, "sharded_wait: no word from a peer within " + std::to_string(timeout_ms) +
                                            " ms (epoch " + std::to_string(s->epoch) + ")" + heard + "; the waits were released, D is not valid");
     }
     s->in_flight = false;
-    int word[4] = {0, 0, 0, 0};
-    if ((rc = read_status(s->h, word))) return rc;
-    if (word[0] != 0)
-        return fail(B200_DEVICE_TIMEOUT, "sharded gemm: a bounded wait ran out on the device (wait id " + std::to_string(word[0]) +
-                                             ", block " + std::to_string(word[1]) + ")");
-    return B200_OK;
+    int wait[4];
+    if ((rc = read_status(s->h, wait))) return rc;
+    return wait_error(wait, "sharded gemm: a bounded wait ran out on the device");
 }
 
 }  // extern "C"

@@ -203,8 +203,9 @@ int b200_gemm_strided_batched(b200_handle* h, b200_stream stream, int transA, in
  *   offsets: groups + 1 ascending 32-bit integers in DEVICE memory with 0 <= offsets[0] and
  *   offsets[groups] <= N; equal neighbours are an empty group.  Read by the kernel, never by the host.
  *   Columns that belong to no group are not written.  Offsets that decrease or leave [0, N] write
- *   nothing and put id 110 into the device status word (b200_device_status; with
- *   B200_OPT_CHECK_ON_CALL the next call returns B200_INVALID_ARG).
+ *   nothing and are reported by b200_device_status as id 110, the number of groups as its detail (a wait that
+ *   ran out is reported first; with B200_OPT_CHECK_ON_CALL the next call returns B200_INVALID_ARG).  Other
+ *   products of the handle are not failed by it.
  *   groups <= 1024.  Types as in b200_gemm_ex; a column's result does not depend on its neighbours'
  *   values.  D may alias C exactly (same pointer, ld and type).
  * The tcgen05 kernel needs 16-byte aligned A and B, lda, ldb and stride_a multiples of 8 elements and
