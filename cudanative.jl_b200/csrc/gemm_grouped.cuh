@@ -433,7 +433,11 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         }
                     };
                     auto wait_tail = [&](int st) {  // the last k-block's foreign rows are zero
-                        const bool done = __all_sync(0xffffffffu, mbar_wait(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail));
+                        // of a pair, one CTA's rows were cleared by ordinary stores in the other CTA and are read from here
+                        bool here;
+                        if constexpr (kPair) here = mbar_wait_cluster(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail);
+                        else here = mbar_wait(tail_ready_bar(st), (tail_ph >> st) & 1u, wc, kWaitTail);
+                        const bool done = __all_sync(0xffffffffu, here);
                         tail_ph ^= 1u << st;
                         return done;
                     };
