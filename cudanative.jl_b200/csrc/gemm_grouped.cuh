@@ -104,6 +104,7 @@ struct GroupedCfg {
     using Epi = EpilogueCfg<kBN>;
     static constexpr int TABLE_BYTES = (kRaggedK ? 1 : 2) * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
+    static constexpr int SCAN_AT = 384;  // among them, behind the barriers: scratch of the groups' scan, a sum per warp
     static constexpr int RECV_BYTES = kSplit == 2 ? 128 * kSplitRow * 4 : kSplit == 4 ? 128 * kBN * 4 : 0;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - RECV_BYTES;
     static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
@@ -114,7 +115,7 @@ struct GroupedCfg {
     static_assert(kSplit != 4 || (kCtas == 1 && kBN == 64 && kSums == kBinary32), "four share K: one-CTA tiles, 16 columns each");
     static_assert(!kRaggedK || BN_LOCAL % 64 == 0, "MN-major B loads 64 columns per box");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
-    static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
+    static_assert(8 * NBARS + 8 <= SCAN_AT && SCAN_AT + THREADS / 32 * 8 <= BAR_BYTES, "barriers, scratch");
 };
 
 // Offsets into shared memory, checked and, for kTiles, with an exclusive scan of the tile columns per
@@ -255,9 +256,8 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
     griddep_launch_dependents();
     griddep_wait();
 
-    // the scan's scratch may lie in the first stage: nothing uses it yet
     const bool offsets_ok = load_groups<!kRaggedK, Cfg::THREADS>(p.offsets, p.groups, kRaggedK ? p.K : p.N, kBN, off, first,
-                                                   reinterpret_cast<unsigned long long*>(smem_gen));
+                                                   reinterpret_cast<unsigned long long*>(bar_gen + Cfg::SCAN_AT));
     if (!offsets_ok && threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
     const int tiles_m = p.raster.rows.d;
     const int num_units = !offsets_ok ? 0 : kRaggedK ? p.groups * p.tiles.d : first[p.groups] * tiles_m;
@@ -501,9 +501,9 @@ gemm_grouped_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     const int boxes = 2 + (inst_n(u) / kCtas + 63) / 64;  // A's two come first, B's follow
                     uint8_t* tile = smem_gen + st * Cfg::STAGE_BYTES;
                     for (int box = 0; box < boxes; ++box)
-                    for (int row = rem + lane / 8; row < end; row += 4)
-                        *reinterpret_cast<uint4*>(tile + box * 8192 + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async;" ::: "memory");
+                        for (int row = rem + lane / 8; row < end; row += 4)
+                            *reinterpret_cast<uint4*>(tile + box * 8192 + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) {
                         if constexpr (kPair) mbar_arrive_cluster(tail_ready_bar(st), 0);

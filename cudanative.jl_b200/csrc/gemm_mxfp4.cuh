@@ -63,6 +63,7 @@ struct MxCfg {
     using Epi = EpilogueCfg<kBN>;
     static constexpr int TABLE_BYTES = 3 * (kMaxGroups + 4) * 4;
     static constexpr int BAR_BYTES = 512;
+    static constexpr int SCAN_AT = 384;  // among them, behind the barriers: scratch of the groups' scan, a sum per warp
     static constexpr int RECV_BYTES = kSplit ? 128 * kSplitRow * 4 : 0;
     static constexpr int BUDGET = 227 * 1024 - 1024 - BAR_BYTES - TABLE_BYTES - RECV_BYTES;
     static constexpr int ACCS = kBN <= 192 ? 2 : 1;
@@ -77,7 +78,7 @@ struct MxCfg {
     static_assert(!kSplit || (kCtas == 1 && kBN <= 32), "split inner dimension: one-CTA tiles, one warp group");
     static_assert(USED_COLS <= 512, "tensor memory");
     static_assert(STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "shared memory");
-    static_assert(8 * NBARS + 8 <= BAR_BYTES, "barriers");
+    static_assert(8 * NBARS + 8 <= SCAN_AT && SCAN_AT + THREADS / 32 * 8 <= BAR_BYTES, "barriers, scratch");
     static_assert(kBN == 32 || kBN == 128 || kBN == 192 || kBN == 256, "a tile of columns begins on a multiple of 32 inside its scale tile");
 };
 
@@ -148,8 +149,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     griddep_launch_dependents();
     griddep_wait();
 
-    // the scan's scratch may lie in the first stage: nothing uses it yet
-    const bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<unsigned long long*>(smem_gen),
+    const bool offsets_ok = load_groups<true, Cfg::THREADS>(p.offsets, p.groups, p.N, kBN, off, first, reinterpret_cast<unsigned long long*>(bar_gen + Cfg::SCAN_AT),
                                                             kBN == 128 ? nullptr : first128);
     if (!offsets_ok && threadIdx.x == 0) report_bad_offsets(p.status, p.groups);
     const int num_units = offsets_ok ? first[p.groups] * p.raster.rows.d : 0;
