@@ -17,7 +17,7 @@ F16, F32, BF16 = 0, 1, 2
 MATRIX_A, MATRIX_B, ACCUMULATOR = 0, 1, 2
 LOWER_WARP, LOWER_TCGEN05 = 0, 1
 KERNEL_AUTO, KERNEL_TCGEN05, KERNEL_SIMPLE = 0, 1, 2
-STATUS_BAD_OFFSETS = 110  # device status word: a grouped product's offsets decrease or leave the matrix
+STATUS_BAD_OFFSETS = 110  # of device_status: a grouped call's offsets decrease or leave the matrix
 (OPT_FORCE_KERNEL, OPT_MAX_CTAS, OPT_WAIT_BUDGET_NS, OPT_TILE_N, OPT_SPLIT_K, OPT_CTA_PAIR,
  OPT_RASTER_GROUP, OPT_CHECK_ON_CALL, OPT_PDL, OPT_F16_ACCUMULATE) = range(10)
 SHARDED_GATED, SHARDED_NO_TRANSFER, SHARDED_NO_COMPUTE = 1, 2, 4

@@ -17,9 +17,10 @@
 //
 // C is read the same way: before it waits for the accumulator the warp brings the tile's lines of C into L2 and
 // asks for the first step's values, then for each next step's while one is stored (where the registers
-// allow it, kAhead).  32 groups of 2048 x 1408, 16384 columns, C and D Float32: 169 us; 184 us without the values
-// ahead, 203 us without the lines, 215 us with the lines of the next tile instead, 182 us with a ring of bulk copies of C
-// in shared memory, which took 48 KiB from the stages (132 against 138 us without a C).
+// allow it, kAhead).  32 groups of 2048 x 1408, 16384 columns, C and D Float32, loops of a few ms: 169 us (180-205 us in
+// blocks of 0.15 s); 184 us without the values ahead, 203 us without the lines, 215 us with the lines of the next tile
+// instead, 182 us with a ring of bulk copies of C in shared memory, which took 48 KiB from the stages (132 against 138 us
+// without a C).
 //
 // kPromoteKb: the tensor core adds into its accumulator without rounding to nearest; every step drops what
 // lies below the last place, which pulls sums towards zero in proportion to the number of steps (measured

@@ -20,8 +20,8 @@
 //             between the arrival of the tile and its use.
 //
 // Roles and barriers are those of gemm_sm100.cuh (warp 0 producer, warp 1 MMA issuer, warp 2 tensor
-// memory) with the epilogue of epilogue_sm100.cuh in warps 4-11; every wait is bounded.  Offsets that decrease or leave [0, total] are
-// reported in the device status word (kBadOffsets) and the launch writes nothing.
+// memory) with the epilogue of epilogue_sm100.cuh in warps 4-11; every wait is bounded.  Offsets that decrease or leave
+// [0, total] are reported (report_bad_offsets) and the launch writes nothing.
 #pragma once
 
 #include "epilogue_sm100.cuh"

@@ -61,7 +61,7 @@ int launch(const CUtensorMap (&tm)[4], const MxGemmParams& p, int grid, cudaStre
 }
 
 // Tile columns, by the mean length of the groups.  256 columns leave tensor memory for one accumulator: its
-// reading out is not hidden, nor is C read ahead.  192 have two.  Measured, 256 against 192: 8192 x 8192, K =
+// reading out is not hidden, nor is C read ahead.  192 have two.  Measured in turn, 256 against 192: 8192 x 8192, K =
 // 8192 210 / 250 us, K = 512 50 / 48 us; with a Float32 C, 8192 x 8192, K = 1024 118 / 111 us, K = 4096 149 / 160 us,
 // and where two rounds of tiles are all there is, 4100 x 1111, K = 4096 33 / 24 us.
 void pick_tile(const b200_handle* h, const MxProblem& g, int* tile_n, int* pair) {

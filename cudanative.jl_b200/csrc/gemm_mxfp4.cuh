@@ -277,7 +277,7 @@ gemm_mxfp4_tcgen05(const __grid_constant__ CUtensorMap tmA, const __grid_constan
                         }
                     };
                     // Two k-blocks a turn: waiting, looking ahead and the loop take as long as half a k-block's products
-                    // (8192^3: 204 us one by one, 187 us).
+                    // (8192^3, loops of a few ms: 204 us one by one, 187 us; 199-226 us in blocks of 0.15 s).
                     for (int kb = 0; kb < kb_total; kb += 2) {
                         const int s1 = s + 1 == STAGES ? 0 : s + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1, s3 = s2 + 1 == STAGES ? 0 : s2 + 1;
                         const uint32_t ph1 = ph ^ (s1 == 0), ph2 = ph1 ^ (s2 == 0), ph3 = ph2 ^ (s3 == 0);

@@ -66,8 +66,9 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t cta_r
 }
 
 // The same without release semantics for memory: for a signal that says only that this warp's tensor-memory
-// stores have completed (tcgen05.wait::st, tcgen05.fence::before_thread_sync).  A release at cluster scope
-// waits for all of the thread's memory operations, about 0.5 us.
+// loads or stores have completed (tcgen05.wait, tcgen05.fence::before_thread_sync; the waiting side has
+// tcgen05.fence::after_thread_sync).  Those two fences order tensor memory around the barrier, nothing else is handed
+// over.  A release at cluster scope waits for all of the thread's memory operations, about 0.5 us.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar, uint32_t cta_rank) {
     asm volatile(
         "{\n"

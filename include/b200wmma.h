@@ -115,7 +115,7 @@ int b200_get_option(b200_handle* h, int option, int64_t* value);
 
 /* After the stream has been synchronised: what the kernels of this handle last wrote into the
  * device status word.  code 0 = nothing; otherwise the id of the wait that ran out, the block
- * it was in and a detail word.  Clears the word.  Plays the role of the reference's polled
+ * it was in and a detail word, or 110 for group offsets that are none.  Clears what it reports.  Plays the role of the reference's polled
  * device exception flag (src/exceptions.jl:55-89, src/device/runtime.jl:18-31). */
 int b200_device_status(b200_handle* h, int* code, int* block, int* detail);
 
@@ -267,11 +267,11 @@ int b200_mxfp4_dequantize(b200_handle* h, b200_stream stream, int64_t K, int64_t
  * M x N column-major in any of the three types and at any alignment.  One weight matrix [out, in] and
  * tokens [tokens, in], stored row by row and quantised with trans = 0, give [tokens, out].  lda and ldb
  * count elements.  Products are exact, accumulation is binary32; the
- * tensor core truncates when it adds, so an accumulator takes at most 8192 products for a Float32 D and 65536
- * for a 16-bit one, and a longer sum adds several with rounding to nearest.  A block with scale 255 makes its row or
- * column of D NaN.  K > 0 unless M or N is 0.  D may alias C exactly (same pointer, ld and type).  There is
- * no simple kernel for 4-bit operands: alignment that the layout above rules out is refused.  The tile
- * options accept 128 and 256 columns (64 counts as 128); the split-K option is ignored. */
+ * tensor core truncates when it adds, so an accumulator takes at most 8192 products for a Float32 D and
+ * 65536 for a 16-bit one, and a longer sum adds several with rounding to nearest.  A block with scale 255
+ * makes its row or column of D NaN.  K > 0 unless M or N is 0.  D may alias C exactly (same pointer, ld and
+ * type).  There is no simple kernel for 4-bit operands: alignment that the layout above rules out is
+ * refused.  The tile options accept 128 and 256 columns (64 counts as 128); the split-K option is ignored. */
 int b200_gemm_mxfp4(b200_handle* h, b200_stream stream, int64_t M, int64_t N, int64_t K, float alpha,
                     const void* A, int64_t lda, const void* a_scales, const void* B, int64_t ldb,
                     const void* b_scales, float beta, const void* C, int64_t ldc, int c_type, void* D,

@@ -104,12 +104,13 @@ def test_the_right_types_reach_the_library(library, entry):
     assert len(library.calls) == 1
 
 
-@pytest.mark.parametrize("entry,operand", [(e, o) for e, (_, types) in ENTRIES.items() for o in types])
-@pytest.mark.parametrize("wrong", [h16, f32, b16, u8, i32, torch.int64, torch.float64], ids=str)
+ALL = [h16, f32, b16, u8, i32, torch.int64, torch.float64]
+WRONG = [(e, o, w) for e, (_, types) in ENTRIES.items() for o, t in types.items() for w in ALL if w not in FREE.get((e, o), (t,))]
+
+
+@pytest.mark.parametrize("entry,operand,wrong", WRONG, ids=str)
 def test_another_type_is_refused(library, entry, operand, wrong):
     call, types = ENTRIES[entry]
-    if wrong in FREE.get((entry, operand), (types[operand],)):
-        pytest.skip("a type it reads")
     with pytest.raises(TypeError):
         call({**{k: Tensor(t) for k, t in types.items()}, operand: Tensor(wrong)})
     assert not library.calls
